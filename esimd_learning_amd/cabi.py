@@ -55,6 +55,13 @@ SIGNATURES = {
     "cek_gemv_fp8_gelu_and_mul_rs": (_i, [_p, _p, _p, _p, _p, _i64, _f, _i64, _i64, _i64, _i, _i, _i, _p]),
     "cek_gemv_fp8_qk_norm_rope_rs": (_i, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _f, _f, _i, _p, _p, _p,
                                           _i64, _f, _i64, _i64, _i64, _i, _i, _i, _p]),
+    "cek_kv_block_tables": (_i, [_p, _p, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p,
+                                 _p]),
+    "cek_kv4_cache_write": (_i, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _p]),
+    "cek_kv4_cache_read": (_i, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _p]),
+    "cek_kv4_attention_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "cek_kv4_attention": (_i, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                               _i64, _f, _i64, _i64, _i64, _i, _p, _i64, _p]),
     "cek_hbm_read_probe": (_i, [_p, _i64, _p, _p]),
 }
 

@@ -1,0 +1,82 @@
+// cek_kv4.h -- layout and number format of the 4-bit key/value cache, shared by
+// the kernels that write, read and attend over it.
+//
+// The bytes of one (block, kv head), bs tokens of hd values:
+//   K codes   [bs][hd / 2]          value d of a token: nibble d % 2 of byte d / 2
+//   V codes   [bs / 4][hd / 4][4]   16-bit words: values 4u .. 4u + 3 of token 4t + i
+//                                   are nibbles 0 .. 3 of word [t][u][i]
+//   K params  [bs]                  bf16 step s (low half), bf16 centre m (high half)
+//   V params  [bs]
+// and a value is m + s (c - 7.5), c = 0 .. 15.  K rows are contiguous because
+// the score product contracts over a row; V words hold four tokens side by side
+// because the output product contracts over tokens: either way a 32-bit load
+// unpacks by masks alone into the pairs an MFMA operand wants.
+#pragma once
+
+#include "cek_common.h"
+
+namespace cek {
+
+struct Kv4Dims {
+  int64_t block_stride;  // bytes from a block to the next
+  int num_blocks, n_kv, bs_log2;
+};
+
+// Byte offsets inside one (block, head); hd / 2 bytes a token and part.
+__host__ __device__ inline int kv4_v_codes(int bs, int hd) { return bs * (hd / 2); }
+__host__ __device__ inline int kv4_k_params(int bs, int hd) { return bs * hd; }
+__host__ __device__ inline int kv4_v_params(int bs, int hd) { return bs * hd + 4 * bs; }
+__host__ __device__ inline int kv4_head_bytes(int bs, int hd) { return bs * (hd + 8); }
+
+__device__ inline float kv4_step(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ inline float kv4_centre(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
+
+// A row's parameters from its extremes.  m = bf16(lo / 2 + hi / 2), s = bf16 of
+// the larger distance from m / 7.5, so that the codes reach both ends whatever
+// m's rounding did; steps below 2^-100 (whose reciprocal would leave the fp32
+// range) are kept as 0: such a row is its centre.  A row with a value that is
+// not finite has m = NaN, s = 0: it reads as NaN throughout.
+constexpr float kKv4MinStep = 0x1p-100f;
+__device__ inline uint32_t kv4_params(float lo, float hi, bool finite) {
+  if (!finite) return 0x7FC00000u;
+  const float m = BF16::to_f32(BF16::from_f32(f32_round(0.5f * lo) + f32_round(0.5f * hi)));
+  const float a = fmaxf(hi - m, m - lo);
+  uint32_t s = BF16::from_f32(a / 7.5f);
+  if (__uint_as_float(s << 16) < kKv4MinStep) s = 0;
+  return s | (__float_as_uint(m) & 0xFFFF0000u);
+}
+
+// The code of x: the nearest step, ties to even codes, all operations in fp32
+// and rounded one by one: rint((x - m) / s + 7.5) within 0 .. 15.  d = quant_div
+// of the row's step; a row of step 0 has code 8.
+__device__ inline uint32_t kv4_code(float x, float m, QuantDiv d, bool has_step) {
+  const float v = f32_round(x - m);
+  const float q0 = f32_round(v * d.r);
+  const float q = fmaf(fmaf(-q0, d.s, v), d.r, q0);
+  const float c = fminf(fmaxf(rintf(f32_round(q) + 7.5f), 0.0f), 15.0f);
+  return has_step ? (uint32_t)c : 8u;
+}
+
+__device__ inline float kv4_value(uint32_t code, uint32_t p) {
+  return f32_round(kv4_step(p) * ((float)code - 7.5f)) + kv4_centre(p);  // the product is exact
+}
+
+// The arguments that the cache's operators share.
+inline int kv4_dims(int64_t n_kv, int64_t hd, int64_t bs, int64_t num_blocks, int64_t block_stride, Kv4Dims& dm) {
+  if (n_kv <= 0 || n_kv > 4096 || num_blocks <= 0 || num_blocks > INT32_MAX) return CEK_ERR_INVALID;
+  if (hd != 64 && hd != 128 && hd != 256) return CEK_ERR_UNSUPPORTED;
+  if (bs < 16 || bs > 256 || (bs & (bs - 1))) return CEK_ERR_UNSUPPORTED;
+  if (block_stride % 16 || block_stride < n_kv * kv4_head_bytes((int)bs, (int)hd)) return CEK_ERR_INVALID;
+  dm = Kv4Dims{block_stride, (int)num_blocks, (int)n_kv, __builtin_ctzll((unsigned long long)bs)};
+  return CEK_OK;
+}
+
+// CALL(64), CALL(128) or CALL(256) for the head size hd.
+#define CEK_KV4_HD(CALL)             \
+  do {                               \
+    if (hd == 64) CALL(64);          \
+    else if (hd == 128) CALL(128);   \
+    else CALL(256);                  \
+  } while (0)
+
+}  // namespace cek

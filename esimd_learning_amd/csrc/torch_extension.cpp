@@ -81,6 +81,22 @@ TORCH_LIBRARY(custom_esimd_kernels_vllm, m) {
         "Tensor q_weight, Tensor k_weight, Tensor positions, int n_q, int n_k, float eps, float theta, "
         "bool is_neox, Tensor(b!) counters, Tensor row_ss, float row_eps, Tensor(c!)? q_out=None) -> ()");
   m.impl("esimd_gemv_fp8_qk_norm_rope_rs", c10::DispatchKey::CUDA, &esimd_gemv_fp8_qk_norm_rope_rs);
+
+  m.def("esimd_kv_block_tables(Tensor(a!) kv_lens, Tensor keep_lens, Tensor q_lens, int block_size, "
+        "Tensor(b!) free_ring, Tensor(c!) ring_state, Tensor(d!) block_tables, Tensor(a!) kv_lens_out, "
+        "Tensor(c!) ring_state_out, Tensor(e!) cu_q, Tensor(f!) slot_mapping, Tensor(g!) positions, "
+        "Tensor(h!) status) -> ()");
+  m.impl("esimd_kv_block_tables", c10::DispatchKey::CUDA, &esimd_kv_block_tables);
+
+  m.def("esimd_kv4_cache_write(Tensor k, Tensor v, Tensor(a!) kv_cache, Tensor slot_mapping) -> ()");
+  m.impl("esimd_kv4_cache_write", c10::DispatchKey::CUDA, &esimd_kv4_cache_write);
+
+  m.def("esimd_kv4_cache_read(Tensor kv_cache, Tensor slot_mapping, Tensor(a!) k, Tensor(b!) v) -> ()");
+  m.impl("esimd_kv4_cache_read", c10::DispatchKey::CUDA, &esimd_kv4_cache_read);
+
+  m.def("esimd_kv4_attention(Tensor q, Tensor kv_cache, Tensor block_tables, Tensor kv_lens, Tensor cu_q, "
+        "Tensor(a!) out, float scale, int max_q_len=0, int max_kv_len=0, int window=0) -> ()");
+  m.impl("esimd_kv4_attention", c10::DispatchKey::CUDA, &esimd_kv4_attention);
 }
 
 PyMODINIT_FUNC PyInit_custom_esimd_kernels() {

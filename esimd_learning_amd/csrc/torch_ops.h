@@ -76,6 +76,17 @@ void esimd_gemv_fp8_qk_norm_rope_rs(at::Tensor input, at::Tensor weight, at::Ten
                                     int64_t n_k, double eps, double theta, bool is_neox, at::Tensor counters,
                                     at::Tensor row_ss, double row_eps, c10::optional<at::Tensor> q_out);
 
+// The 4-bit key/value cache: block tables and slots of a step, writes, reads
+// and attention (cek_kv4.h).
+void esimd_kv_block_tables(at::Tensor kv_lens, at::Tensor keep_lens, at::Tensor q_lens, int64_t block_size,
+                           at::Tensor free_ring, at::Tensor ring_state, at::Tensor block_tables, at::Tensor kv_lens_out,
+                           at::Tensor ring_state_out, at::Tensor cu_q, at::Tensor slot_mapping, at::Tensor positions,
+                           at::Tensor status);
+void esimd_kv4_cache_write(at::Tensor k, at::Tensor v, at::Tensor kv_cache, at::Tensor slot_mapping);
+void esimd_kv4_cache_read(at::Tensor kv_cache, at::Tensor slot_mapping, at::Tensor k, at::Tensor v);
+void esimd_kv4_attention(at::Tensor q, at::Tensor kv_cache, at::Tensor block_tables, at::Tensor kv_lens, at::Tensor cu_q,
+                         at::Tensor out, double scale, int64_t max_q_len, int64_t max_kv_len, int64_t window);
+
 at::Tensor esimd_gemm_fp8_a8w8(at::Tensor a, at::Tensor a_scale, at::Tensor b, at::Tensor b_scale,
                                at::Tensor output);
 

@@ -34,6 +34,12 @@ from custom_esimd_kernels_vllm.ops import (  # noqa: F401
     esimd_gemv_fp8_pern_rs,
     esimd_gemv_fp8_gelu_and_mul_rs,
     esimd_gemv_fp8_qk_norm_rope_rs,
+    kv4_cache,
+    kv_free_ring,
+    esimd_kv_block_tables,
+    esimd_kv4_cache_write,
+    esimd_kv4_cache_read,
+    esimd_kv4_attention,
     esimd_gemm_fp8_a8w8,
     esimd_gemm_fp8_a8w8_gelu_and_mul,
 )

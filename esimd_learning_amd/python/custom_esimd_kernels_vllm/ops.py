@@ -235,6 +235,102 @@ def esimd_gemv_fp8_qk_norm_rope_rs(
                                         n_k, eps, theta, is_neox, counters, row_ss, row_eps, q_out)
 
 
+def kv4_cache(num_blocks, n_kv, block_size, head_dim, device) -> torch.Tensor:
+    """A 4-bit key/value cache, uint8 [num_blocks, n_kv, block_size, head_dim + 8].
+
+    One (block, kv head) of bs tokens holds, in this order, the K codes
+    [bs, head_dim / 2] (value d: nibble d % 2 of byte d / 2), the V codes
+    [bs / 4, head_dim / 4, 4] in 16-bit words (values 4u .. 4u + 3 of token
+    4t + i are the nibbles of word [t, u, i]), and the K and the V parameters
+    [bs], a bf16 step s and a bf16 centre m each; a value is m + s (c - 7.5).
+    block_size: a power of two from 16 to 256; head_dim 64, 128 or 256.  Not
+    initialised: what lies behind a request's length is never used."""
+    return torch.empty(num_blocks, n_kv, block_size, head_dim + 8, dtype=torch.uint8, device=device)
+
+
+def kv_free_ring(num_blocks, device):
+    """(free_ring, ring_state) with all blocks free, in ascending order."""
+    ring = torch.arange(num_blocks, dtype=torch.int32, device=device)
+    return ring, torch.tensor([0, num_blocks], dtype=torch.int32, device=device)
+
+
+def esimd_kv_block_tables(
+    kv_lens: torch.Tensor, keep_lens: torch.Tensor, q_lens: torch.Tensor, block_size: int,
+    free_ring: torch.Tensor, ring_state: torch.Tensor, block_tables: torch.Tensor,
+    kv_lens_out: torch.Tensor, ring_state_out: torch.Tensor, cu_q: torch.Tensor,
+    slot_mapping: torch.Tensor, positions: torch.Tensor, status: torch.Tensor,
+) -> None:
+    """Block tables, slots and positions of one step, from the lengths alone.
+
+    Request r holds kv_lens[r] cached tokens in the first ceil(kv_lens /
+    block_size) entries of block_tables[r].  keep_lens[r] of them stay (fewer
+    after rejected drafts, 0 for a request that ended or starts over) and
+    q_lens[r] new ones follow.  Blocks it lacks are taken from the free ring,
+    blocks it no longer needs are returned to it, both in request order and
+    ascending in the table; a block returned by a call can be taken from the
+    next call on.  free_ring int32 [num_blocks] with ring_state int32 [2] =
+    (place of the first free block, how many are free): ``kv_free_ring``.
+
+    Written: block_tables and free_ring (the changed entries), kv_lens_out =
+    keep + q, ring_state_out, cu_q int32 [R + 1] (offsets of the requests' new
+    tokens), slot_mapping and positions int64 [T] of the new tokens in order
+    (behind the last one: -1 and 0), and status int32 [R]: 0; 1 the blocks up
+    to and with this request's are more than are free; 2 block_tables is too
+    narrow for it; 3 the new tokens up to and with its own are more than T.  A
+    request with status != 0 gets no new token (its q counts as 0) and takes
+    no block, but returns what lies behind keep_lens.  Status 1 and 3 count the
+    wishes of all requests before, refused ones too; a request that needs no
+    new block is never refused for one.
+
+    kv_lens_out may be kv_lens and ring_state_out ring_state (a captured step
+    replayed); no other two may share memory.  Lengths are taken within 0 ..
+    the table's reach, keep_lens within 0 .. kv_lens.  At most 4096 requests."""
+    _ops.esimd_kv_block_tables(kv_lens, keep_lens, q_lens, block_size, free_ring, ring_state, block_tables, kv_lens_out,
+                               ring_state_out, cu_q, slot_mapping, positions, status)
+
+
+def esimd_kv4_cache_write(
+    k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
+) -> None:
+    """Quantise k and v rows to 4 bits into kv_cache at their slots.
+
+    k, v [T, n_kv, head_dim] or [T, n_kv * head_dim], fp16 or bf16, any row
+    stride; slot_mapping int64 [T], block * block_size + token.  Rows whose slot
+    lies outside the cache (-1: padding) are skipped.  A slot may occur once.
+    Per row and head: m = bf16((min + max) / 2), s = bf16(max(max - m, m - min)
+    / 7.5), c = clamp(rint((x - m) / s + 7.5), 0, 15); a row with a value that
+    is not finite reads back as NaN throughout."""
+    _ops.esimd_kv4_cache_write(k, v, kv_cache, slot_mapping)
+
+
+def esimd_kv4_cache_read(
+    kv_cache: torch.Tensor, slot_mapping: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+) -> None:
+    """The cached rows of slot_mapping [T] into k and v [T, n_kv, head_dim] (or
+    [T, n_kv * head_dim]), fp16 or bf16: m + s (c - 7.5), rounded once.  Rows
+    whose slot lies outside the cache are zero."""
+    _ops.esimd_kv4_cache_read(kv_cache, slot_mapping, k, v)
+
+
+def esimd_kv4_attention(
+    q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor, kv_lens: torch.Tensor,
+    cu_q: torch.Tensor, out: torch.Tensor, scale: float, max_q_len: int = 0, max_kv_len: int = 0,
+    window: int = 0,
+) -> None:
+    """Causal attention of new tokens over the cache, which holds theirs too.
+
+    q, out [T, n_q, head_dim] or [T, n_q * head_dim] (any row strides); rows
+    cu_q[r] .. cu_q[r + 1] - 1 are the last tokens of request r, whose kv_lens[r]
+    keys and values lie in the blocks of block_tables[r].  Row at position p
+    sees keys 0 .. p, with window > 0 keys p - window + 1 .. p; query head h
+    reads kv head h / (n_q / n_kv).  out = sum softmax(scale q k) v; rows without
+    a key (kv_lens 0) are zero; rows of q before cu_q[0] or behind cu_q[R] are
+    left as they were.  Tokens whose table entry lies outside the cache count
+    as absent.  max_q_len and max_kv_len, the longest of the batch (0: not
+    known), choose the kernels; wrong ones cost time, not results."""
+    _ops.esimd_kv4_attention(q, kv_cache, block_tables, kv_lens, cu_q, out, scale, max_q_len, max_kv_len, window)
+
+
 def esimd_gemm_fp8_a8w8(
     a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
     output: torch.Tensor,

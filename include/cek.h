@@ -370,6 +370,65 @@ int cek_qk_norm_rope(void* q, void* k, const void* qw, const void* kw, const int
                      int is_neox, int io_dtype, void* stream);
 
 /*
+ * The 4-bit key/value cache (NEW, all of it).  num_blocks blocks, block_stride
+ * bytes apart (a multiple of 16), each [n_kv][block_size][head_dim + 8] bytes;
+ * the bytes of one (block, head), bs tokens of hd values:
+ *   K codes  [bs][hd / 2]         value d: nibble d % 2 of byte d / 2
+ *   V codes  [bs / 4][hd / 4][4]  16-bit words, values 4u .. 4u + 3 of token 4t + i
+ *                                 in the nibbles of word [t][u][i]
+ *   K params [bs], V params [bs]  bf16 step s, bf16 centre m
+ * value = m + s (c - 7.5).  head_dim 64, 128 or 256, block_size a power of two
+ * from 16 to 256 (CEK_ERR_UNSUPPORTED otherwise); a slot is block * block_size +
+ * token.
+ *
+ * cek_kv_block_tables: a step's bookkeeping.  Of kv_lens[r] cached tokens
+ * keep_lens[r] stay and q_lens[r] follow; blocks that request r < R lacks are
+ * taken from the ring free_ring [num_blocks] (ring_state: place of the first
+ * free block, count), blocks it no longer needs go back behind its last one,
+ * in request order.  Writes the changed entries of block_tables (rows of
+ * max_blocks, table_stride apart) and free_ring, kv_lens_out, ring_state_out,
+ * cu_q [R + 1], slot_mapping and positions [T] (behind the last new token -1
+ * and 0) and status [R] (0, or 1 not enough free blocks, 2 table too narrow, 3
+ * more than T tokens: that request gets no token and takes no block).
+ * kv_lens_out may be kv_lens and ring_state_out ring_state; other arrays must
+ * not overlap.  R <= 4096.
+ *
+ * cek_kv4_cache_write: k, v rows (strides in elements) quantised into the cache,
+ * m = bf16((min + max) / 2), s = bf16(max(max - m, m - min) / 7.5), c =
+ * clamp(rint((x - m) / s + 7.5), 0, 15).  Rows with a slot outside the cache are
+ * skipped; a slot may occur once.  cek_kv4_cache_read: the inverse; zeros for
+ * rows with a slot outside the cache.
+ *
+ * cek_kv4_attention: out rows cu_q[r] .. cu_q[r + 1] - 1 = attention of the same
+ * q rows, the last tokens of request r, over its kv_lens[r] cached tokens; the
+ * row at position p sees keys 0 .. p (window > 0: p - window + 1 .. p).  Rows
+ * without a key are zero, rows outside cu_q[0] .. cu_q[R] left as they were.
+ * Tokens in blocks outside the cache count as absent.  max_q_len and max_kv_len
+ * (0: not known) choose the kernels and never change results beyond the order
+ * of sums.  workspace: cek_kv4_attention_workspace_size bytes for the same
+ * arguments, 16-byte aligned, no initialisation; with less the call does not
+ * split the keys.
+ */
+int cek_kv_block_tables(const int32_t* kv_lens, const int32_t* keep_lens, const int32_t* q_lens, int64_t R,
+                        int64_t block_size, int32_t* free_ring, int64_t num_blocks, const int32_t* ring_state,
+                        int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* kv_lens_out,
+                        int32_t* ring_state_out, int32_t* cu_q, int64_t* slot_mapping, int64_t* positions, int64_t T,
+                        int32_t* status, void* stream);
+int cek_kv4_cache_write(const void* k, const void* v, void* cache, const int64_t* slot_mapping, int64_t T, int64_t n_kv,
+                        int64_t head_dim, int64_t block_size, int64_t num_blocks, int64_t k_stride, int64_t v_stride,
+                        int64_t block_stride, int io_dtype, void* stream);
+int cek_kv4_cache_read(const void* cache, const int64_t* slot_mapping, void* k, void* v, int64_t T, int64_t n_kv,
+                       int64_t head_dim, int64_t block_size, int64_t num_blocks, int64_t k_stride, int64_t v_stride,
+                       int64_t block_stride, int io_dtype, void* stream);
+int64_t cek_kv4_attention_workspace_size(int64_t T, int64_t R, int64_t n_q, int64_t n_kv, int64_t head_dim,
+                                         int64_t max_q_len, int64_t max_kv_len);
+int cek_kv4_attention(const void* q, const void* cache, const int32_t* block_tables, const int32_t* kv_lens,
+                      const int32_t* cu_q, void* out, int64_t T, int64_t R, int64_t n_q, int64_t n_kv, int64_t head_dim,
+                      int64_t block_size, int64_t num_blocks, int64_t q_stride, int64_t out_stride, int64_t block_stride,
+                      int64_t table_stride, int64_t max_blocks, float scale, int64_t max_q_len, int64_t max_kv_len,
+                      int64_t window, int io_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Measurement utility, no counterpart in the reference: reads `bytes` bytes
  * of buf (16-byte aligned, bytes % 16 == 0) once with 16-byte non-temporal
  * loads.  With sink != NULL it writes the XOR of each of its 1024

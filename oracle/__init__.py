@@ -18,4 +18,4 @@ itself) is listed per module in its docstring; the tests that perform the
 pins live in ``tests/test_oracle_fp8.py`` (codec) and ``tests/test_oracle_ops.py`` (ops).
 """
 
-from . import fp8, gemv, norm, act, gemm, layer  # noqa: F401
+from . import fp8, gemv, norm, act, gemm, kv4, layer  # noqa: F401
