@@ -65,6 +65,8 @@ struct Kv4Work {
   int r, q0, rows, kv, n_new, lo, tile, chunk, nch, item0, keys;
 };
 
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 __device__ inline int wave_scan_incl(int x) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -127,8 +129,9 @@ __device__ inline bool kv4_find_work(const Kv4AttnArgs& a, int item, Kv4Work& w)
       w.nch = get(nch);
       const int t = get(tiles);
       w.item0 = get(incl) - t * w.nch;
-      w.tile = t - 1 - (item - w.item0) / w.nch;  // the last rows, which see most keys, first
-      w.chunk = (item - w.item0) % w.nch;
+      const int at_tile = uniform((item - w.item0) / w.nch);
+      w.tile = t - 1 - at_tile;  // the last rows, which see most keys, first
+      w.chunk = item - w.item0 - at_tile * w.nch;
       w.keys = C;
       return true;
     }
@@ -137,6 +140,9 @@ __device__ inline bool kv4_find_work(const Kv4AttnArgs& a, int item, Kv4Work& w)
   return false;
 }
 
+// Parameters of 16 tokens that do not exist.
+__device__ const uint8_t kv4_zeros[64] __attribute__((aligned(16))) = {};
+
 __device__ inline uint32_t pack_h2(float a, float b) {
   return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});
 }
@@ -144,7 +150,7 @@ __device__ inline uint32_t pack_h2(float a, float b) {
 // KVSPLIT: the workgroup's four waves share QT x 16 rows and take every fourth 32
 // tokens each; else each wave has QT x 16 rows of its own and all the tokens.
 template <typename T, int HD, int QT, bool KVSPLIT>
-__global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
   constexpr int ND = HD / 32;                    // 32-bit words per lane, part and 16 tokens
   constexpr int NP = HD >= 128 ? HD / 128 : 1;   // parts of a row: 128 values, or 64
   constexpr int NH = HD >= 128 ? 2 : 1;          // runs of four values per lane and part
@@ -156,7 +162,7 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
 
   Kv4Work w;
   if (!kv4_find_work<BR>(a, blockIdx.x, w)) return;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.y;
   const int bs = 1 << a.dm.bs_log2;
@@ -180,11 +186,11 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
     const bool real = rr < w.rows;
     const int t = rr / a.group, h = kvh * a.group + rr % a.group;
     const uint16_t* src = a.q + (int64_t)(w.q0 + (real ? t : 0)) * a.q_stride + (int64_t)(real ? h : 0) * HD;
-    pos[i] = real ? w.kv - w.n_new + t : INT32_MAX;
+    pos[i] = real ? w.kv - w.n_new + t : INT32_MAX - 1;
     if (row0 + i * 16 < w.rows) {
       // uniform: rows are in order of position
-      pmin = min(pmin, w.kv - w.n_new + (row0 + i * 16) / a.group);
-      pmax = max(pmax, w.kv - w.n_new + (min(row0 + i * 16 + 16, w.rows) - 1) / a.group);
+      pmin = uniform(min(pmin, w.kv - w.n_new + (row0 + i * 16) / a.group));
+      pmax = uniform(max(pmax, w.kv - w.n_new + (min(row0 + i * 16 + 16, w.rows) - 1) / a.group));
     }
     uint32_t raw[ND][4];
 #pragma unroll
@@ -234,10 +240,11 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
   }
 
   // ---- the range of keys ----
+  const int window = a.window > 0 ? a.window : INT32_MAX;  // pos - window stays in range
   const int t_lo = a.window > 0 ? max(0, pmin - a.window + 1) & ~31 : 0;
-  int begin = w.nch > 1 ? max(t_lo, w.lo + w.chunk * w.keys) : t_lo;
-  int end = w.nch > 1 ? (int)min((int64_t)pmax + 1, (int64_t)w.lo + ((int64_t)w.chunk + 1) * w.keys) : pmax + 1;
-  if (KVSPLIT) begin += 32 * wave;
+  const int begin = uniform((w.nch > 1 ? max(t_lo, w.lo + w.chunk * w.keys) : t_lo) + (KVSPLIT ? 32 * wave : 0));
+  const int end = uniform(
+      w.nch > 1 ? (int)min((int64_t)pmax + 1, (int64_t)w.lo + ((int64_t)w.chunk + 1) * w.keys) : pmax + 1);
   constexpr int STEP = KVSPLIT ? 32 * kAttnWaves : 32;
 
   f4 o[QT][NP][NH][4];
@@ -254,154 +261,197 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
     for (int x = 0; x < NP * NH * 4; ++x) o[i][x / (NH * 4)][x / 4 % NH][x % 4] = f4{0.f, 0.f, 0.f, 0.f};
   }
 
-  struct Tile {
-    uint32_t k[2][ND], v[2][ND];
-    u4 kp[2], vp[2];
-    bool bad[2];
-  };
   const uint8_t* head = a.cache + (int64_t)kvh * kv4_head_bytes(bs, HD);
-  const int k_lane = c * (HD / 2) + g * (PW / 8);
-  const int v_lane = kv4_v_codes(bs, HD) + g * HD * 2 + c * (PW / 8);
-  const int kp_lane = kv4_k_params(bs, HD) + 16 * g;
-  const int vp_lane = kv4_v_params(bs, HD) + 16 * g;
+  const uint32_t k_lane = c * (HD / 2) + g * (PW / 8);
+  const uint32_t v_lane = kv4_v_codes(bs, HD) + g * HD * 2 + c * (PW / 8);
+  const uint32_t kp_lane = kv4_k_params(bs, HD) + 16 * g;
+  const uint32_t vp_lane = kv4_v_params(bs, HD) + 16 * g;
   const const_i32 table = (const_i32)(uintptr_t)(a.tables + (int64_t)w.r * a.table_stride);
 
   struct Blocks { int b[2]; };
+  // the blocks of 32 tokens; behind the last key (a half of them may lie there) none
   auto blocks_of = [&](int t0) {
     Blocks x;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) x.b[s] = t0 + 16 * s < w.kv ? table[(t0 + 16 * s) >> a.dm.bs_log2] : -1;
+    x.b[0] = uniform(table[t0 >> a.dm.bs_log2]);
+    x.b[1] = uniform(table[min(t0 + 16, w.kv - 1) >> a.dm.bs_log2]);
+    if (t0 + 16 >= w.kv) x.b[1] = -1;
     return x;
   };
-  auto load = [&](int t0, const Blocks& x, Tile& y) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int b = x.b[s];
-      y.bad[s] = b < 0 || b >= a.dm.num_blocks;
-      const int tok = (t0 + 16 * s) & (bs - 1);
-      const uint8_t* base = head + (int64_t)(y.bad[s] ? 0 : b) * a.dm.block_stride;
+  // A block outside the cache holds no token: block 0 is read in its place.
+  auto at_block = [&](int t0, const Blocks& x, int i, int& tok) {
+    const int b = x.b[i];
+    tok = (t0 + 16 * i) & (bs - 1);
+    return head + (int64_t)(b < 0 || b >= a.dm.num_blocks ? 0 : b) * a.dm.block_stride;
+  };
+  auto load_codes = [&](const uint8_t* base, uint32_t at, uint32_t (&to)[ND], uint32_t part) {
+    if constexpr (HD == 64) {
+      const uint2 x = *reinterpret_cast<const uint2*>(base + at);
+      to[0] = x.x, to[1] = x.y;
+    } else {
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        if constexpr (HD == 64) {
-          const uint2 kk = *reinterpret_cast<const uint2*>(base + tok * (HD / 2) + k_lane);
-          const uint2 vv = *reinterpret_cast<const uint2*>(base + tok * (HD / 2) + v_lane);
-          y.k[s][0] = kk.x, y.k[s][1] = kk.y, y.v[s][0] = vv.x, y.v[s][1] = vv.y;
-        } else {
-          // a part of 128 values: 64 bytes of a K row, 256 of four tokens of V
-          const u4 kk = load_u4(base + tok * (HD / 2) + k_lane + p * (PW / 2));
-          const u4 vv = load_u4(base + tok * (HD / 2) + v_lane + p * (PW * 2));
+        const u4 x = load_u4(base + p * part + at);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y.k[s][4 * p + e] = kk[e], y.v[s][4 * p + e] = vv[e];
-        }
+        for (int e = 0; e < 4; ++e) to[4 * p + e] = x[e];
       }
-      y.kp[s] = load_u4(base + 4 * tok + kp_lane);
-      y.vp[s] = load_u4(base + 4 * tok + vp_lane);
+    }
+  };
+  uint32_t kc[2][ND], vc[2][ND];  // the codes of 32 tokens, 16 and 16
+  u4 kp[2], vp[2];                // their parameters, of tokens 4 g ..
+  float none[2];                  // 0, or -infinity where the block lies outside the cache
+  auto load_k = [&](int t0, const Blocks& x) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int tok;
+      const uint8_t* base = at_block(t0, x, i, tok);
+      load_codes(base + tok * (HD / 2), k_lane, kc[i], PW / 2);  // 64 bytes of a row and part of 128 values
+    }
+  };
+  auto load_v = [&](int t0, const Blocks& x) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int tok;
+      const uint8_t* base = at_block(t0, x, i, tok);
+      load_codes(base + tok * (HD / 2), v_lane, vc[i], PW * 2);  // 256 bytes of four tokens and part
+    }
+  };
+  auto load_params = [&](int t0, const Blocks& x) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int tok;
+      const uint8_t* base = at_block(t0, x, i, tok) + 4 * tok;
+      const bool out = x.b[i] < 0 || x.b[i] >= a.dm.num_blocks;
+      // tokens that do not exist have parameters 0, whatever lies in block 0
+      kp[i] = load_u4(out ? kv4_zeros + 16 * g : base + kp_lane);
+      vp[i] = load_u4(out ? kv4_zeros + 16 * g : base + vp_lane);
+      none[i] = out ? -INFINITY : 0.f;
     }
   };
 
-  auto step32 = [&](int t0, Tile& y, auto mask) {
+  auto sees = [&](int i, int t0, int h, int e) {  // row c of tile i the token 16 h + 4 g + e at t0
+    const int t = t0 + 16 * h + 4 * g + e;
+    return (t <= pos[i]) & (t < end) & (t > pos[i] - window);  // no branches
+  };
+
+  // Scores of 32 tokens: x (exponents / qmul), their maxima xm and that of the V steps.
+  float x[QT][2][4], xm[QT], top;
+  auto scores = [&](int t0, auto mask) {
     constexpr bool masked = decltype(mask)::value;
     if constexpr (masked) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (y.bad[s] || t0 + 16 * s + 4 * g + e >= end) y.kp[s][e] = y.vp[s][e] = 0;  // no token: whatever lies there
+        for (int e = 0; e < 4; ++e) {
+          const bool out = t0 + 16 * h + 4 * g + e >= end;  // no token: whatever lies there
+          kp[h][e] = out ? 0u : kp[h][e];
+          vp[h][e] = out ? 0u : vp[h][e];
+        }
     }
-    // S^T: tokens 16 s + 4 g + e of row c
+    // S^T: tokens 16 h + 4 g + e of row c
     f4 acc[QT][2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int i = 0; i < QT; ++i) acc[i][s] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < QT; ++i) acc[i][h] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int n = 0; n < ND; ++n) {
-        const uint32_t x = y.k[s][n], x8 = x >> 8;
-        const u4 f = u4{x & 0x000F000Fu, x & 0x00F000F0u, x8 & 0x000F000Fu, x8 & 0x00F000F0u};
+        const uint32_t y = kc[h][n], y8 = y >> 8;
+        const u4 f = u4{y & 0x000F000Fu, y & 0x00F000F0u, y8 & 0x000F000Fu, y8 & 0x00F000F0u};
 #pragma unroll
-        for (int i = 0; i < QT; ++i) acc[i][s] = mfma16x16x32<F16>(f, qf[i][n], acc[i][s]);
+        for (int i = 0; i < QT; ++i) acc[i][h] = mfma16x16x32<F16>(f, qf[i][n], acc[i][h]);
       }
     }
-    float sk[2][4], mk[2][4], sv[2][4], mv[2][4], top = -1.f;
+    top = -1.f;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int i = 0; i < QT; ++i) xm[i] = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float xh[QT];
+#pragma unroll
+      for (int i = 0; i < QT; ++i) xh[i] = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        sk[s][e] = kv4_step(y.kp[s][e]);
-        mk[s][e] = fmaf(-7.5f, sk[s][e], kv4_centre(y.kp[s][e]));
-        sv[s][e] = kv4_step(y.vp[s][e]);
-        mv[s][e] = kv4_centre(y.vp[s][e]);
-        top = fmaxf(top, sv[s][e]);
+        const float sk = kv4_step(kp[h][e]), mk = fmaf(-7.5f, sk, kv4_centre(kp[h][e]));
+        top = fmaxf(top, kv4_step(vp[h][e]));
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+          x[i][h][e] = fmaf(sk, acc[i][h][e], mk * qsum[i]);
+          if constexpr (masked) x[i][h][e] = sees(i, t0, h, e) ? x[i][h][e] : -INFINITY;
+          xh[i] = fmaxf(xh[i], x[i][h][e]);
+        }
       }
-    float x[QT][2][4], xm[QT];
-    bool ok[QT][2][4];
-    bool grow = top > sv_top;
+#pragma unroll
+      for (int i = 0; i < QT; ++i) xm[i] = fmaxf(xm[i], xh[i] + none[h]);
+    }
+  };
+  auto grows = [&]() {
+    bool y = top > sv_top;
+#pragma unroll
+    for (int i = 0; i < QT; ++i) y = y | (xm[i] * qmul[i] > m[i] + (float)kAttnHead);
+    return __any(y);
+  };
+  // New references, and the sums so far brought to them.
+  auto rescale = [&]() {
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    ev = max(ev, (int)((__float_as_uint(fmaxf(top, 0.f)) >> 23) & 255) - 126);
+    sv_top = __uint_as_float((uint32_t)(ev + 127) << 23);
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-      xm[i] = -INFINITY;
+      float t = fmaxf(m[i], xm[i] * qmul[i]);
+      t = fmaxf(t, __shfl_xor(t, 16, 64));
+      t = fmaxf(t, __shfl_xor(t, 32, 64));
+      m[i] = t;
+      const float nr = t + (float)(ev - kAttnBase);
+      const float f = __builtin_amdgcn_exp2f(ref[i] - nr);
+      ref[i] = nr;
+      l[i] *= f;
+      z[i] *= f;
+      wsum[i] *= f;
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int p = 0; p < NP; ++p)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[i][s][e] = fmaf(sk[s][e], acc[i][s][e], mk[s][e] * qsum[i]);
-          if constexpr (masked) {
-            const int t = t0 + 16 * s + 4 * g + e;
-            ok[i][s][e] = t <= pos[i] && t < end && !y.bad[s] && (a.window == 0 || t > pos[i] - a.window);
-            x[i][s][e] = ok[i][s][e] ? x[i][s][e] : -INFINITY;
-          }
-          xm[i] = fmaxf(xm[i], x[i][s][e]);
-        }
-      xm[i] *= qmul[i];
-      grow = grow || xm[i] > m[i] + (float)kAttnHead;
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) o[i][p][h][b] *= f;
     }
-    if (__any(grow)) {
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      ev = max(ev, (int)((__float_as_uint(fmaxf(top, 0.f)) >> 23) & 255) - 126);
-      sv_top = __uint_as_float((uint32_t)(ev + 127) << 23);
-#pragma unroll
-      for (int i = 0; i < QT; ++i) {
-        float t = fmaxf(m[i], xm[i]);
-        t = fmaxf(t, __shfl_xor(t, 16, 64));
-        t = fmaxf(t, __shfl_xor(t, 32, 64));
-        m[i] = t;
-        const float nr = t + (float)(ev - kAttnBase);
-        const float f = __builtin_amdgcn_exp2f(ref[i] - nr);
-        ref[i] = nr;
-        l[i] *= f;
-        z[i] *= f;
-        wsum[i] *= f;
-#pragma unroll
-        for (int p = 0; p < NP; ++p)
-#pragma unroll
-          for (int h = 0; h < NH; ++h)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) o[i][p][h][b] *= f;
-      }
-    }
+  };
+  // Weights and the sums over them.  As soon as the registers of one kind of
+  // operand are used, the next tile's (at t1, in blocks nx) are loaded into them.
+  auto accumulate = [&](int t0, int t1, const Blocks& nx, auto mask) {
+    constexpr bool masked = decltype(mask)::value;
+    load_k(t1, nx);
     u4 pf[QT];  // the weights times sv, fp16: tokens 4 g .. of both halves
 #pragma unroll
-    for (int i = 0; i < QT; ++i) {
+    for (int h = 0; h < 2; ++h) {
+      float pv[QT][4], off[QT];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        float pv[4];
+      for (int i = 0; i < QT; ++i) off[i] = none[h] - ref[i];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(x[i][s][e], qmul[i], -ref[i]));
-          pv[e] = p * sv[s][e];
+      for (int e = 0; e < 4; ++e) {
+        const float sv = kv4_step(vp[h][e]), mv = kv4_centre(vp[h][e]);
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(x[i][h][e], qmul[i], off[i]));
+          pv[i][e] = p * sv;
           if constexpr (masked) {
-            l[i] += ok[i][s][e] ? p : 0.f;
-            z[i] = ok[i][s][e] ? fmaf(p, mv[s][e], z[i]) : z[i];
-            pv[e] = ok[i][s][e] ? pv[e] : 0.f;
+            const bool ok = sees(i, t0, h, e);
+            l[i] += ok ? p : 0.f;
+            z[i] = ok ? fmaf(p, mv, z[i]) : z[i];
+            pv[i][e] = ok ? pv[i][e] : 0.f;
           } else {
             l[i] += p;
-            z[i] = fmaf(p, mv[s][e], z[i]);
+            z[i] = fmaf(p, mv, z[i]);
           }
         }
-        pf[i][2 * s] = pack_h2(pv[0], pv[1]);
-        pf[i][2 * s + 1] = pack_h2(pv[2], pv[3]);
+      }
+#pragma unroll
+      for (int i = 0; i < QT; ++i) {
+        pf[i][2 * h] = pack_h2(pv[i][0], pv[i][1]);
+        pf[i][2 * h + 1] = pack_h2(pv[i][2], pv[i][3]);
       }
     }
+    load_params(t1, nx);
     // O^T: values 4 (NH c + h) + b of each part, in rows c
     const u4 halves = u4{0x47804780u, 0x47804780u, 0x47804780u, 0x47804780u};  // 7.5
 #pragma unroll
@@ -411,7 +461,7 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
         const int n = (p * NH + h) * 2;
-        const uint32_t a0 = y.v[0][n], a1 = y.v[0][n + 1], b0 = y.v[1][n], b1 = y.v[1][n + 1];
+        const uint32_t a0 = vc[0][n], a1 = vc[0][n + 1], b0 = vc[1][n], b1 = vc[1][n + 1];
         u4 f[4];
         f[0] = u4{a0 & 0x000F000Fu, a1 & 0x000F000Fu, b0 & 0x000F000Fu, b1 & 0x000F000Fu};
         f[1] = u4{a0 & 0x00F000F0u, a1 & 0x00F000F0u, b0 & 0x00F000F0u, b1 & 0x00F000F0u};
@@ -422,47 +472,41 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
 #pragma unroll
           for (int i = 0; i < QT; ++i) o[i][p][h][b] = mfma16x16x32<F16>(f[b], pf[i], o[i][p][h][b]);
       }
+    load_v(t1, nx);
   };
 
-  // does a row see less than every one of the 32 tokens?
-  auto cut = [&](int t0, const Tile& y) {
-    return t0 + 31 > pmin || (a.window > 0 && t0 <= pmax - a.window) || t0 + 32 > end || y.bad[0] || y.bad[1];
-  };
-
-  // The next tile's codes are loaded before the present one is computed, the
-  // table's entries one tile earlier still; two tiles a turn, each with registers
-  // of its own, but for the few that need masks.
+  // Tiles in order: those that the window cuts, those that every row sees whole (up
+  // to `full`), those that the rows' own positions or the end cut.  The cut ones
+  // mask, and rescale without asking.
   if (begin < end) {
     const int last = begin + (end - 1 - begin) / STEP * STEP;
-    Tile ta, tb;
+    const int full = uniform(min(pmin - 31, end - 32));
     Blocks nb = blocks_of(begin);
-    auto next = [&](int t0, Tile& y) {
-      load(min(t0 + STEP, last), nb, y);
-      nb = blocks_of(min(t0 + 2 * STEP, last));
-    };
-    load(begin, nb, ta);
+    load_k(begin, nb);
+    load_params(begin, nb);
+    load_v(begin, nb);
     nb = blocks_of(min(begin + STEP, last));
-    for (int t0 = begin; t0 < end;) {
-      if (cut(t0, ta)) {
-        next(t0, tb);
-        step32(t0, ta, std::true_type{});
-        t0 += STEP;
-        ta = tb;
-        continue;
+    int t0 = begin;
+    auto advance = [&](auto mask) {
+      const Blocks nx = nb;
+      nb = blocks_of(min(t0 + 2 * STEP, last));  // a tile ahead of the loads that need them
+      accumulate(t0, min(t0 + STEP, last), nx, mask);
+      t0 += STEP;
+    };
+    auto cut_to = [&](int to) {
+      while (t0 < to) {
+        scores(t0, std::true_type{});
+        rescale();
+        advance(std::true_type{});
       }
-      do {
-        next(t0, tb);
-        step32(t0, ta, std::false_type{});
-        t0 += STEP;
-        if (t0 >= end || cut(t0, tb)) {
-          ta = tb;
-          break;
-        }
-        next(t0, ta);
-        step32(t0, tb, std::false_type{});
-        t0 += STEP;
-      } while (t0 < end && !cut(t0, ta));
+    };
+    if (a.window > 0) cut_to(min(end, pmax - a.window + 1));
+    while (t0 <= full) {
+      scores(t0, std::false_type{});
+      if (grows()) rescale();
+      advance(std::false_type{});
     }
+    cut_to(end);
   }
 
   // ---- the end: sums over the lanes of a row, parts to the workspace, rows out ----
@@ -652,7 +696,7 @@ AttnPlan attn_plan(int64_t T, int64_t R, int64_t n_q, int64_t n_kv, int64_t hd, 
   p.many = rows > kAttnFewRows;
   p.few = !p.many || R > 1;
   const int64_t few_rows = p.many ? group : rows;  // of a request, as a rule
-  p.qt_few = few_rows <= 16 ? 1 : (few_rows <= 32 || hd == 256 ? 2 : 4);
+  p.qt_few = few_rows <= 16 || hd == 256 ? 1 : 2;
   p.qt_many = hd == 256 ? 1 : 2;
   const int64_t seqs = std::min(R, T);
   p.items_few = T * group / (16 * p.qt_few) + seqs;
@@ -682,8 +726,7 @@ void launch_attn(const AttnPlan& p, Kv4AttnArgs a, int64_t n_kv, int64_t n_q, hi
     b.part_row0 = 0;
     const dim3 grid((unsigned)p.items_few, (unsigned)n_kv);
     if (p.qt_few == 1) kv4_attn_kernel<T, HD, 1, true><<<grid, 256, 0, st>>>(b);
-    else if (p.qt_few == 2) kv4_attn_kernel<T, HD, 2, true><<<grid, 256, 0, st>>>(b);
-    else if constexpr (HD != 256) kv4_attn_kernel<T, HD, 4, true><<<grid, 256, 0, st>>>(b);
+    else if constexpr (HD != 256) kv4_attn_kernel<T, HD, 2, true><<<grid, 256, 0, st>>>(b);
   }
   if (p.many) {
     Kv4AttnArgs b = a;
