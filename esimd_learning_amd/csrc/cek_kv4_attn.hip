@@ -43,12 +43,12 @@ struct Kv4AttnArgs {
   const int32_t *tables, *kv_lens, *cu_q;
   float* part;     // split keys: rows of hd sums
   float* part_ml;  // and their (reference exponent, sum of weights)
-  int4* meta;      // per query token: first partial row, parts, rows a tile, place in its request
+  int4* meta;      // per row of a kv head: first part's row, parts, rows a slot, rows a tile
   int64_t T, q_stride, out_stride, table_stride;
   Kv4Dims dm;
   int R, group, max_blocks, window;
   int rows_above, rows_upto;  // this launch serves requests with that many rows
-  int target;                 // work items (per kv head) to split the keys into; 0: not split
+  int wgs;                    // workgroups per kv head that share the keys evenly; 0: keys stay whole
   int part_row0;              // first partial row of this launch
   int vec_q, vec_out;
   float scale;
@@ -60,85 +60,115 @@ constexpr float kAttnNone = -1e30f;
 
 typedef const __attribute__((address_space(4))) int32_t* const_i32;  // scalar loads
 
-// One request as the work list sees it.
+// A stretch of work: units [unit, unit + units) of the keys of one tile of rows.
 struct Kv4Work {
-  int r, q0, rows, kv, n_new, lo, tile, chunk, nch, item0, keys;
+  int r, q0, rows, kv, n_new, lo, tile;
+  int unit, units, all;  // all: the tile's units
+  int first;             // the tile's first unit in the list
 };
 
 __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// Inclusive sum over the lanes, by DPP: rows of 16 by shifts, then the rows' last
+// lanes broadcast into the rows behind them.
+#define CEK_DPP_ADD(x, ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xF, true)
 __device__ inline int wave_scan_incl(int x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(x, off, 64);
-    if (lane >= off) x += y;
-  }
+  CEK_DPP_ADD(x, 0x111, 0xF);  // row_shr 1, 2, 4, 8
+  CEK_DPP_ADD(x, 0x112, 0xF);
+  CEK_DPP_ADD(x, 0x114, 0xF);
+  CEK_DPP_ADD(x, 0x118, 0xF);
+  CEK_DPP_ADD(x, 0x142, 0xA);  // row_bcast 15 into rows 1 and 3
+  CEK_DPP_ADD(x, 0x143, 0xC);  // row_bcast 31 into rows 2 and 3
   return x;
 }
 
-// Work item -> (request, row tile, part of the keys).  A request has
-// ceil(rows / BR) tiles and its keys (from the first that any row sees, down to
-// a multiple of 32) in parts of C, the same for the whole call: C = the sum over
-// requests of tiles x keys, over `target`, at least 128 and a multiple of 128.
-// Every wave of the grid computes the same from the lengths; items of a call
-// number at most target + tiles, which is the grid.
+// The work list: every request has ceil(rows / BR) tiles of rows, and each tile its
+// keys (from the first that any row sees, down to a multiple of 32) in units of
+// `len` tokens, or in one.  Tiles lie one after another, a request's last one
+// first (its rows see most keys).  Every wave of the grid computes its place
+// from the lengths alone.
 template <int BR>
-__device__ inline bool kv4_find_work(const Kv4AttnArgs& a, int item, Kv4Work& w) {
-  const int lane = threadIdx.x & 63;
-  const int64_t reach = (int64_t)a.max_blocks << a.dm.bs_log2;
-  auto request = [&](int r, int& q0, int& rows, int& kv, int& n_new, int& lo, int& tiles) {
-    q0 = n_new = rows = kv = lo = tiles = 0;
-    if (r >= a.R) return;
-    q0 = max(0, a.cu_q[r]);
-    n_new = (int)min((int64_t)a.cu_q[r + 1], a.T) - q0;
-    if (n_new <= 0) return;
-    const int64_t n = (int64_t)n_new * a.group;
-    if (n <= a.rows_above || n > a.rows_upto) return;
-    rows = (int)n;
-    kv = (int)min((int64_t)max(a.kv_lens[r], 0), reach);
-    lo = a.window > 0 ? max(0, kv - n_new - a.window + 1) & ~31 : 0;
-    tiles = (rows + BR - 1) / BR;
-  };
-  int q0, rows, kv, n_new, lo, tiles;
-  int C = INT32_MAX;
-  if (a.target > 0) {
-    float total = 0.f;
+struct Kv4List {
+  const Kv4AttnArgs& a;
+  int len = 0;    // tokens of a unit; 0: all of a tile's
+  int total = 0;  // units, where the keys are shared
+
+  struct Req { int q0, rows, kv, n_new, lo, tiles; };
+  __device__ inline Req request(int r) const {
+    Req x;
+    const int at = min(r, a.R - 1);
+    const int c0 = a.cu_q[at], c1 = a.cu_q[at + 1], kv = a.kv_lens[at];
+    x.q0 = max(0, c0);
+    x.n_new = (int)min((int64_t)c1, a.T) - x.q0;
+    const int64_t n = (int64_t)x.n_new * a.group;
+    const bool mine = (r < a.R) & (x.n_new > 0) & (n > a.rows_above) & (n <= a.rows_upto);
+    x.rows = mine ? (int)n : 0;
+    x.kv = (int)min((int64_t)max(kv, 0), (int64_t)a.max_blocks << a.dm.bs_log2);
+    x.lo = a.window > 0 ? max(0, x.kv - x.n_new - a.window + 1) & ~31 : 0;
+    x.tiles = (x.rows + BR - 1) / BR;
+    return x;
+  }
+  __device__ inline int units(const Req& x) const {
+    return len ? (int)(((unsigned)max(x.kv - x.lo, 1) + (unsigned)len - 1u) / (unsigned)len) : 1;
+  }
+  // Units of `step` tokens, or as many times that as keep their number in 30 bits.
+  __device__ inline void share(const Req& first, int step) {
+    const int lane = threadIdx.x & 63;
+    for (len = step;; len *= 2) {
+      float sum = (float)first.tiles * (float)units(first);
+      int n = first.tiles * units(first);
+      for (int base = 64; base < a.R; base += 64) {
+        const Req x = request(base + lane);
+        sum += (float)x.tiles * (float)units(x);
+        n += x.tiles * units(x);
+      }
+      total = __builtin_amdgcn_readlane(wave_scan_incl(n), 63);
+      if (wave_sum_dpp(sum) < 0x1p30f) return;
+    }
+  }
+  // Workgroup j of n gets each = total / n units, the first `more` one more.
+  int each = 0, more = 0;
+  __device__ inline void deal(int n) {
+    each = uniform((int)((unsigned)total / (unsigned)n));
+    more = total - each * n;
+  }
+  __device__ inline int begin_of(int j) const { return each * j + min(j, more); }
+  __device__ inline int owner_of(int u) const {
+    const int far = more * (each + 1);
+    return uniform(u < far ? (int)((unsigned)u / (unsigned)(each + 1)) : more + (int)((unsigned)(u - far) / (unsigned)max(each, 1)));
+  }
+  // The stretch that starts at unit u, up to unit `to`; false behind the last one.
+  __device__ inline bool find(const Req& first, int u, int to, Kv4Work& w) const {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
     for (int base = 0; base < a.R; base += 64) {
-      request(base + lane, q0, rows, kv, n_new, lo, tiles);
-      total += (float)tiles * (float)(kv - lo);
+      const Req x = base == 0 ? first : request(base + lane);
+      const int n = units(x);
+      const int incl = before + wave_scan_incl(x.tiles * n);
+      const uint64_t above = __ballot(incl > u);
+      if (above) {
+        const int at = __builtin_ctzll(above);
+        auto get = [&](int y) { return __builtin_amdgcn_readlane(y, at); };
+        w.r = base + at;
+        w.q0 = get(x.q0);
+        w.rows = get(x.rows);
+        w.kv = get(x.kv);
+        w.n_new = get(x.n_new);
+        w.lo = get(x.lo);
+        w.all = get(n);
+        const int tiles = get(x.tiles), start = get(incl) - tiles * w.all;
+        const int nth = uniform((u - start) / w.all);
+        w.tile = tiles - 1 - nth;
+        w.first = start + nth * w.all;
+        w.unit = u - w.first;
+        w.units = min(w.all - w.unit, to - u);
+        return true;
+      }
+      before = __builtin_amdgcn_readlane(incl, 63);
     }
-    total = wave_sum(total);
-    C = max(1, (int)ceilf(total * 1.001f / ((float)a.target * 128.f))) * 128;
+    return false;
   }
-  int first = 0;
-  for (int base = 0; base < a.R; base += 64) {
-    request(base + lane, q0, rows, kv, n_new, lo, tiles);
-    const int nch = a.target > 0 ? max(1, (int)(((unsigned)(kv - lo) + (unsigned)C - 1u) / (unsigned)C)) : 1;
-    const int incl = first + wave_scan_incl(tiles * nch);
-    const uint64_t above = __ballot(incl > item);
-    if (above) {
-      const int at = __builtin_ctzll(above);
-      auto get = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
-      w.r = base + at;
-      w.q0 = get(q0);
-      w.rows = get(rows);
-      w.kv = get(kv);
-      w.n_new = get(n_new);
-      w.lo = get(lo);
-      w.nch = get(nch);
-      const int t = get(tiles);
-      w.item0 = get(incl) - t * w.nch;
-      const int at_tile = uniform((item - w.item0) / w.nch);
-      w.tile = t - 1 - at_tile;  // the last rows, which see most keys, first
-      w.chunk = item - w.item0 - at_tile * w.nch;
-      w.keys = C;
-      return true;
-    }
-    first = __builtin_amdgcn_readlane(incl, 63);
-  }
-  return false;
-}
+};
 
 // Parameters of 16 tokens that do not exist.
 __device__ const uint8_t kv4_zeros[64] __attribute__((aligned(16))) = {};
@@ -147,63 +177,213 @@ __device__ inline uint32_t pack_h2(float a, float b) {
   return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});
 }
 
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
+// One load instruction straight to LDS: N bytes a lane, lane after lane from `to`.
+template <int N>
+__device__ inline void load_lds(const uint8_t* from, uint8_t* to) {
+  static_assert(N == 4 || N == 16, "bytes a lane");
+  if constexpr (N == 16) __builtin_amdgcn_global_load_lds(from, (lds_ptr_t)to, 16, 0, 0);
+  else __builtin_amdgcn_global_load_lds(from, (lds_ptr_t)to, 4, 0, 0);
+}
+__device__ inline uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(lds_ptr_t)p; }
+
+// LDS reads behind a wave's own direct loads.  In asm, each with its wait: the
+// compiler would wait for every direct load in flight before any LDS read.
+template <int O0, int O1, int O2, int O3>
+__device__ inline void lds_read4(uint32_t at, u4& a, u4& b, u4& c, u4& d) {
+  asm volatile(
+      "ds_read_b128 %0, %4 offset:%5\n\tds_read_b128 %1, %4 offset:%6\n\t"
+      "ds_read_b128 %2, %4 offset:%7\n\tds_read_b128 %3, %4 offset:%8\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
+      : "v"(at), "n"(O0), "n"(O1), "n"(O2), "n"(O3)
+      : "memory");
+}
+// A lane's codes of 32 tokens, 16 and 16, from byte OFF of a slot on.
+template <int HD, int OFF>
+__device__ inline void read_codes(uint32_t at, uint32_t (&to)[2][HD / 32]) {
+  if constexpr (HD == 64) {
+    u2 a, b;
+    asm volatile("ds_read_b64 %0, %2 offset:%3\n\tds_read_b64 %1, %2 offset:%4\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(a), "=&v"(b)
+                 : "v"(at), "n"(OFF), "n"(OFF + 512)
+                 : "memory");
+    to[0][0] = a[0], to[0][1] = a[1], to[1][0] = b[0], to[1][1] = b[1];
+  } else if constexpr (HD == 128) {
+    u4 a, b;
+    asm volatile("ds_read_b128 %0, %2 offset:%3\n\tds_read_b128 %1, %2 offset:%4\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(a), "=&v"(b)
+                 : "v"(at), "n"(OFF), "n"(OFF + 1024)
+                 : "memory");
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[0][e] = a[e], to[1][e] = b[e];
+  } else {
+    u4 x[4];
+    lds_read4<OFF, OFF + 1024, OFF + 2048, OFF + 3072>(at, x[0], x[1], x[2], x[3]);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) to[e / 8][e % 8] = x[e / 4][e % 4];
+  }
+}
+
+// Workgroups that a CU holds at once (waves a SIMD): by registers and LDS.
+constexpr int attn_held(int hd, int qt) { return hd == 256 ? 2 : (hd == 64 ? 5 - qt : 4 - qt); }
+
 // KVSPLIT: the workgroup's four waves share QT x 16 rows and take every fourth 32
 // tokens each; else each wave has QT x 16 rows of its own and all the tokens.
 template <typename T, int HD, int QT, bool KVSPLIT>
-__global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4AttnArgs a) {
   constexpr int ND = HD / 32;                    // 32-bit words per lane, part and 16 tokens
   constexpr int NP = HD >= 128 ? HD / 128 : 1;   // parts of a row: 128 values, or 64
   constexpr int NH = HD >= 128 ? 2 : 1;          // runs of four values per lane and part
   constexpr int PW = HD / NP;                    // values of a part
   constexpr int BR = QT * 16 * (KVSPLIT ? 1 : kAttnWaves);
   constexpr int LSTR = HD + 4;                   // LDS row stride: rows 4 banks apart
-  __shared__ float lds_o[KVSPLIT ? kAttnWaves * 16 * LSTR : 1];
-  __shared__ float lds_ml[KVSPLIT ? kAttnWaves * 16 * 2 : 1];
+  constexpr int CODES = HD >= 128 ? 4 * NP * 1024 : 2048;  // bytes of 32 tokens' codes
+  constexpr int SLOT = CODES + 256;                        // and parameters
+  constexpr int DEPTH = HD == 256 ? 2 : 3;                 // slots a wave
+  constexpr int LOADS = CODES / 1024 + 1;                  // load instructions of a slot
+  constexpr int OUT_BYTES = KVSPLIT ? kAttnWaves * 16 * (LSTR + 2) * 4 : 0;
+  constexpr int RING_BYTES = kAttnWaves * DEPTH * SLOT;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[RING_BYTES > OUT_BYTES ? RING_BYTES : OUT_BYTES];
+  float* const lds_o = reinterpret_cast<float*>(lds);
+  float* const lds_ml = lds_o + kAttnWaves * 16 * LSTR;
 
-  Kv4Work w;
-  if (!kv4_find_work<BR>(a, blockIdx.x, w)) return;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.y;
   const int bs = 1 << a.dm.bs_log2;
+  Kv4List<BR> list{a};
+  const auto mine = list.request(lane);
+  int u = blockIdx.x, u_end = u + 1;
+  if (a.wgs > 0) {
+    list.share(mine, KVSPLIT ? 32 * kAttnWaves : 512);
+    list.deal(a.wgs);
+    u = list.begin_of(blockIdx.x);
+    u_end = list.begin_of(blockIdx.x + 1);
+  }
+  for (Kv4Work w; u < u_end && list.find(mine, u, u_end, w); u += w.units) {
   const int row0 = w.tile * BR + (KVSPLIT ? 0 : wave * QT * 16);  // this wave's first row in the request
-
-  if (a.meta && kvh == 0 && w.chunk == 0) {
-    // for the launch that joins the parts
-    const int t0 = w.tile * BR / a.group, t1 = min(w.rows, (w.tile + 1) * BR);
-    for (int t = t0 + (int)threadIdx.x; t * a.group < t1; t += 256)
-      a.meta[w.q0 + t] = int4{a.part_row0 + w.item0 * a.dm.n_kv * BR, w.nch, BR, t};
+  // Partial rows: of a tile's first stretch in 2 wg + 1, of the others in 2 wg.
+  const bool whole = w.units == w.all;
+  const int64_t part0 =
+      a.part_row0 + ((int64_t)(2 * blockIdx.x + (w.unit == 0)) * a.dm.n_kv + kvh) * BR;
+  if (a.meta && kvh == 0 && w.unit == 0 && (int)threadIdx.x < BR) {
+    // for the launch that joins the parts: the first one's row and their number
+    const int rr = w.tile * BR + (int)threadIdx.x;
+    const int parts = whole ? 1 : list.owner_of(w.first + w.all - 1) - (int)blockIdx.x + 1;
+    if (rr < w.rows) a.meta[(int64_t)w.q0 * a.group + rr] = int4{(int)part0 + (int)threadIdx.x, parts, a.dm.n_kv * BR, BR};
   }
 
-  // ---- q: this lane's 16-bit values of row c of each tile, in the order of K's words ----
-  u4 qf[QT][ND];        // MFMA operands
-  float qsum[QT], qmul[QT];
+  // ---- rows and the range of keys ----
   int pos[QT];          // position of the row; padding rows see everything
   int pmin = INT32_MAX, pmax = -1;  // over this wave's rows
+  const uint16_t* qsrc[QT];
+  bool real[QT];
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     const int rr = row0 + i * 16 + c;
-    const bool real = rr < w.rows;
+    real[i] = rr < w.rows;
     const int t = rr / a.group, h = kvh * a.group + rr % a.group;
-    const uint16_t* src = a.q + (int64_t)(w.q0 + (real ? t : 0)) * a.q_stride + (int64_t)(real ? h : 0) * HD;
-    pos[i] = real ? w.kv - w.n_new + t : INT32_MAX - 1;
+    qsrc[i] = a.q + (int64_t)(w.q0 + (real[i] ? t : 0)) * a.q_stride + (int64_t)(real[i] ? h : 0) * HD;
+    pos[i] = real[i] ? w.kv - w.n_new + t : INT32_MAX - 1;
     if (row0 + i * 16 < w.rows) {
       // uniform: rows are in order of position
       pmin = uniform(min(pmin, w.kv - w.n_new + (row0 + i * 16) / a.group));
       pmax = uniform(max(pmax, w.kv - w.n_new + (min(row0 + i * 16 + 16, w.rows) - 1) / a.group));
     }
+  }
+  const int window = a.window > 0 ? a.window : INT32_MAX;  // pos - window stays in range
+  const int t_lo = a.window > 0 ? max(0, pmin - a.window + 1) & ~31 : 0;
+  const int begin = uniform((list.len ? max(t_lo, w.lo + w.unit * list.len) : t_lo) + (KVSPLIT ? 32 * wave : 0));
+  const int end = uniform(
+      list.len ? (int)min((int64_t)pmax + 1, (int64_t)w.lo + (int64_t)(w.unit + w.units) * list.len) : pmax + 1);
+  constexpr int STEP = KVSPLIT ? 32 * kAttnWaves : 32;
+
+
+  // ---- codes and parameters: through a ring of LDS slots ----
+  // Each wave keeps the next DEPTH tiles' loads in flight without a register: a
+  // lane reads back what it loaded itself (the codes), so that nothing but the
+  // wave's own vmcnt orders the two.
+  const uint8_t* head = a.cache + (int64_t)kvh * kv4_head_bytes(bs, HD);
+  const const_i32 table = (const_i32)(uintptr_t)(a.tables + (int64_t)w.r * a.table_stride);
+  struct Blocks { int b[2]; };
+  auto blocks_of = [&](int t0) {
+    return Blocks{{table[t0 >> a.dm.bs_log2], table[min(t0 + 16, w.kv - 1) >> a.dm.bs_log2]}};
+  };
+  // Does the first or second half of the 32 tokens at t0 lie in no block?  (The
+  // second one may lie behind the last key.)
+  auto outside = [&](int t0, const Blocks& x, int h) {
+    return ((uint32_t)x.b[h] >= (uint32_t)a.dm.num_blocks) | (t0 + 16 * h >= w.kv);
+  };
+  uint8_t* const ring = lds + wave * (DEPTH * SLOT);
+  const int half = HD >= 128 ? 0 : lane >> 5;  // hd 64: the 32 tokens' codes in one load
+  const uint32_t k_lane = HD >= 128 ? c * (HD / 2) + g * 16 : (lane & 31) * 16;
+  const uint32_t v_lane = kv4_v_codes(bs, HD) + (HD >= 128 ? g * HD * 2 + c * 16 : (lane & 31) * 16);
+  const uint32_t p_lane = (g >> 1 ? kv4_v_params(bs, HD) : kv4_k_params(bs, HD)) + 4 * c;
+  // returns which halves lie in no block
+  auto fetch = [&](int t0, const Blocks& x, int slot) -> int {
+    uint8_t* const to = ring + slot * SLOT;
+    const uint8_t* base[2];  // a block outside the cache holds no token: block 0 is read in its place
+    int tok[2];
+    bool out[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      tok[h] = (t0 + 16 * h) & (bs - 1);
+      out[h] = outside(t0, x, h);
+      base[h] = head + (int64_t)(out[h] ? 0 : x.b[h]) * a.dm.block_stride;
+    }
+    if constexpr (HD >= 128) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          // part p of 16 tokens: 64 bytes of each K row, 256 of each four tokens of V
+          load_lds<16>(base[h] + tok[h] * (HD / 2) + p * (PW / 2) + k_lane, to + (h * NP + p) * 1024);
+          load_lds<16>(base[h] + tok[h] * (HD / 2) + p * (PW * 2) + v_lane, to + ((2 + h) * NP + p) * 1024);
+        }
+    } else {
+      const uint8_t* b = half ? base[1] + tok[1] * (HD / 2) : base[0] + tok[0] * (HD / 2);
+      load_lds<16>(b + k_lane, to);
+      load_lds<16>(b + v_lane, to + 1024);
+    }
+    // lanes 16 x (K, V) .. : parameters of the first and the second 16 tokens; 0
+    // for tokens that do not exist, whatever lies in block 0
+    const uint8_t* zeros = kv4_zeros;
+    const uint8_t* b0 = out[0] ? zeros : base[0] + 4 * tok[0];
+    const uint8_t* b1 = out[1] ? zeros : base[1] + 4 * tok[1];
+    const uint32_t o0 = out[0] ? 4 * c : p_lane, o1 = out[1] ? 4 * c : p_lane;
+    load_lds<4>((g & 1 ? b1 : b0) + (g & 1 ? o1 : o0), to + CODES);
+    return (int)out[0] + 2 * (int)out[1];
+  };
+  const int last = begin + (end - 1 - begin) / STEP * STEP;
+  Blocks nb;                       // of the tile DEPTH ahead
+  int outs = 0;                    // two bits a slot, the present tile's first: halves outside the cache
+  if (begin < end) {
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {
+      nb = blocks_of(min(begin + i * STEP, last));
+      outs |= fetch(min(begin + i * STEP, last), nb, i) << (2 * i);
+    }
+    nb = blocks_of(min(begin + DEPTH * STEP, last));
+  }
+
+  // ---- q: this lane's 16-bit values of row c of each tile, in the order of K's words ----
+  u4 qf[QT][ND];        // MFMA operands
+  float qsum[QT], qmul[QT];
+#pragma unroll
+  for (int i = 0; i < QT; ++i) {
     uint32_t raw[ND][4];
 #pragma unroll
     for (int n = 0; n < ND; ++n) {
       const int d0 = (n / (PW / 32)) * PW + g * (PW / 4) + (n % (PW / 32)) * 8;
       if (a.vec_q) {
-        const u4 x = load_u4(src + d0);
+        const u4 x = load_u4(qsrc[i] + d0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) raw[n][e] = real ? x[e] : 0;
+        for (int e = 0; e < 4; ++e) raw[n][e] = real[i] ? x[e] : 0;
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          raw[n][e] = real ? (uint32_t)src[d0 + 2 * e] | ((uint32_t)src[d0 + 2 * e + 1] << 16) : 0;
+          raw[n][e] = real[i] ? (uint32_t)qsrc[i][d0 + 2 * e] | ((uint32_t)qsrc[i][d0 + 2 * e + 1] << 16) : 0;
       }
     }
     float top = 0.f;
@@ -239,13 +419,6 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
     qmul[i] = ldexpf(a.scale * 1.4426950408889634f, 24 - k);
   }
 
-  // ---- the range of keys ----
-  const int window = a.window > 0 ? a.window : INT32_MAX;  // pos - window stays in range
-  const int t_lo = a.window > 0 ? max(0, pmin - a.window + 1) & ~31 : 0;
-  const int begin = uniform((w.nch > 1 ? max(t_lo, w.lo + w.chunk * w.keys) : t_lo) + (KVSPLIT ? 32 * wave : 0));
-  const int end = uniform(
-      w.nch > 1 ? (int)min((int64_t)pmax + 1, (int64_t)w.lo + ((int64_t)w.chunk + 1) * w.keys) : pmax + 1);
-  constexpr int STEP = KVSPLIT ? 32 * kAttnWaves : 32;
 
   f4 o[QT][NP][NH][4];
   f4 wsum[QT];
@@ -261,76 +434,34 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
     for (int x = 0; x < NP * NH * 4; ++x) o[i][x / (NH * 4)][x / 4 % NH][x % 4] = f4{0.f, 0.f, 0.f, 0.f};
   }
 
-  const uint8_t* head = a.cache + (int64_t)kvh * kv4_head_bytes(bs, HD);
-  const uint32_t k_lane = c * (HD / 2) + g * (PW / 8);
-  const uint32_t v_lane = kv4_v_codes(bs, HD) + g * HD * 2 + c * (PW / 8);
-  const uint32_t kp_lane = kv4_k_params(bs, HD) + 16 * g;
-  const uint32_t vp_lane = kv4_v_params(bs, HD) + 16 * g;
-  const const_i32 table = (const_i32)(uintptr_t)(a.tables + (int64_t)w.r * a.table_stride);
-
-  struct Blocks { int b[2]; };
-  // the blocks of 32 tokens; behind the last key (a half of them may lie there) none
-  auto blocks_of = [&](int t0) {
-    Blocks x;
-    x.b[0] = uniform(table[t0 >> a.dm.bs_log2]);
-    x.b[1] = uniform(table[min(t0 + 16, w.kv - 1) >> a.dm.bs_log2]);
-    if (t0 + 16 >= w.kv) x.b[1] = -1;
-    return x;
-  };
-  // A block outside the cache holds no token: block 0 is read in its place.
-  auto at_block = [&](int t0, const Blocks& x, int i, int& tok) {
-    const int b = x.b[i];
-    tok = (t0 + 16 * i) & (bs - 1);
-    return head + (int64_t)(b < 0 || b >= a.dm.num_blocks ? 0 : b) * a.dm.block_stride;
-  };
-  auto load_codes = [&](const uint8_t* base, uint32_t at, uint32_t (&to)[ND], uint32_t part) {
-    if constexpr (HD == 64) {
-      const uint2 x = *reinterpret_cast<const uint2*>(base + at);
-      to[0] = x.x, to[1] = x.y;
-    } else {
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        const u4 x = load_u4(base + p * part + at);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) to[4 * p + e] = x[e];
-      }
-    }
-  };
-  uint32_t kc[2][ND], vc[2][ND];  // the codes of 32 tokens, 16 and 16
-  u4 kp[2], vp[2];                // their parameters, of tokens 4 g ..
-  float none[2];                  // 0, or -infinity where the block lies outside the cache
-  auto load_k = [&](int t0, const Blocks& x) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      int tok;
-      const uint8_t* base = at_block(t0, x, i, tok);
-      load_codes(base + tok * (HD / 2), k_lane, kc[i], PW / 2);  // 64 bytes of a row and part of 128 values
-    }
-  };
-  auto load_v = [&](int t0, const Blocks& x) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      int tok;
-      const uint8_t* base = at_block(t0, x, i, tok);
-      load_codes(base + tok * (HD / 2), v_lane, vc[i], PW * 2);  // 256 bytes of four tokens and part
-    }
-  };
-  auto load_params = [&](int t0, const Blocks& x) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      int tok;
-      const uint8_t* base = at_block(t0, x, i, tok) + 4 * tok;
-      const bool out = x.b[i] < 0 || x.b[i] >= a.dm.num_blocks;
-      // tokens that do not exist have parameters 0, whatever lies in block 0
-      kp[i] = load_u4(out ? kv4_zeros + 16 * g : base + kp_lane);
-      vp[i] = load_u4(out ? kv4_zeros + 16 * g : base + vp_lane);
-      none[i] = out ? -INFINITY : 0.f;
-    }
-  };
-
   auto sees = [&](int i, int t0, int h, int e) {  // row c of tile i the token 16 h + 4 g + e at t0
     const int t = t0 + 16 * h + 4 * g + e;
     return (t <= pos[i]) & (t < end) & (t > pos[i] - window);  // no branches
+  };
+
+  uint32_t kc[2][ND], vc[2][ND];  // the codes of 32 tokens, 16 and 16
+  u4 kp[2], vp[2];                // their parameters, of tokens 4 g ..
+  float none[2];                  // 0, or -infinity where the block lies outside the cache
+  int slot = 0;
+  const uint32_t lds_codes = lds_offset(ring) + (HD >= 128 ? lane * 16 : c * 32 + g * 8);
+  const uint32_t lds_words = lds_offset(ring) + (HD >= 128 ? lane * 16 : lane * 8);
+  const uint32_t lds_par = lds_offset(ring) + CODES + 16 * g;
+  // The present tile from its slot: K codes and parameters once they are there,
+  // V codes later, and then the slot to the tile DEPTH ahead.
+  auto read_k = [&]() {
+    wait_vmcnt<(DEPTH - 1) * LOADS>();
+    const uint32_t at = slot * SLOT;
+    none[0] = outs & 1 ? -INFINITY : 0.f;
+    none[1] = outs & 2 ? -INFINITY : 0.f;
+    lds_read4<0, 64, 128, 192>(lds_par + at, kp[0], kp[1], vp[0], vp[1]);
+    read_codes<HD, 0>(lds_codes + at, kc);
+  };
+  auto read_v = [&]() { read_codes<HD, (HD >= 128 ? CODES / 2 : 1024)>(lds_words + slot * SLOT, vc); };
+  auto refill = [&](int t0) {
+    const Blocks nx = nb;
+    nb = blocks_of(min(t0 + (DEPTH + 1) * STEP, last));  // a tile ahead of the loads that need them
+    outs = (outs >> 2) | (fetch(min(t0 + DEPTH * STEP, last), nx, slot) << (2 * (DEPTH - 1)));
+    slot = slot + 1 == DEPTH ? 0 : slot + 1;
   };
 
   // Scores of 32 tokens: x (exponents / qmul), their maxima xm and that of the V steps.
@@ -416,11 +547,9 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
           for (int b = 0; b < 4; ++b) o[i][p][h][b] *= f;
     }
   };
-  // Weights and the sums over them.  As soon as the registers of one kind of
-  // operand are used, the next tile's (at t1, in blocks nx) are loaded into them.
-  auto accumulate = [&](int t0, int t1, const Blocks& nx, auto mask) {
+  // Weights and the sums over them.
+  auto accumulate = [&](int t0, auto mask) {
     constexpr bool masked = decltype(mask)::value;
-    load_k(t1, nx);
     u4 pf[QT];  // the weights times sv, fp16: tokens 4 g .. of both halves
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -451,7 +580,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
         pf[i][2 * h + 1] = pack_h2(pv[i][2], pv[i][3]);
       }
     }
-    load_params(t1, nx);
+    read_v();
+    refill(t0);
     // O^T: values 4 (NH c + h) + b of each part, in rows c
     const u4 halves = u4{0x47804780u, 0x47804780u, 0x47804780u, 0x47804780u};  // 7.5
 #pragma unroll
@@ -472,42 +602,33 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
 #pragma unroll
           for (int i = 0; i < QT; ++i) o[i][p][h][b] = mfma16x16x32<F16>(f[b], pf[i], o[i][p][h][b]);
       }
-    load_v(t1, nx);
   };
 
   // Tiles in order: those that the window cuts, those that every row sees whole (up
   // to `full`), those that the rows' own positions or the end cut.  The cut ones
   // mask, and rescale without asking.
   if (begin < end) {
-    const int last = begin + (end - 1 - begin) / STEP * STEP;
     const int full = uniform(min(pmin - 31, end - 32));
-    Blocks nb = blocks_of(begin);
-    load_k(begin, nb);
-    load_params(begin, nb);
-    load_v(begin, nb);
-    nb = blocks_of(min(begin + STEP, last));
     int t0 = begin;
-    auto advance = [&](auto mask) {
-      const Blocks nx = nb;
-      nb = blocks_of(min(t0 + 2 * STEP, last));  // a tile ahead of the loads that need them
-      accumulate(t0, min(t0 + STEP, last), nx, mask);
-      t0 += STEP;
-    };
     auto cut_to = [&](int to) {
-      while (t0 < to) {
+      for (; t0 < to; t0 += STEP) {
+        read_k();
         scores(t0, std::true_type{});
         rescale();
-        advance(std::true_type{});
+        accumulate(t0, std::true_type{});
       }
     };
     if (a.window > 0) cut_to(min(end, pmax - a.window + 1));
-    while (t0 <= full) {
+    for (; t0 <= full; t0 += STEP) {
+      read_k();
       scores(t0, std::false_type{});
       if (grows()) rescale();
-      advance(std::false_type{});
+      accumulate(t0, std::false_type{});
     }
     cut_to(end);
+    wait_vmcnt<0>();  // loads in flight land in LDS that is about to be used, or given back
   }
+  if (KVSPLIT) __syncthreads();
 
   // ---- the end: sums over the lanes of a row, parts to the workspace, rows out ----
 #pragma unroll
@@ -555,8 +676,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
         }
       }
       if (rr < w.rows) {
-        if (w.nch > 1) {
-          const int64_t pr = a.part_row0 + ((int64_t)(w.item0 + w.tile * w.nch + w.chunk) * a.dm.n_kv + kvh) * BR + i * 16 + row;
+        if (!whole) {
+          const int64_t pr = part0 + i * 16 + row;
 #pragma unroll
           for (int e = 0; e < HD / 16; e += 4)
             *reinterpret_cast<f4*>(a.part + pr * HD + seg * (HD / 16) + e) = f4{y[e], y[e + 1], y[e + 2], y[e + 3]};
@@ -585,9 +706,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
     } else {
       const int rr = row0 + i * 16 + c;
       if (rr < w.rows) {
-        if (w.nch > 1) {
-          const int64_t pr = a.part_row0 + ((int64_t)(w.item0 + w.tile * w.nch + w.chunk) * a.dm.n_kv + kvh) * BR +
-                             wave * QT * 16 + i * 16 + c;
+        if (!whole) {
+          const int64_t pr = part0 + wave * QT * 16 + i * 16 + c;
 #pragma unroll
           for (int p = 0; p < NP; ++p)
 #pragma unroll
@@ -626,44 +746,59 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
       }
     }
   }
+  if (KVSPLIT) __syncthreads();  // the rows have been read: LDS is free for the next stretch's codes
+  }
 }
 
-// Joins the parts of a row: one workgroup per (query token, query head), its waves
-// taking every fourth part.
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4AttnArgs a) {
+// Joins the parts of the rows that several workgroups share.  Part 0 of a row is
+// its first workgroup's, part p that of the p-th after it, two row tiles on each.
+// WAVES waves a row: four where there are few rows with many parts, one else.
+template <typename T, int HD, int WAVES>
+__global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4AttnArgs a, int n_q) {
   constexpr int E = HD / 64;
-  const int t = blockIdx.x, h = blockIdx.y;
-  if (t < a.cu_q[0] || t >= a.cu_q[a.R]) return;
-  const int4 mt = a.meta[t];
-  const int nch = mt.y, BR = mt.z;
-  if (nch <= 1) return;
-  const int rr = mt.w * a.group + h % a.group, tile = rr / BR;
-  const int64_t pr0 = mt.x + ((int64_t)tile * nch * a.dm.n_kv + h / a.group) * BR + rr % BR;
-  const int64_t step = (int64_t)a.dm.n_kv * BR;
-  __shared__ float so[kAttnWaves][HD], sl[kAttnWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float top = kAttnNone;
-  for (int p = lane; p < nch; p += 64) top = fmaxf(top, a.part_ml[2 * (pr0 + p * step)]);
-  top = wave_max(top);
-  float den = 0.f, y[E] = {};
-#pragma unroll 4
-  for (int p = wave; p < nch; p += kAttnWaves) {
-    const int64_t pr = pr0 + p * step;
-    const float lp = a.part_ml[2 * pr + 1];
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * pr] - top);
-    den = fmaf(lp, f, den);
+  const int64_t item = WAVES == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  const int64_t t = item / n_q;
+  const int h = (int)(item - t * n_q);
+  if (t >= a.T) return;
+  const int kvh = h / a.group;
+  const int c0 = a.cu_q[0], c1 = a.cu_q[a.R];
+  const int4 mt = a.meta[t * a.group + h - kvh * a.group];
+  if (t < c0 || t >= c1 || mt.y <= 1) return;
+  const int parts = mt.y;
+  auto row_of = [&](int p) { return mt.x + (int64_t)kvh * mt.w + (int64_t)mt.z * max(2 * p - 1, 0); };
+  float top = kAttnNone, den = 0.f, y[E] = {};
+  for (int base = 0; base < parts; base += 64) {
+    // a lane for a part: references and sums; then the parts' rows by their weights
+    const bool in = base + lane < parts;
+    const int64_t mine = row_of(min(base + lane, parts - 1));
+    const float r = in ? a.part_ml[2 * mine] : kAttnNone, l = in ? a.part_ml[2 * mine + 1] : 0.f;
+    const float nt = fmaxf(top, wave_max(r)), keep = __builtin_amdgcn_exp2f(top - nt);
+    const float f = __builtin_amdgcn_exp2f(r - nt);
+    top = nt;
+    den = fmaf(den, keep, wave_sum(f * l));
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = fmaf(a.part[pr * HD + lane * E + e], f, y[e]);
+    for (int e = 0; e < E; ++e) y[e] *= keep;
+    const int n = min(64, parts - base);
+#pragma unroll 8
+    for (int p = WAVES == 4 ? wave : 0; p < n; p += WAVES) {
+      const float fp = __shfl(f, p, 64);
+      const float* row = a.part + row_of(base + p) * HD + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] = fmaf(row[e], fp, y[e]);
+    }
   }
+  uint16_t* const dst = a.out + t * a.out_stride + (int64_t)h * HD;
+  if constexpr (WAVES == 4) {
+    __shared__ float so[4][HD];
 #pragma unroll
-  for (int e = 0; e < E; ++e) so[wave][lane * E + e] = y[e];
-  if (lane == 0) sl[wave] = den;
-  __syncthreads();
-  den = sl[0] + sl[1] + sl[2] + sl[3];
-  for (int d = threadIdx.x; d < HD; d += 256) {
-    const float v = so[0][d] + so[1][d] + so[2][d] + so[3][d];
-    a.out[(int64_t)t * a.out_stride + (int64_t)h * HD + d] = T::from_f32(den != 0.f ? v / den : 0.f);
+    for (int e = 0; e < E; ++e) so[wave][lane * E + e] = y[e];
+    __syncthreads();
+    for (int d = threadIdx.x; d < HD; d += 256)
+      dst[d] = T::from_f32(den != 0.f ? (so[0][d] + so[1][d] + so[2][d] + so[3][d]) / den : 0.f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) dst[lane * E + e] = T::from_f32(den != 0.f ? y[e] / den : 0.f);
   }
 }
 
@@ -673,17 +808,17 @@ using namespace cek;
 
 namespace {
 
-// What the host knows of a call: which kernels, their tiles and how the keys are
-// split.  Requests with more than kAttnFewRows rows (query tokens x heads of a kv
-// head) go to the kernel whose waves have rows of their own.
+// What the host knows of a call: which kernels, their tiles, and whether the keys
+// are shared.  Requests with more than kAttnFewRows rows (query tokens x heads of a
+// kv head) go to the kernel whose waves have rows of their own.
 constexpr int kAttnFewRows = 64;
-constexpr int kAttnSplitWgs = 512;  // workgroups to split the keys for
+constexpr int kAttnCus = 256;
 
 struct AttnPlan {
   bool few, many;
   int qt_few, qt_many;
-  int64_t items_few, items_many;  // bounds of the work items per kv head
-  int target_few, target_many;    // 0: the keys stay whole
+  int64_t tiles_few, tiles_many;  // bounds of the row tiles per kv head
+  int wgs_few, wgs_many;          // workgroups per kv head that share the keys; 0: one for each tile
   int64_t part_rows_few, part_rows;
   int64_t bytes;
 };
@@ -694,25 +829,25 @@ AttnPlan attn_plan(int64_t T, int64_t R, int64_t n_q, int64_t n_kv, int64_t hd, 
   if (max_q_len <= 0 || max_q_len > T) max_q_len = T;
   const int64_t rows = max_q_len * group;
   p.many = rows > kAttnFewRows;
-  p.few = !p.many || R > 1;
+  // (all requests of one length: none for it)
+  p.few = !p.many || T < R * max_q_len;
   const int64_t few_rows = p.many ? group : rows;  // of a request, as a rule
   p.qt_few = few_rows <= 16 || hd == 256 ? 1 : 2;
   p.qt_many = hd == 256 ? 1 : 2;
   const int64_t seqs = std::min(R, T);
-  p.items_few = T * group / (16 * p.qt_few) + seqs;
-  if (p.many) p.items_few = std::min(p.items_few, seqs * (kAttnFewRows / (16 * p.qt_few)));
-  p.items_many = T * group / (64 * p.qt_many) + seqs;
+  p.tiles_few = T * group / (16 * p.qt_few) + seqs;
+  if (p.many) p.tiles_few = std::min(p.tiles_few, seqs * (kAttnFewRows / (16 * p.qt_few)));
+  p.tiles_many = T * group / (64 * p.qt_many) + seqs;
+  // As many workgroups as the CUs hold at once, each with an equal share of all
+  // keys.  Not for short keys, where joining the parts would take longer than
+  // they, nor for more row tiles than workgroups of the kernel for many rows.
   const bool long_keys = max_kv_len <= 0 || max_kv_len > 256;
-  auto target = [&](int64_t items) {
-    return long_keys && items * n_kv < 4 * kAttnSplitWgs ? (int)std::max<int64_t>(1, (kAttnSplitWgs + n_kv - 1) / n_kv) : 0;
-  };
-  if (p.few) p.target_few = target(p.many ? seqs : p.items_few);
-  if (p.many) p.target_many = target(p.items_many);
-  p.items_few += p.target_few;
-  p.items_many += p.target_many;
-  p.part_rows_few = p.target_few ? p.items_few * n_kv * 16 * p.qt_few : 0;
-  p.part_rows = p.part_rows_few + (p.target_many ? p.items_many * n_kv * 64 * p.qt_many : 0);
-  if (p.target_few || p.target_many) p.bytes = p.part_rows * (hd + 2) * 4 + T * 16;
+  if (p.few && long_keys) p.wgs_few = (int)std::max<int64_t>(1, kAttnCus * attn_held((int)hd, p.qt_few) / n_kv);
+  if (p.many && long_keys && p.tiles_many * n_kv < 2 * kAttnCus)
+    p.wgs_many = (int)std::max<int64_t>(1, 2 * kAttnCus / n_kv);
+  p.part_rows_few = (int64_t)2 * p.wgs_few * n_kv * 16 * p.qt_few;
+  p.part_rows = p.part_rows_few + (int64_t)2 * p.wgs_many * n_kv * 64 * p.qt_many;
+  if (p.part_rows > 0) p.bytes = p.part_rows * (hd + 2) * 4 + T * group * 16;
   return p;
 }
 
@@ -722,9 +857,9 @@ void launch_attn(const AttnPlan& p, Kv4AttnArgs a, int64_t n_kv, int64_t n_q, hi
     Kv4AttnArgs b = a;
     b.rows_above = 0;
     b.rows_upto = p.many ? kAttnFewRows : INT32_MAX;
-    b.target = p.target_few;
+    b.wgs = p.wgs_few;
     b.part_row0 = 0;
-    const dim3 grid((unsigned)p.items_few, (unsigned)n_kv);
+    const dim3 grid((unsigned)(p.wgs_few ? p.wgs_few : p.tiles_few), (unsigned)n_kv);
     if (p.qt_few == 1) kv4_attn_kernel<T, HD, 1, true><<<grid, 256, 0, st>>>(b);
     else if constexpr (HD != 256) kv4_attn_kernel<T, HD, 2, true><<<grid, 256, 0, st>>>(b);
   }
@@ -732,13 +867,15 @@ void launch_attn(const AttnPlan& p, Kv4AttnArgs a, int64_t n_kv, int64_t n_q, hi
     Kv4AttnArgs b = a;
     b.rows_above = p.few ? kAttnFewRows : 0;
     b.rows_upto = INT32_MAX;
-    b.target = p.target_many;
+    b.wgs = p.wgs_many;
     b.part_row0 = (int)p.part_rows_few;
-    const dim3 grid((unsigned)p.items_many, (unsigned)n_kv);
+    const dim3 grid((unsigned)(p.wgs_many ? p.wgs_many : p.tiles_many), (unsigned)n_kv);
     kv4_attn_kernel<T, HD, HD == 256 ? 1 : 2, false><<<grid, 256, 0, st>>>(b);
   }
-  if (p.target_few || p.target_many) {
-    kv4_attn_join_kernel<T, HD><<<dim3((unsigned)a.T, (unsigned)n_q), 256, 0, st>>>(a);
+  if (p.part_rows > 0) {
+    const int64_t rows = a.T * n_q;
+    if (rows <= 1024) kv4_attn_join_kernel<T, HD, 4><<<(unsigned)rows, 256, 0, st>>>(a, (int)n_q);
+    else kv4_attn_join_kernel<T, HD, 1><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a, (int)n_q);
   }
 }
 
@@ -788,15 +925,15 @@ extern "C" int cek_kv4_attention(const void* q, const void* cache, const int32_t
   a.vec_out = aligned(out, 8) && out_stride % 4 == 0;
   AttnPlan p = attn_plan(T, R, n_q, n_kv, hd, max_q_len, max_kv_len);
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) {
-    p.items_few -= p.target_few;
-    p.items_many -= p.target_many;
-    p.target_few = p.target_many = 0;
+    p.wgs_few = p.wgs_many = 0;  // whole keys
+    p.part_rows = 0;
   } else if (p.bytes > 0) {
     a.part = static_cast<float*>(workspace);
     a.part_ml = a.part + p.part_rows * hd;
     a.meta = reinterpret_cast<int4*>(a.part_ml + p.part_rows * 2);
   }
-  if (p.items_few > INT32_MAX || p.items_many > INT32_MAX || p.part_rows > INT32_MAX) return CEK_ERR_UNSUPPORTED;
+  if (p.tiles_few > INT32_MAX || p.tiles_many > INT32_MAX || p.part_rows > INT32_MAX || T * n_q > INT32_MAX)
+    return CEK_ERR_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
 #define CEK_GO(D)                                                       \
   do {                                                                  \
