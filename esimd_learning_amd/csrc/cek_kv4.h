@@ -66,6 +66,7 @@ inline int kv4_dims(int64_t n_kv, int64_t hd, int64_t bs, int64_t num_blocks, in
   if (n_kv <= 0 || n_kv > 4096 || num_blocks <= 0 || num_blocks > INT32_MAX) return CEK_ERR_INVALID;
   if (hd != 64 && hd != 128 && hd != 256) return CEK_ERR_UNSUPPORTED;
   if (bs < 16 || bs > 256 || (bs & (bs - 1))) return CEK_ERR_UNSUPPORTED;
+  if (block_stride > UINT32_MAX) return CEK_ERR_UNSUPPORTED;
   if (block_stride % 16 || block_stride < n_kv * kv4_head_bytes((int)bs, (int)hd)) return CEK_ERR_INVALID;
   dm = Kv4Dims{block_stride, (int)num_blocks, (int)n_kv, __builtin_ctzll((unsigned long long)bs)};
   return CEK_OK;

@@ -170,8 +170,8 @@ struct Kv4List {
   }
 };
 
-// Parameters of 16 tokens that do not exist.
-__device__ const uint8_t kv4_zeros[64] __attribute__((aligned(16))) = {};
+// Parameters of tokens that do not exist: K's and, 4 bs bytes on, V's.
+__device__ const uint8_t kv4_zeros[4 * 256 + 64] __attribute__((aligned(16))) = {};
 
 __device__ inline uint32_t pack_h2(float a, float b) {
   return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});
@@ -179,50 +179,57 @@ __device__ inline uint32_t pack_h2(float a, float b) {
 
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
-// One load instruction straight to LDS: N bytes a lane, lane after lane from `to`.
-template <int N>
-__device__ inline void load_lds(const uint8_t* from, uint8_t* to) {
-  static_assert(N == 4 || N == 16, "bytes a lane");
-  if constexpr (N == 16) __builtin_amdgcn_global_load_lds(from, (lds_ptr_t)to, 16, 0, 0);
-  else __builtin_amdgcn_global_load_lds(from, (lds_ptr_t)to, 4, 0, 0);
+__device__ inline __amdgpu_buffer_rsrc_t kv4_rsrc(const uint8_t* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, bytes, 0x00020000);
 }
 __device__ inline uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(lds_ptr_t)p; }
 
-// LDS reads behind a wave's own direct loads.  In asm, each with its wait: the
-// compiler would wait for every direct load in flight before any LDS read.
-template <int O0, int O1, int O2, int O3>
-__device__ inline void lds_read4(uint32_t at, u4& a, u4& b, u4& c, u4& d) {
-  asm volatile(
-      "ds_read_b128 %0, %4 offset:%5\n\tds_read_b128 %1, %4 offset:%6\n\t"
-      "ds_read_b128 %2, %4 offset:%7\n\tds_read_b128 %3, %4 offset:%8\n\ts_waitcnt lgkmcnt(0)"
-      : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
-      : "v"(at), "n"(O0), "n"(O1), "n"(O2), "n"(O3)
-      : "memory");
-}
-// A lane's codes of 32 tokens, 16 and 16, from byte OFF of a slot on.
-template <int HD, int OFF>
+// LDS reads behind a wave's own direct loads, in asm with their wait: the compiler
+// would wait for every direct load in flight before any LDS read.  A lane's
+// codes of 32 tokens (K or V: two loads of 16 tokens, HALF bytes apart) and the
+// parameters of its tokens (one or two loads each).
+template <int HD, int HALF>
 __device__ inline void read_codes(uint32_t at, uint32_t (&to)[2][HD / 32]) {
   if constexpr (HD == 64) {
     u2 a, b;
-    asm volatile("ds_read_b64 %0, %2 offset:%3\n\tds_read_b64 %1, %2 offset:%4\n\ts_waitcnt lgkmcnt(0)"
+    asm volatile("ds_read_b64 %0, %2\n\tds_read_b64 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
                  : "=&v"(a), "=&v"(b)
-                 : "v"(at), "n"(OFF), "n"(OFF + 512)
+                 : "v"(at), "n"(HALF)
                  : "memory");
     to[0][0] = a[0], to[0][1] = a[1], to[1][0] = b[0], to[1][1] = b[1];
   } else if constexpr (HD == 128) {
     u4 a, b;
-    asm volatile("ds_read_b128 %0, %2 offset:%3\n\tds_read_b128 %1, %2 offset:%4\n\ts_waitcnt lgkmcnt(0)"
+    asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
                  : "=&v"(a), "=&v"(b)
-                 : "v"(at), "n"(OFF), "n"(OFF + 1024)
+                 : "v"(at), "n"(HALF)
                  : "memory");
 #pragma unroll
     for (int e = 0; e < 4; ++e) to[0][e] = a[e], to[1][e] = b[e];
   } else {
     u4 x[4];
-    lds_read4<OFF, OFF + 1024, OFF + 2048, OFF + 3072>(at, x[0], x[1], x[2], x[3]);
+    asm volatile(
+        "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\t"
+        "ds_read_b128 %2, %4 offset:%5\n\tds_read_b128 %3, %4 offset:%6\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+        : "v"(at), "n"(HALF), "n"(HALF + 1024)
+        : "memory");
 #pragma unroll
     for (int e = 0; e < 16; ++e) to[e / 8][e % 8] = x[e / 4][e % 4];
   }
+}
+__device__ inline void read_params(uint32_t at, u4 (&k)[2], u4 (&v)[2]) {
+  asm volatile(
+      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:64\n\t"
+      "ds_read_b128 %2, %4 offset:128\n\tds_read_b128 %3, %4 offset:192\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(k[0]), "=&v"(k[1]), "=&v"(v[0]), "=&v"(v[1])
+      : "v"(at)
+      : "memory");
+}
+__device__ inline void read_params(uint32_t at, u4 (&k)[1], u4 (&v)[1]) {
+  asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:128\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(k[0]), "=&v"(v[0])
+               : "v"(at)
+               : "memory");
 }
 
 // Workgroups that a CU holds at once (waves a SIMD): by registers and LDS.
@@ -230,16 +237,22 @@ constexpr int attn_held(int hd, int qt) { return hd == 256 ? 2 : (hd == 64 ? 5 -
 
 // KVSPLIT: the workgroup's four waves share QT x 16 rows and take every fourth 32
 // tokens each; else each wave has QT x 16 rows of its own and all the tokens.
-template <typename T, int HD, int QT, bool KVSPLIT>
+// FOLD: tiles of 8 rows, in the MFMA's columns twice, so that columns 0 .. 7 have
+// the scores of the first 16 tokens at hand and columns 8 .. 15 those of the second
+// 16: half the arithmetic between the two products.
+template <typename T, int HD, int QT, bool KVSPLIT, bool FOLD>
 __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4AttnArgs a) {
   constexpr int ND = HD / 32;                    // 32-bit words per lane, part and 16 tokens
   constexpr int NP = HD >= 128 ? HD / 128 : 1;   // parts of a row: 128 values, or 64
   constexpr int NH = HD >= 128 ? 2 : 1;          // runs of four values per lane and part
   constexpr int PW = HD / NP;                    // values of a part
-  constexpr int BR = QT * 16 * (KVSPLIT ? 1 : kAttnWaves);
+  constexpr int RT = FOLD ? 8 : 16;              // rows of a tile
+  constexpr int NX = FOLD ? 1 : 2;               // groups of four tokens a lane has scores of
+  constexpr int BR = QT * RT * (KVSPLIT ? 1 : kAttnWaves);
   constexpr int LSTR = HD + 4;                   // LDS row stride: rows 4 banks apart
   constexpr int CODES = HD >= 128 ? 4 * NP * 1024 : 2048;  // bytes of 32 tokens' codes
   constexpr int SLOT = CODES + 256;                        // and parameters
+  constexpr int HALF = CODES / 2;                          // 16 tokens: K codes, V codes
   constexpr int DEPTH = HD == 256 ? 2 : 3;                 // slots a wave
   constexpr int LOADS = CODES / 1024 + 1;                  // load instructions of a slot
   constexpr int OUT_BYTES = KVSPLIT ? kAttnWaves * 16 * (LSTR + 2) * 4 : 0;
@@ -262,7 +275,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     u_end = list.begin_of(blockIdx.x + 1);
   }
   for (Kv4Work w; u < u_end && list.find(mine, u, u_end, w); u += w.units) {
-  const int row0 = w.tile * BR + (KVSPLIT ? 0 : wave * QT * 16);  // this wave's first row in the request
+  const int row0 = w.tile * BR + (KVSPLIT ? 0 : wave * QT * RT);  // this wave's first row in the request
   // Partial rows: of a tile's first stretch in 2 wg + 1, of the others in 2 wg.
   const bool whole = w.units == w.all;
   const int64_t part0 =
@@ -281,15 +294,15 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   bool real[QT];
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
-    const int rr = row0 + i * 16 + c;
+    const int rr = row0 + i * RT + (FOLD ? c & 7 : c);
     real[i] = rr < w.rows;
     const int t = rr / a.group, h = kvh * a.group + rr % a.group;
     qsrc[i] = a.q + (int64_t)(w.q0 + (real[i] ? t : 0)) * a.q_stride + (int64_t)(real[i] ? h : 0) * HD;
     pos[i] = real[i] ? w.kv - w.n_new + t : INT32_MAX - 1;
-    if (row0 + i * 16 < w.rows) {
+    if (row0 + i * RT < w.rows) {
       // uniform: rows are in order of position
-      pmin = uniform(min(pmin, w.kv - w.n_new + (row0 + i * 16) / a.group));
-      pmax = uniform(max(pmax, w.kv - w.n_new + (min(row0 + i * 16 + 16, w.rows) - 1) / a.group));
+      pmin = uniform(min(pmin, w.kv - w.n_new + (row0 + i * RT) / a.group));
+      pmax = uniform(max(pmax, w.kv - w.n_new + (min(row0 + i * RT + RT, w.rows) - 1) / a.group));
     }
   }
   const int window = a.window > 0 ? a.window : INT32_MAX;  // pos - window stays in range
@@ -304,56 +317,45 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   // Each wave keeps the next DEPTH tiles' loads in flight without a register: a
   // lane reads back what it loaded itself (the codes), so that nothing but the
   // wave's own vmcnt orders the two.
-  const uint8_t* head = a.cache + (int64_t)kvh * kv4_head_bytes(bs, HD);
+  const int head_bytes = kv4_head_bytes(bs, HD);
+  const uint8_t* head = a.cache + (int64_t)kvh * head_bytes;
   const const_i32 table = (const_i32)(uintptr_t)(a.tables + (int64_t)w.r * a.table_stride);
   struct Blocks { int b[2]; };
   auto blocks_of = [&](int t0) {
     return Blocks{{table[t0 >> a.dm.bs_log2], table[min(t0 + 16, w.kv - 1) >> a.dm.bs_log2]}};
   };
-  // Does the first or second half of the 32 tokens at t0 lie in no block?  (The
-  // second one may lie behind the last key.)
-  auto outside = [&](int t0, const Blocks& x, int h) {
-    return ((uint32_t)x.b[h] >= (uint32_t)a.dm.num_blocks) | (t0 + 16 * h >= w.kv);
-  };
   uint8_t* const ring = lds + wave * (DEPTH * SLOT);
-  const int half = HD >= 128 ? 0 : lane >> 5;  // hd 64: the 32 tokens' codes in one load
-  const uint32_t k_lane = HD >= 128 ? c * (HD / 2) + g * 16 : (lane & 31) * 16;
-  const uint32_t v_lane = kv4_v_codes(bs, HD) + (HD >= 128 ? g * HD * 2 + c * 16 : (lane & 31) * 16);
-  const uint32_t p_lane = (g >> 1 ? kv4_v_params(bs, HD) : kv4_k_params(bs, HD)) + 4 * c;
-  // returns which halves lie in no block
+  // hd 64: K and V of 16 tokens in one load, 32 lanes each
+  const uint32_t k_lane = HD >= 128 ? c * (HD / 2) + g * 16 : (lane & 31) * 16 + (lane >> 5) * kv4_v_codes(bs, HD);
+  const uint32_t v_lane = kv4_v_codes(bs, HD) + g * HD * 2 + c * 16;
+  // parameters, 16 lanes each: K's of the first and the second 16 tokens, V's
+  const uint32_t p_lane = (g & 2 ? 4 * bs : 0) + 4 * c;
+  // The 32 tokens at t0 into a slot; returns which halves lie in no block (bits 0
+  // and 1; the second one may lie behind the last key).  No code is read there (the
+  // buffer has no bytes) and the parameters are 0.
   auto fetch = [&](int t0, const Blocks& x, int slot) -> int {
     uint8_t* const to = ring + slot * SLOT;
-    const uint8_t* base[2];  // a block outside the cache holds no token: block 0 is read in its place
-    int tok[2];
-    bool out[2];
+    int outs = 0;
+    const uint8_t* par[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      tok[h] = (t0 + 16 * h) & (bs - 1);
-      out[h] = outside(t0, x, h);
-      base[h] = head + (int64_t)(out[h] ? 0 : x.b[h]) * a.dm.block_stride;
+      const bool out = ((uint32_t)x.b[h] >= (uint32_t)a.dm.num_blocks) | (t0 + 16 * h >= w.kv);
+      outs |= (int)out << h;
+      const uint64_t at = (uint64_t)(uint32_t)(out ? 0 : x.b[h]) * (uint32_t)a.dm.block_stride;
+      const auto src = kv4_rsrc(head + at, out ? 0 : head_bytes);
+      const int tok = (t0 + 16 * h) & (bs - 1);
+#define CEK_FETCH(lane_off, dst, bytes, off) \
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_ptr_t)(dst), bytes, lane_off, off, 0, 0)
+      // a part of 128 values and 16 tokens: 64 bytes of each K row, 256 of each four tokens of V
+      CEK_FETCH(k_lane, to + h * HALF, 16, tok * (HD / 2));
+      if constexpr (HD == 256) CEK_FETCH(k_lane, to + h * HALF + 1024, 16, tok * (HD / 2) + 64);
+      if constexpr (HD >= 128) CEK_FETCH(v_lane, to + h * HALF + NP * 1024, 16, tok * (HD / 2));
+      if constexpr (HD == 256) CEK_FETCH(v_lane, to + h * HALF + 3072, 16, tok * (HD / 2) + 256);
+#undef CEK_FETCH
+      par[h] = out ? kv4_zeros : head + at + kv4_k_params(bs, HD) + 4 * tok;
     }
-    if constexpr (HD >= 128) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          // part p of 16 tokens: 64 bytes of each K row, 256 of each four tokens of V
-          load_lds<16>(base[h] + tok[h] * (HD / 2) + p * (PW / 2) + k_lane, to + (h * NP + p) * 1024);
-          load_lds<16>(base[h] + tok[h] * (HD / 2) + p * (PW * 2) + v_lane, to + ((2 + h) * NP + p) * 1024);
-        }
-    } else {
-      const uint8_t* b = half ? base[1] + tok[1] * (HD / 2) : base[0] + tok[0] * (HD / 2);
-      load_lds<16>(b + k_lane, to);
-      load_lds<16>(b + v_lane, to + 1024);
-    }
-    // lanes 16 x (K, V) .. : parameters of the first and the second 16 tokens; 0
-    // for tokens that do not exist, whatever lies in block 0
-    const uint8_t* zeros = kv4_zeros;
-    const uint8_t* b0 = out[0] ? zeros : base[0] + 4 * tok[0];
-    const uint8_t* b1 = out[1] ? zeros : base[1] + 4 * tok[1];
-    const uint32_t o0 = out[0] ? 4 * c : p_lane, o1 = out[1] ? 4 * c : p_lane;
-    load_lds<4>((g & 1 ? b1 : b0) + (g & 1 ? o1 : o0), to + CODES);
-    return (int)out[0] + 2 * (int)out[1];
+    __builtin_amdgcn_global_load_lds((g & 1 ? par[1] : par[0]) + p_lane, (lds_ptr_t)(to + CODES), 4, 0, 0);
+    return outs;
   };
   const int last = begin + (end - 1 - begin) / STEP * STEP;
   Blocks nb;                       // of the tile DEPTH ahead
@@ -434,29 +436,35 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     for (int x = 0; x < NP * NH * 4; ++x) o[i][x / (NH * 4)][x / 4 % NH][x % 4] = f4{0.f, 0.f, 0.f, 0.f};
   }
 
-  auto sees = [&](int i, int t0, int h, int e) {  // row c of tile i the token 16 h + 4 g + e at t0
-    const int t = t0 + 16 * h + 4 * g + e;
+  auto token = [&](int h, int e) { return 16 * (FOLD ? c >> 3 : h) + 4 * g + e; };
+  auto sees = [&](int i, int t0, int h, int e) {  // this lane's row of tile i that token at t0
+    const int t = t0 + token(h, e);
     return (t <= pos[i]) & (t < end) & (t > pos[i] - window);  // no branches
   };
 
   uint32_t kc[2][ND], vc[2][ND];  // the codes of 32 tokens, 16 and 16
-  u4 kp[2], vp[2];                // their parameters, of tokens 4 g ..
-  float none[2];                  // 0, or -infinity where the block lies outside the cache
+  u4 kp[NX], vp[NX];              // the parameters of this lane's tokens, 4 g .. of 16
+  float none[NX];                 // 0, or -infinity where those lie in no block
   int slot = 0;
-  const uint32_t lds_codes = lds_offset(ring) + (HD >= 128 ? lane * 16 : c * 32 + g * 8);
-  const uint32_t lds_words = lds_offset(ring) + (HD >= 128 ? lane * 16 : lane * 8);
-  const uint32_t lds_par = lds_offset(ring) + CODES + 16 * g;
+  const uint32_t ring_at = lds_offset(ring);
+  const uint32_t k_at = ring_at + (HD >= 128 ? lane * 16 : c * 32 + g * 8);
+  const uint32_t v_at = ring_at + (HD >= 128 ? NP * 1024 + lane * 16 : 512 + lane * 8);
+  const uint32_t p_at = ring_at + CODES + 16 * g + (FOLD ? (c >> 3) * 64 : 0);
   // The present tile from its slot: K codes and parameters once they are there,
   // V codes later, and then the slot to the tile DEPTH ahead.
   auto read_k = [&]() {
     wait_vmcnt<(DEPTH - 1) * LOADS>();
     const uint32_t at = slot * SLOT;
-    none[0] = outs & 1 ? -INFINITY : 0.f;
-    none[1] = outs & 2 ? -INFINITY : 0.f;
-    lds_read4<0, 64, 128, 192>(lds_par + at, kp[0], kp[1], vp[0], vp[1]);
-    read_codes<HD, 0>(lds_codes + at, kc);
+    if constexpr (FOLD) {
+      none[0] = outs >> (c >> 3) & 1 ? -INFINITY : 0.f;
+    } else {
+      none[0] = outs & 1 ? -INFINITY : 0.f;
+      none[1] = outs & 2 ? -INFINITY : 0.f;
+    }
+    read_params(p_at + at, kp, vp);
+    read_codes<HD, HALF>(k_at + at, kc);
   };
-  auto read_v = [&]() { read_codes<HD, (HD >= 128 ? CODES / 2 : 1024)>(lds_words + slot * SLOT, vc); };
+  auto read_v = [&]() { read_codes<HD, HALF>(v_at + slot * SLOT, vc); };
   auto refill = [&](int t0) {
     const Blocks nx = nb;
     nb = blocks_of(min(t0 + (DEPTH + 1) * STEP, last));  // a tile ahead of the loads that need them
@@ -465,15 +473,15 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   };
 
   // Scores of 32 tokens: x (exponents / qmul), their maxima xm and that of the V steps.
-  float x[QT][2][4], xm[QT], top;
+  float x[QT][NX][4], xm[QT], top;
   auto scores = [&](int t0, auto mask) {
     constexpr bool masked = decltype(mask)::value;
     if constexpr (masked) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < NX; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool out = t0 + 16 * h + 4 * g + e >= end;  // no token: whatever lies there
+          const bool out = t0 + token(h, e) >= end;  // no token: whatever lies there
           kp[h][e] = out ? 0u : kp[h][e];
           vp[h][e] = out ? 0u : vp[h][e];
         }
@@ -495,8 +503,14 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     top = -1.f;
 #pragma unroll
     for (int i = 0; i < QT; ++i) xm[i] = -INFINITY;
+    if constexpr (FOLD) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+      for (int i = 0; i < QT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][0][e] = c < 8 ? acc[i][0][e] : acc[i][1][e];
+    }
+#pragma unroll
+    for (int h = 0; h < NX; ++h) {
       float xh[QT];
 #pragma unroll
       for (int i = 0; i < QT; ++i) xh[i] = -INFINITY;
@@ -521,17 +535,21 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     for (int i = 0; i < QT; ++i) y = y | (xm[i] * qmul[i] > m[i] + (float)kAttnHead);
     return __any(y);
   };
+  // Over the lanes that hold one row.
+  auto over_row = [&](float v, auto op) {
+    if constexpr (FOLD) v = op(v, __shfl_xor(v, 8, 64));
+    v = op(v, __shfl_xor(v, 16, 64));
+    return op(v, __shfl_xor(v, 32, 64));
+  };
   // New references, and the sums so far brought to them.
   auto rescale = [&]() {
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    top = over_row(top, [](float p, float q) { return fmaxf(p, q); });
     ev = max(ev, (int)((__float_as_uint(fmaxf(top, 0.f)) >> 23) & 255) - 126);
     sv_top = __uint_as_float((uint32_t)(ev + 127) << 23);
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
       float t = fmaxf(m[i], xm[i] * qmul[i]);
-      t = fmaxf(t, __shfl_xor(t, 16, 64));
-      t = fmaxf(t, __shfl_xor(t, 32, 64));
+      t = over_row(t, [](float p, float q) { return fmaxf(p, q); });
       m[i] = t;
       const float nr = t + (float)(ev - kAttnBase);
       const float f = __builtin_amdgcn_exp2f(ref[i] - nr);
@@ -552,7 +570,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     constexpr bool masked = decltype(mask)::value;
     u4 pf[QT];  // the weights times sv, fp16: tokens 4 g .. of both halves
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < NX; ++h) {
       float pv[QT][4], off[QT];
 #pragma unroll
       for (int i = 0; i < QT; ++i) off[i] = none[h] - ref[i];
@@ -579,6 +597,13 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
         pf[i][2 * h] = pack_h2(pv[i][0], pv[i][1]);
         pf[i][2 * h + 1] = pack_h2(pv[i][2], pv[i][3]);
       }
+    }
+    if constexpr (FOLD) {
+      // the other half's weights, of columns 0 .. 7 (8 .. 15 hold nothing that is used)
+#pragma unroll
+      for (int i = 0; i < QT; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) pf[i][2 + e] = __builtin_amdgcn_mov_dpp(pf[i][e], 0x128, 0xF, 0xF, true);  // row_ror 8
     }
     read_v();
     refill(t0);
@@ -633,10 +658,8 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   // ---- the end: sums over the lanes of a row, parts to the workspace, rows out ----
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
-    l[i] += __shfl_xor(l[i], 16, 64);
-    l[i] += __shfl_xor(l[i], 32, 64);
-    z[i] += __shfl_xor(z[i], 16, 64);
-    z[i] += __shfl_xor(z[i], 32, 64);
+    l[i] = over_row(l[i], [](float p, float q) { return p + q; });
+    z[i] = over_row(z[i], [](float p, float q) { return p + q; });
     const float off = z[i] - wsum[i][0];  // every row of the MFMA's result holds 7.5 sum(P sv)
     // lane (c, g): values p PW + g PW / 4 + 4 NH e + 4 h + b of row c
     auto value = [&](int p, int e, int h, int b) {
@@ -659,7 +682,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
       __syncthreads();
       // thread (row, sixteenth of the row)
       const int row = threadIdx.x >> 4, seg = threadIdx.x & 15;
-      const int rr = w.tile * BR + i * 16 + row;
+      const int rr = w.tile * BR + i * RT + row;
       float top = kAttnNone, den = 0.f, y[HD / 16] = {};
 #pragma unroll
       for (int v = 0; v < kAttnWaves; ++v) top = fmaxf(top, lds_ml[(v * 16 + row) * 2]);
@@ -675,9 +698,9 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
           for (int b = 0; b < 4; ++b) y[e + b] = fmaf(s[b], f, y[e + b]);
         }
       }
-      if (rr < w.rows) {
+      if (row < RT && rr < w.rows) {
         if (!whole) {
-          const int64_t pr = part0 + i * 16 + row;
+          const int64_t pr = part0 + i * RT + row;
 #pragma unroll
           for (int e = 0; e < HD / 16; e += 4)
             *reinterpret_cast<f4*>(a.part + pr * HD + seg * (HD / 16) + e) = f4{y[e], y[e + 1], y[e + 2], y[e + 3]};
@@ -704,10 +727,10 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
         }
       }
     } else {
-      const int rr = row0 + i * 16 + c;
-      if (rr < w.rows) {
+      const int rr = row0 + i * RT + c;
+      if (c < RT && rr < w.rows) {
         if (!whole) {
-          const int64_t pr = part0 + wave * QT * 16 + i * 16 + c;
+          const int64_t pr = part0 + wave * QT * RT + i * RT + c;
 #pragma unroll
           for (int p = 0; p < NP; ++p)
 #pragma unroll
@@ -816,6 +839,7 @@ constexpr int kAttnCus = 256;
 
 struct AttnPlan {
   bool few, many;
+  bool fold;                      // tiles of 8 rows in the kernel for few rows
   int qt_few, qt_many;
   int64_t tiles_few, tiles_many;  // bounds of the row tiles per kv head
   int wgs_few, wgs_many;          // workgroups per kv head that share the keys; 0: one for each tile
@@ -832,11 +856,13 @@ AttnPlan attn_plan(int64_t T, int64_t R, int64_t n_q, int64_t n_kv, int64_t hd, 
   // (all requests of one length: none for it)
   p.few = !p.many || T < R * max_q_len;
   const int64_t few_rows = p.many ? group : rows;  // of a request, as a rule
+  p.fold = few_rows <= 8;
   p.qt_few = few_rows <= 16 || hd == 256 ? 1 : 2;
+  const int64_t br_few = p.fold ? 8 : 16 * p.qt_few;
   p.qt_many = hd == 256 ? 1 : 2;
   const int64_t seqs = std::min(R, T);
-  p.tiles_few = T * group / (16 * p.qt_few) + seqs;
-  if (p.many) p.tiles_few = std::min(p.tiles_few, seqs * (kAttnFewRows / (16 * p.qt_few)));
+  p.tiles_few = T * group / br_few + seqs;
+  if (p.many) p.tiles_few = std::min(p.tiles_few, seqs * (kAttnFewRows / br_few));
   p.tiles_many = T * group / (64 * p.qt_many) + seqs;
   // As many workgroups as the CUs hold at once, each with an equal share of all
   // keys.  Not for short keys, where joining the parts would take longer than
@@ -845,7 +871,7 @@ AttnPlan attn_plan(int64_t T, int64_t R, int64_t n_q, int64_t n_kv, int64_t hd, 
   if (p.few && long_keys) p.wgs_few = (int)std::max<int64_t>(1, kAttnCus * attn_held((int)hd, p.qt_few) / n_kv);
   if (p.many && long_keys && p.tiles_many * n_kv < 2 * kAttnCus)
     p.wgs_many = (int)std::max<int64_t>(1, 2 * kAttnCus / n_kv);
-  p.part_rows_few = (int64_t)2 * p.wgs_few * n_kv * 16 * p.qt_few;
+  p.part_rows_few = (int64_t)2 * p.wgs_few * n_kv * br_few;
   p.part_rows = p.part_rows_few + (int64_t)2 * p.wgs_many * n_kv * 64 * p.qt_many;
   if (p.part_rows > 0) p.bytes = p.part_rows * (hd + 2) * 4 + T * group * 16;
   return p;
@@ -860,8 +886,9 @@ void launch_attn(const AttnPlan& p, Kv4AttnArgs a, int64_t n_kv, int64_t n_q, hi
     b.wgs = p.wgs_few;
     b.part_row0 = 0;
     const dim3 grid((unsigned)(p.wgs_few ? p.wgs_few : p.tiles_few), (unsigned)n_kv);
-    if (p.qt_few == 1) kv4_attn_kernel<T, HD, 1, true><<<grid, 256, 0, st>>>(b);
-    else if constexpr (HD != 256) kv4_attn_kernel<T, HD, 2, true><<<grid, 256, 0, st>>>(b);
+    if (p.fold) kv4_attn_kernel<T, HD, 1, true, true><<<grid, 256, 0, st>>>(b);
+    else if (p.qt_few == 1) kv4_attn_kernel<T, HD, 1, true, false><<<grid, 256, 0, st>>>(b);
+    else if constexpr (HD != 256) kv4_attn_kernel<T, HD, 2, true, false><<<grid, 256, 0, st>>>(b);
   }
   if (p.many) {
     Kv4AttnArgs b = a;
@@ -870,7 +897,7 @@ void launch_attn(const AttnPlan& p, Kv4AttnArgs a, int64_t n_kv, int64_t n_q, hi
     b.wgs = p.wgs_many;
     b.part_row0 = (int)p.part_rows_few;
     const dim3 grid((unsigned)(p.wgs_many ? p.wgs_many : p.tiles_many), (unsigned)n_kv);
-    kv4_attn_kernel<T, HD, HD == 256 ? 1 : 2, false><<<grid, 256, 0, st>>>(b);
+    kv4_attn_kernel<T, HD, HD == 256 ? 1 : 2, false, false><<<grid, 256, 0, st>>>(b);
   }
   if (p.part_rows > 0) {
     const int64_t rows = a.T * n_q;
