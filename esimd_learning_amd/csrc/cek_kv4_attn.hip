@@ -173,6 +173,15 @@ struct Kv4List {
 // Parameters of tokens that do not exist: K's and, 4 bs bytes on, V's.
 __device__ const uint8_t kv4_zeros[4 * 256 + 64] __attribute__((aligned(16))) = {};
 
+// v of lanes l, l ^ 16, l ^ 32, l ^ 48, joined by op.
+template <typename OP>
+__device__ inline float over_rows(float v, OP op) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 __device__ inline uint32_t pack_h2(float a, float b) {
   return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});
 }
@@ -253,7 +262,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   constexpr int CODES = HD >= 128 ? 4 * NP * 1024 : 2048;  // bytes of 32 tokens' codes
   constexpr int SLOT = CODES + 256;                        // and parameters
   constexpr int HALF = CODES / 2;                          // 16 tokens: K codes, V codes
-  constexpr int DEPTH = HD == 256 ? 2 : 3;                 // slots a wave
+  constexpr int DEPTH = 2;                 // slots a wave
   constexpr int LOADS = CODES / 1024 + 1;                  // load instructions of a slot
   constexpr int OUT_BYTES = KVSPLIT ? kAttnWaves * 16 * (LSTR + 2) * 4 : 0;
   constexpr int RING_BYTES = kAttnWaves * DEPTH * SLOT;
@@ -313,6 +322,25 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   constexpr int STEP = KVSPLIT ? 32 * kAttnWaves : 32;
 
 
+
+  // ---- q: this lane's 16-bit values of its row of each tile, in the order of K's
+  // words; on their way while the codes' addresses are found ----
+  uint32_t raw[QT][ND][4];
+#pragma unroll
+  for (int i = 0; i < QT; ++i)
+#pragma unroll
+    for (int n = 0; n < ND; ++n) {
+      const int d0 = (n / (PW / 32)) * PW + g * (PW / 4) + (n % (PW / 32)) * 8;
+      if (a.vec_q) {
+        const u4 x = load_u4(qsrc[i] + d0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[i][n][e] = x[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[i][n][e] = (uint32_t)qsrc[i][d0 + 2 * e] | ((uint32_t)qsrc[i][d0 + 2 * e + 1] << 16);
+      }
+    }
+
   // ---- codes and parameters: through a ring of LDS slots ----
   // Each wave keeps the next DEPTH tiles' loads in flight without a register: a
   // lane reads back what it loaded itself (the codes), so that nothing but the
@@ -369,33 +397,21 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     nb = blocks_of(min(begin + DEPTH * STEP, last));
   }
 
-  // ---- q: this lane's 16-bit values of row c of each tile, in the order of K's words ----
-  u4 qf[QT][ND];        // MFMA operands
+  // ---- q as MFMA operands ----
+  u4 qf[QT][ND];
   float qsum[QT], qmul[QT];
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
-    uint32_t raw[ND][4];
-#pragma unroll
-    for (int n = 0; n < ND; ++n) {
-      const int d0 = (n / (PW / 32)) * PW + g * (PW / 4) + (n % (PW / 32)) * 8;
-      if (a.vec_q) {
-        const u4 x = load_u4(qsrc[i] + d0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) raw[n][e] = real[i] ? x[e] : 0;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          raw[n][e] = real[i] ? (uint32_t)qsrc[i][d0 + 2 * e] | ((uint32_t)qsrc[i][d0 + 2 * e + 1] << 16) : 0;
-      }
-    }
     float top = 0.f;
+    if (!real[i])
+#pragma unroll
+      for (int n = 0; n < 4 * ND; ++n) raw[i][n / 4][n % 4] = 0;
 #pragma unroll
     for (int n = 0; n < ND; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        top = fmaxf(top, fmaxf(fabsf(T::to_f32(raw[n][e] & 0xFFFF)), fabsf(T::to_f32(raw[n][e] >> 16))));
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = fmaxf(top, fmaxf(fabsf(T::to_f32(raw[i][n][e] & 0xFFFF)), fabsf(T::to_f32(raw[i][n][e] >> 16))));
+    top = over_rows(top, [](float p, float q) { return fmaxf(p, q); });
     // the row times 2^k, its largest value in 2^13 .. 2^14: exact in fp16 down to 2^-33 of it
     int k = 0;
     if (top > 0.f) k = min(120, 140 - (int)((__float_as_uint(top) >> 23) & 255));
@@ -406,8 +422,8 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
       float f[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        f[2 * e] = T::to_f32(raw[n][e] & 0xFFFF) * up;
-        f[2 * e + 1] = T::to_f32(raw[n][e] >> 16) * up;
+        f[2 * e] = T::to_f32(raw[i][n][e] & 0xFFFF) * up;
+        f[2 * e + 1] = T::to_f32(raw[i][n][e] >> 16) * up;
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum += f[e];
@@ -415,8 +431,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
       qf[i][n] = u4{pack_h2(f[0], f[4]), pack_h2(f[1] * 0.0625f, f[5] * 0.0625f), pack_h2(f[2], f[6]),
                     pack_h2(f[3] * 0.0625f, f[7] * 0.0625f)};
     }
-    sum += __shfl_xor(sum, 16, 64);
-    sum += __shfl_xor(sum, 32, 64);
+    sum = over_rows(sum, [](float p, float q) { return p + q; });
     qsum[i] = sum * 0x1p-24f;
     qmul[i] = ldexpf(a.scale * 1.4426950408889634f, 24 - k);
   }
@@ -537,9 +552,8 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   };
   // Over the lanes that hold one row.
   auto over_row = [&](float v, auto op) {
-    if constexpr (FOLD) v = op(v, __shfl_xor(v, 8, 64));
-    v = op(v, __shfl_xor(v, 16, 64));
-    return op(v, __shfl_xor(v, 32, 64));
+    if constexpr (FOLD) v = op(v, CEK_DPP_F32(v, 0x128));  // row_ror 8
+    return over_rows(v, op);
   };
   // New references, and the sums so far brought to them.
   auto rescale = [&]() {
@@ -775,12 +789,15 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
 
 // Joins the parts of the rows that several workgroups share.  Part 0 of a row is
 // its first workgroup's, part p that of the p-th after it, two row tiles on each.
-// WAVES waves a row: four where there are few rows with many parts, one else.
-template <typename T, int HD, int WAVES>
+// WIDE: few rows of many parts, a workgroup for 32 values of a row, eight groups of
+// threads taking every eighth part; else a wave for a row.
+template <typename T, int HD, bool WIDE>
 __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4AttnArgs a, int n_q) {
-  constexpr int E = HD / 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t item = WAVES == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  constexpr int G = WIDE ? 8 : 1;         // groups of threads that share the parts
+  constexpr int E = WIDE ? 1 : HD / 64;   // values of a thread
+  constexpr int AHEAD = 8;                // parts of a group that are loaded at once
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t item = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + (tid >> 6);
   const int64_t t = item / n_q;
   const int h = (int)(item - t * n_q);
   if (t >= a.T) return;
@@ -788,40 +805,58 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4AttnArgs a, int n
   const int c0 = a.cu_q[0], c1 = a.cu_q[a.R];
   const int4 mt = a.meta[t * a.group + h - kvh * a.group];
   if (t < c0 || t >= c1 || mt.y <= 1) return;
-  const int parts = mt.y;
-  auto row_of = [&](int p) { return mt.x + (int64_t)kvh * mt.w + (int64_t)mt.z * max(2 * p - 1, 0); };
+  const int parts = mt.y, grp = WIDE ? tid >> 5 : 0;
+  const int d0 = WIDE ? (int)blockIdx.y * 32 + (tid & 31) : lane * E;
+  const int64_t row0 = mt.x + (int64_t)kvh * mt.w;
+  auto row_of = [&](int p) { return row0 + (int64_t)mt.z * (p > 0 ? 2 * p - 1 : 0); };
   float top = kAttnNone, den = 0.f, y[E] = {};
   for (int base = 0; base < parts; base += 64) {
     // a lane for a part: references and sums; then the parts' rows by their weights
     const bool in = base + lane < parts;
-    const int64_t mine = row_of(min(base + lane, parts - 1));
+    const int64_t mine = row_of(in ? base + lane : 0);
     const float r = in ? a.part_ml[2 * mine] : kAttnNone, l = in ? a.part_ml[2 * mine + 1] : 0.f;
-    const float nt = fmaxf(top, wave_max(r)), keep = __builtin_amdgcn_exp2f(top - nt);
-    const float f = __builtin_amdgcn_exp2f(r - nt);
-    top = nt;
-    den = fmaf(den, keep, wave_sum(f * l));
-#pragma unroll
-    for (int e = 0; e < E; ++e) y[e] *= keep;
     const int n = min(64, parts - base);
-#pragma unroll 8
-    for (int p = WAVES == 4 ? wave : 0; p < n; p += WAVES) {
-      const float fp = __shfl(f, p, 64);
-      const float* row = a.part + row_of(base + p) * HD + lane * E;
+    float nt = 0.f, f = 0.f;
+    for (int p0 = 0; p0 < n; p0 += G * AHEAD) {  // the same for all lanes
+      float v[AHEAD][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) y[e] = fmaf(row[e], fp, y[e]);
+      for (int i = 0; i < AHEAD; ++i) {
+        const float* row = a.part + row_of(base + min(p0 + grp + G * i, n - 1)) * HD + d0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[i][e] = row[e];
+      }
+      if (p0 == 0) {
+        nt = fmaxf(top, wave_max(r));
+        const float keep = __builtin_amdgcn_exp2f(top - nt);
+        f = __builtin_amdgcn_exp2f(r - nt);
+        top = nt;
+        den = fmaf(den, keep, wave_sum(f * l));
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] *= keep;
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int p = p0 + grp + G * i;
+        const float w = __shfl(f, min(p, 63), 64), fp = p < n ? w : 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = fp != 0.f ? fmaf(v[i][e], fp, y[e]) : y[e];
+      }
     }
   }
   uint16_t* const dst = a.out + t * a.out_stride + (int64_t)h * HD;
-  if constexpr (WAVES == 4) {
-    __shared__ float so[4][HD];
-#pragma unroll
-    for (int e = 0; e < E; ++e) so[wave][lane * E + e] = y[e];
+  if constexpr (WIDE) {
+    __shared__ float so[G][32];
+    so[grp][tid & 31] = y[0];
     __syncthreads();
-    for (int d = threadIdx.x; d < HD; d += 256)
-      dst[d] = T::from_f32(den != 0.f ? (so[0][d] + so[1][d] + so[2][d] + so[3][d]) / den : 0.f);
+    if (tid < 32) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < G; ++i) v += so[i][tid];
+      dst[d0] = T::from_f32(den != 0.f ? v / den : 0.f);
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) dst[lane * E + e] = T::from_f32(den != 0.f ? y[e] / den : 0.f);
+    for (int e = 0; e < E; ++e) dst[d0 + e] = T::from_f32(den != 0.f ? y[e] / den : 0.f);
   }
 }
 
@@ -867,7 +902,7 @@ AttnPlan attn_plan(int64_t T, int64_t R, int64_t n_q, int64_t n_kv, int64_t hd, 
   // As many workgroups as the CUs hold at once, each with an equal share of all
   // keys.  Not for short keys, where joining the parts would take longer than
   // they, nor for more row tiles than workgroups of the kernel for many rows.
-  const bool long_keys = max_kv_len <= 0 || max_kv_len > 256;
+  const bool long_keys = max_kv_len <= 0 || max_kv_len > 1024;
   if (p.few && long_keys) p.wgs_few = (int)std::max<int64_t>(1, kAttnCus * attn_held((int)hd, p.qt_few) / n_kv);
   if (p.many && long_keys && p.tiles_many * n_kv < 2 * kAttnCus)
     p.wgs_many = (int)std::max<int64_t>(1, 2 * kAttnCus / n_kv);
@@ -901,8 +936,8 @@ void launch_attn(const AttnPlan& p, Kv4AttnArgs a, int64_t n_kv, int64_t n_q, hi
   }
   if (p.part_rows > 0) {
     const int64_t rows = a.T * n_q;
-    if (rows <= 1024) kv4_attn_join_kernel<T, HD, 4><<<(unsigned)rows, 256, 0, st>>>(a, (int)n_q);
-    else kv4_attn_join_kernel<T, HD, 1><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a, (int)n_q);
+    if (rows <= 512) kv4_attn_join_kernel<T, HD, true><<<dim3((unsigned)rows, HD / 32), 256, 0, st>>>(a, (int)n_q);
+    else kv4_attn_join_kernel<T, HD, false><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a, (int)n_q);
   }
 }
 
