@@ -372,8 +372,9 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
       const uint64_t at = (uint64_t)(uint32_t)(out ? 0 : x.b[h]) * (uint32_t)a.dm.block_stride;
       const auto src = kv4_rsrc(head + at, out ? 0 : head_bytes);
       const int tok = (t0 + 16 * h) & (bs - 1);
+      // (aux 2: not kept in the caches where each code is read once, by KVSPLIT)
 #define CEK_FETCH(lane_off, dst, bytes, off) \
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_ptr_t)(dst), bytes, lane_off, off, 0, 0)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_ptr_t)(dst), bytes, lane_off, off, 0, KVSPLIT ? 2 : 0)
       // a part of 128 values and 16 tokens: 64 bytes of each K row, 256 of each four tokens of V
       CEK_FETCH(k_lane, to + h * HALF, 16, tok * (HD / 2));
       if constexpr (HD == 256) CEK_FETCH(k_lane, to + h * HALF + 1024, 16, tok * (HD / 2) + 64);
