@@ -29,12 +29,14 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 struct F16 {
   static constexpr int code = CEK_F16;
   typedef h2 pair;
+  static constexpr uint16_t inf = 0x7C00;
   __device__ static inline float to_f32(uint16_t b) { return (float)__builtin_bit_cast(_Float16, b); }
   __device__ static inline uint16_t from_f32(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
 };
 struct BF16 {
   static constexpr int code = CEK_BF16;
   typedef bf2 pair;
+  static constexpr uint16_t inf = 0x7F80;
   __device__ static inline float to_f32(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
   // v_cvt_pk_bf16_f32 on gfx950: round to nearest even, NaN stays NaN.
   __device__ static inline uint16_t from_f32(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }

@@ -22,6 +22,21 @@ struct Kv4Dims {
   int num_blocks, n_kv, bs_log2;
 };
 
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Inclusive sum over the lanes, by DPP: rows of 16 by shifts, then the rows' last
+// lanes broadcast into the rows behind them.
+#define CEK_DPP_ADD(x, ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xF, true)
+__device__ inline int wave_scan_incl(int x) {
+  CEK_DPP_ADD(x, 0x111, 0xF);  // row_shr 1, 2, 4, 8
+  CEK_DPP_ADD(x, 0x112, 0xF);
+  CEK_DPP_ADD(x, 0x114, 0xF);
+  CEK_DPP_ADD(x, 0x118, 0xF);
+  CEK_DPP_ADD(x, 0x142, 0xA);  // row_bcast 15 into rows 1 and 3
+  CEK_DPP_ADD(x, 0x143, 0xC);  // row_bcast 31 into rows 2 and 3
+  return x;
+}
+
 // Byte offsets inside one (block, head); hd / 2 bytes a token and part.
 __host__ __device__ inline int kv4_v_codes(int bs, int hd) { return bs * (hd / 2); }
 __host__ __device__ inline int kv4_k_params(int bs, int hd) { return bs * hd; }
@@ -40,25 +55,24 @@ constexpr float kKv4MinStep = 0x1p-100f;
 __device__ inline uint32_t kv4_params(float lo, float hi, bool finite) {
   if (!finite) return 0x7FC00000u;
   const float m = BF16::to_f32(BF16::from_f32(f32_round(0.5f * lo) + f32_round(0.5f * hi)));
-  const float a = fmaxf(hi - m, m - lo);
-  uint32_t s = BF16::from_f32(a / 7.5f);
+  // a / 7.5 by the rounded reciprocal and one correction: the correctly rounded quotient
+  const float a = fmaxf(hi - m, m - lo), q0 = a * (1.0f / 7.5f);
+  uint32_t s = BF16::from_f32(fmaf(fmaf(-q0, 7.5f, a), 1.0f / 7.5f, q0));
   if (__uint_as_float(s << 16) < kKv4MinStep) s = 0;
   return s | (__float_as_uint(m) & 0xFFFF0000u);
 }
 
-// The code of x: the nearest step, ties to even codes, all operations in fp32
-// and rounded one by one: rint((x - m) / s + 7.5) within 0 .. 15.  d = quant_div
-// of the row's step; a row of step 0 has code 8.
-__device__ inline uint32_t kv4_code(float x, float m, QuantDiv d, bool has_step) {
-  const float v = f32_round(x - m);
-  const float q0 = f32_round(v * d.r);
-  const float q = fmaf(fmaf(-q0, d.s, v), d.r, q0);
-  const float c = fminf(fmaxf(rintf(f32_round(q) + 7.5f), 0.0f), 15.0f);
-  return has_step ? (uint32_t)c : 8u;
+// The nearest step to x, ties to even codes, all operations in fp32 and rounded
+// one by one: rint((x - m) / s + 7.5), d = quant_div of the row's step.  0 .. 15
+// without a clamp: |x - m| <= 7.5 s (1 + 2^-8), s being a / 7.5 to within 2^-9.  A row
+// of step 0 has code 8 throughout (the caller's part).
+__device__ inline float kv4_code(float x, float m, QuantDiv d) {
+  const float v = x - m, q0 = v * d.r;
+  return rintf(fmaf(fmaf(-q0, d.s, v), d.r, q0) + 7.5f);
 }
 
 __device__ inline float kv4_value(uint32_t code, uint32_t p) {
-  return f32_round(kv4_step(p) * ((float)code - 7.5f)) + kv4_centre(p);  // the product is exact
+  return fmaf(kv4_step(p), (float)code - 7.5f, kv4_centre(p));  // the product is exact
 }
 
 // The arguments that the cache's operators share.

@@ -67,21 +67,6 @@ struct Kv4Work {
   int first;             // the tile's first unit in the list
 };
 
-__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-
-// Inclusive sum over the lanes, by DPP: rows of 16 by shifts, then the rows' last
-// lanes broadcast into the rows behind them.
-#define CEK_DPP_ADD(x, ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xF, true)
-__device__ inline int wave_scan_incl(int x) {
-  CEK_DPP_ADD(x, 0x111, 0xF);  // row_shr 1, 2, 4, 8
-  CEK_DPP_ADD(x, 0x112, 0xF);
-  CEK_DPP_ADD(x, 0x114, 0xF);
-  CEK_DPP_ADD(x, 0x118, 0xF);
-  CEK_DPP_ADD(x, 0x142, 0xA);  // row_bcast 15 into rows 1 and 3
-  CEK_DPP_ADD(x, 0x143, 0xC);  // row_bcast 31 into rows 2 and 3
-  return x;
-}
-
 // The work list: every request has ceil(rows / BR) tiles of rows, and each tile its
 // keys (from the first that any row sees, down to a multiple of 32) in units of
 // `len` tokens, or in one.  Tiles lie one after another, a request's last one

@@ -8,17 +8,24 @@
 // the tail -- places that no block is taken from in the same call, so nothing
 // is read after it was overwritten.  Offsets are prefix sums over the requests.
 //
-// All integer work on a few kilobytes: latency is what it costs.  One
-// workgroup holds the requests (up to four a thread) and does the scans in
-// LDS, the tables and the ring; kv_lens_out and ring_state_out are written
-// after the barrier behind the last read of kv_lens and ring_state, so that
-// they may be the same memory.
-#include "cek_common.h"
+// All integer work on a few kilobytes: what it costs is latency, of the launch,
+// two rounds of loads and four barriers.  One workgroup, no larger than the
+// requests and tokens need, holds up to four requests a thread, scans their
+// counts by DPP, keeps the offsets in LDS and hands the moved blocks and the
+// tokens out evenly, each finding its request by bisection there; a new token's
+// block comes from the ring itself, so that nothing waits for the tables that are
+// being written.  Above kTablesOneLaunch tokens a second launch fills the slots.
+// kv_lens_out and ring_state_out are written behind the barrier that follows the
+// last read of kv_lens and ring_state, so that they may be the same memory.
+#include <algorithm>
+
+#include "cek_kv4.h"
 
 namespace cek {
 
 constexpr int kTablesThreads = 1024;
 constexpr int kTablesMaxRequests = 4096;
+constexpr int64_t kTablesOneLaunch = 4096;
 
 struct KvTablesArgs {
   const int32_t *kv_lens, *keep_lens, *q_lens, *ring_state;
@@ -28,152 +35,188 @@ struct KvTablesArgs {
   int R, cap, width, bs_log2;
 };
 
-// Inclusive scans of N values over the workgroup, in thread order.
-template <int N>
-__device__ inline void wg_scan(int64_t (&x)[N], int64_t (*sh)[N]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+__device__ inline int64_t wave_scan_incl(int64_t x) {
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int64_t y = __shfl_up((long long)x[i], off, 64);
-      if (lane >= off) x[i] += y;
-    }
+    const int64_t y = __shfl_up((long long)x, off, 64);
+    if (lane >= off) x += y;
   }
-  if (lane == 63)
-    for (int i = 0; i < N; ++i) sh[wave][i] = x[i];
+  return x;
+}
+
+// Inclusive scans of N values over the workgroup, in thread order; total: the sums.
+template <typename I, int N>
+__device__ inline void wg_scan(I (&x)[N], I (&total)[N], I (*sh)[N]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    x[i] = wave_scan_incl(x[i]);
+    if (lane == 63) sh[wave][i] = x[i];
+    total[i] = 0;
+  }
   __syncthreads();
   for (int w = 0; w < waves; ++w)
-    if (w < wave)
-      for (int i = 0; i < N; ++i) x[i] += sh[w][i];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (w < wave) x[i] += sh[w][i];
+      total[i] += sh[w][i];
+    }
   __syncthreads();
 }
 
-// The slot and position of token t: its request by bisection in cu[0 .. R].
-template <typename CU, typename KEEP>
-__device__ inline void token_slot(const KvTablesArgs& a, int64_t t, const CU& cu, const KEEP& keep_of) {
-  int64_t pos = 0, slot = -1;
-  if (t < cu(a.R)) {
-    int lo = 0, hi = a.R;  // cu(lo) <= t < cu(hi)
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (cu(mid) <= t) lo = mid;
-      else hi = mid;
+// The last i < n with at[i] <= x; at[0] <= x, at[n] > x.
+__device__ inline int find_in(const int32_t* at, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (at[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// I: the type of the counts' sums -- 32 bits where they cannot overflow.
+template <typename I>
+__global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(KvTablesArgs a, int fill_slots) {
+  constexpr int N = kTablesMaxRequests;
+  __shared__ I sh2[kTablesThreads / 64][2], sh3[kTablesThreads / 64][3];
+  // offsets of the requests' new tokens, taken and returned blocks; kept tokens, blocks held and wanted
+  __shared__ int32_t at_q[N + 1], at_need[N + 1], at_gone[N + 1], keep_s[N], have_s[N], want_s[N];
+  const int tid = threadIdx.x, nt = blockDim.x;
+  const int per = (a.R + nt - 1) / nt;  // requests per thread, consecutive
+  const int bs = 1 << a.bs_log2;
+  const int64_t reach = (int64_t)a.width << a.bs_log2;  // tokens that a table row holds
+  // the ring's state, kept in range whatever it holds
+  const int count = min(max(a.ring_state[1], 0), a.cap);
+  int head = a.ring_state[0];
+  if (head < 0 || head >= a.cap) head = (head % a.cap + a.cap) % a.cap;
+  auto place = [&](int64_t i) {  // of the ring, i < 3 cap from the head on
+    i += head;
+    i -= i >= a.cap ? a.cap : 0;
+    i -= i >= a.cap ? a.cap : 0;
+    return i - (i >= a.cap ? a.cap : 0);
+  };
+
+  int64_t q[4];
+  int len[4], keep[4], have[4], need[4], st[4];
+  I sum[2] = {0, 0}, total2[2];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int r = tid * per + j;
+    len[j] = keep[j] = have[j] = need[j] = st[j] = 0;
+    q[j] = 0;
+    if (j < per && r < a.R) {
+      len[j] = (int)min((int64_t)max(a.kv_lens[r], 0), reach);
+      keep[j] = min(max(a.keep_lens[r], 0), len[j]);
+      q[j] = max(a.q_lens[r], 0);
+      if (keep[j] + q[j] > reach) st[j] = 2, q[j] = 0;
+      have[j] = (len[j] + bs - 1) >> a.bs_log2;
+      need[j] = max((int)((keep[j] + q[j] + bs - 1) >> a.bs_log2) - have[j], 0);
+      // (counts beyond what there is are as good as one more than that)
+      sum[0] += (I)min(need[j], a.cap + 1);
+      sum[1] += (I)min(q[j], a.T + 1);
     }
-    pos = keep_of(lo) + (t - cu(lo));
-    const int32_t blk = a.tables[(int64_t)lo * a.table_stride + (pos >> a.bs_log2)];
+  }
+  const I own[2] = {sum[0], sum[1]};
+  wg_scan<I, 2>(sum, total2, sh2);
+  sum[0] -= own[0];
+  sum[1] -= own[1];
+  // requests whose blocks or rows the sums up to them leave no room for
+  int want[4], gone[4];
+  I at[3] = {0, 0, 0}, total[3];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    sum[0] += (I)min(need[j], a.cap + 1);
+    sum[1] += (I)min(q[j], a.T + 1);
+    if (st[j] == 0) st[j] = need[j] > 0 && sum[0] > (I)count ? 1 : (q[j] > 0 && sum[1] > (I)a.T ? 3 : 0);
+    if (st[j]) need[j] = 0, q[j] = 0;
+    want[j] = (int)((keep[j] + q[j] + bs - 1) >> a.bs_log2);
+    gone[j] = min(max(have[j] - want[j], 0), a.cap + 1);
+    at[0] += (I)need[j];
+    at[1] += (I)q[j];
+    at[2] += (I)gone[j];
+  }
+  const I mine[3] = {at[0], at[1], at[2]};
+  wg_scan<I, 3>(at, total, sh3);  // (the reads of kv_lens and ring_state are behind its barriers)
+#pragma unroll
+  for (int i = 0; i < 3; ++i) at[i] -= mine[i];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int r = tid * per + j;
+    if (j < per && r < a.R) {
+      at_need[r] = (int)at[0];
+      a.cu_q[r] = at_q[r] = (int)at[1];
+      at_gone[r] = (int)at[2];
+      keep_s[r] = keep[j];
+      have_s[r] = have[j];
+      want_s[r] = want[j];
+      a.kv_lens_out[r] = keep[j] + (int)q[j];
+      a.status[r] = st[j];
+    }
+    at[0] += (I)need[j];
+    at[1] += (I)q[j];
+    at[2] += (I)gone[j];
+  }
+  const int taken = (int)total[0], rows = (int)total[1];
+  // (lengths of more blocks than there are return no more than the ring has room for)
+  const int given = (int)min((int64_t)total[2], (int64_t)a.cap - count + taken);
+  if (tid == 0) {
+    at_need[a.R] = taken;
+    a.cu_q[a.R] = at_q[a.R] = rows;
+    at_gone[a.R] = (int)total[2];
+    a.ring_state_out[0] = (int)place(taken);
+    a.ring_state_out[1] = count - taken + given;
+  }
+  __syncthreads();
+  // The blocks that are taken, and those that are returned: a row's entries beyond
+  // the wanted ones are its own, and the ring's places behind the free blocks no one's.
+  for (int i = tid; i < taken; i += nt) {
+    const int r = find_in(at_need, a.R, i);
+    a.tables[(int64_t)r * a.table_stride + have_s[r] + i - at_need[r]] = a.ring[place(i)];
+  }
+  for (int i = tid; i < given; i += nt) {
+    const int r = find_in(at_gone, a.R, i);
+    a.ring[place((int64_t)count + i)] = a.tables[(int64_t)r * a.table_stride + want_s[r] + i - at_gone[r]];
+  }
+  if (!fill_slots) return;
+  for (int t = tid; t < (int)a.T; t += nt) {
+    int64_t pos = 0, slot = -1;
+    if (t < rows) {
+      const int r = find_in(at_q, a.R, t);
+      pos = keep_s[r] + t - at_q[r];
+      const int i = (int)(pos >> a.bs_log2);
+      const int32_t blk = i < have_s[r] ? a.tables[(int64_t)r * a.table_stride + i]
+                                        : a.ring[place((int64_t)at_need[r] + i - have_s[r])];
+      slot = blk < 0 ? -1 : ((int64_t)blk << a.bs_log2) + (pos & (bs - 1));
+    }
+    a.slots[t] = slot;
+    a.positions[t] = pos;
+  }
+}
+
+// Slots and positions of many tokens, behind kv_tables_kernel on the stream:
+// what stays of a request is what it has now less its new tokens.
+__global__ __launch_bounds__(256) void kv_slots_kernel(KvTablesArgs a) {
+  __shared__ int32_t at_q[kTablesMaxRequests + 1];
+  for (int i = threadIdx.x; i <= a.R; i += 256) at_q[i] = a.cu_q[i];
+  __syncthreads();
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= a.T) return;
+  int64_t pos = 0, slot = -1;
+  if (t < at_q[a.R]) {
+    const int r = find_in(at_q, a.R, (int)t);
+    pos = (int64_t)a.kv_lens_out[r] - at_q[r + 1] + t;
+    const int32_t blk = a.tables[(int64_t)r * a.table_stride + (pos >> a.bs_log2)];
     slot = blk < 0 ? -1 : ((int64_t)blk << a.bs_log2) + (pos & ((1 << a.bs_log2) - 1));
   }
   a.slots[t] = slot;
   a.positions[t] = pos;
 }
 
-__global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(KvTablesArgs a, int fill_slots) {
-  __shared__ int64_t sh[kTablesThreads / 64][3];
-  __shared__ int32_t cu_s[kTablesMaxRequests + 1], keep_s[kTablesMaxRequests];
-  const int tid = threadIdx.x, nt = blockDim.x;
-  const int per = (a.R + nt - 1) / nt;  // requests per thread, consecutive
-  const int bs = 1 << a.bs_log2;
-  const int64_t reach = (int64_t)a.width << a.bs_log2;  // tokens that a table row holds
-  // the ring's state, kept in range whatever it holds
-  int64_t head = a.ring_state[0], count = a.ring_state[1];
-  count = count < 0 ? 0 : (count > a.cap ? a.cap : count);
-  head %= a.cap;
-  if (head < 0) head += a.cap;
-
-  int64_t len[4], keep[4], q[4], need[4], sum[2] = {0, 0};
-  int st[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int r = tid * per + j;
-    len[j] = keep[j] = q[j] = need[j] = 0;
-    st[j] = 0;
-    if (j < per && r < a.R) {
-      len[j] = min((int64_t)max(a.kv_lens[r], 0), reach);
-      keep[j] = min((int64_t)max(a.keep_lens[r], 0), len[j]);
-      q[j] = max(a.q_lens[r], 0);
-      if (keep[j] + q[j] > reach) st[j] = 2;
-      if (st[j]) q[j] = 0;
-      need[j] = max(((keep[j] + q[j] + bs - 1) >> a.bs_log2) - ((len[j] + bs - 1) >> a.bs_log2), (int64_t)0);
-      sum[0] += need[j];
-      sum[1] += q[j];
-    }
-  }
-  const int64_t own0 = sum[0], own1 = sum[1];
-  wg_scan<2>(sum, reinterpret_cast<int64_t(*)[2]>(sh));
-  sum[0] -= own0;
-  sum[1] -= own1;
-  // requests whose blocks or rows the sums up to them leave no room for
-  int64_t gone[4], tot[3] = {0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    sum[0] += need[j];
-    sum[1] += q[j];
-    if (need[j] > 0 && sum[0] > count) st[j] = 1;
-    else if (q[j] > 0 && sum[1] > a.T) st[j] = 3;
-    if (st[j]) need[j] = q[j] = 0;
-    gone[j] = max(((len[j] + bs - 1) >> a.bs_log2) - ((keep[j] + q[j] + bs - 1) >> a.bs_log2), (int64_t)0);
-    tot[0] += need[j];
-    tot[1] += q[j];
-    tot[2] += gone[j];
-  }
-  int64_t at[3] = {tot[0], tot[1], tot[2]};
-  wg_scan<3>(at, sh);
-  const int64_t end0 = at[0], end1 = at[1], end2 = at[2];
-#pragma unroll
-  for (int i = 0; i < 3; ++i) at[i] -= tot[i];
-  // every read of kv_lens, keep_lens and ring_state is behind the scans' barriers
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int r = tid * per + j;
-    if (j < per && r < a.R) {
-      const int64_t have = (len[j] + bs - 1) >> a.bs_log2, want = (keep[j] + q[j] + bs - 1) >> a.bs_log2;
-      int32_t* row = a.tables + (int64_t)r * a.table_stride;
-      for (int64_t i = 0; i < need[j]; ++i) {
-        int64_t p = head + at[0] + i;
-        if (p >= a.cap) p -= a.cap;
-        row[have + i] = a.ring[p];
-      }
-      for (int64_t i = 0; i < gone[j]; ++i) {
-        int64_t p = head + count + at[2] + i;
-        p -= p >= a.cap ? a.cap : 0;
-        p -= p >= a.cap ? a.cap : 0;
-        a.ring[p] = row[want + i];
-      }
-      a.cu_q[r] = cu_s[r] = (int32_t)at[1];
-      keep_s[r] = (int32_t)keep[j];
-      a.kv_lens_out[r] = (int32_t)(keep[j] + q[j]);
-      a.status[r] = st[j];
-    }
-#pragma unroll
-    for (int i = 0; i < 3; ++i) at[i] += i == 0 ? need[j] : (i == 1 ? q[j] : gone[j]);
-  }
-  if (tid == nt - 1) {
-    a.cu_q[a.R] = cu_s[a.R] = (int32_t)end1;
-    a.ring_state_out[0] = (int32_t)((head + end0) % a.cap);
-    a.ring_state_out[1] = (int32_t)(count - end0 + end2);
-  }
-  if (!fill_slots) return;
-  __syncthreads();  // tables and cu_s of the whole workgroup
-  for (int64_t t = tid; t < a.T; t += nt)
-    token_slot(a, t, [&](int r) { return (int64_t)cu_s[r]; }, [&](int r) { return (int64_t)keep_s[r]; });
-}
-
-// Slots and positions of many tokens, behind kv_tables_kernel on the stream:
-// what stays of a request is what it has now less its new tokens.
-__global__ __launch_bounds__(256) void kv_slots_kernel(KvTablesArgs a) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= a.T) return;
-  token_slot(a, t, [&](int r) { return (int64_t)a.cu_q[r]; },
-             [&](int r) { return (int64_t)a.kv_lens_out[r] - (a.cu_q[r + 1] - a.cu_q[r]); });
-}
-
 }  // namespace cek
 
 using namespace cek;
-
-// Tokens up to which the one workgroup fills the slots itself.
-constexpr int64_t kTablesOneLaunch = 4096;
 
 extern "C" int cek_kv_block_tables(const int32_t* kv_lens, const int32_t* keep_lens, const int32_t* q_lens, int64_t R,
                                    int64_t block_size, int32_t* free_ring, int64_t num_blocks, const int32_t* ring_state,
@@ -193,7 +236,11 @@ extern "C" int cek_kv_block_tables(const int32_t* kv_lens, const int32_t* keep_l
                        __builtin_ctzll((unsigned long long)block_size)};
   hipStream_t st = (hipStream_t)stream;
   const int one = T <= kTablesOneLaunch;
-  kv_tables_kernel<<<1, kTablesThreads, 0, st>>>(a, one);
+  // a thread for each request and, where they are few, for each token
+  const int64_t want = std::max<int64_t>(R, one ? T : 256);
+  const int threads = (int)std::min<int64_t>(kTablesThreads, std::max<int64_t>(1, (want + 63) / 64) * 64);
+  if (R * (std::max<int64_t>(T, num_blocks) + 1) < INT32_MAX) kv_tables_kernel<int><<<1, threads, 0, st>>>(a, one);
+  else kv_tables_kernel<int64_t><<<1, threads, 0, st>>>(a, one);
   int rc = check_launch();
   if (rc != CEK_OK || one) return rc;
   kv_slots_kernel<<<(unsigned)((T + 255) / 256), 256, 0, st>>>(a);

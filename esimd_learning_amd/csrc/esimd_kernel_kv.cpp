@@ -7,8 +7,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <iterator>
 #include <string>
-#include <vector>
 
 #include "shim_common.h"
 
@@ -125,21 +125,23 @@ void esimd_kv_block_tables(at::Tensor kv_lens, at::Tensor keep_lens, at::Tensor 
   TORCH_CHECK(block_tables.size(1) * block_size <= INT32_MAX, op, ": a row of block_tables reaches beyond 2^31 tokens");
   // every output apart from the inputs and the other outputs, but for lengths
   // and ring state that are updated in place
-  const std::vector<at::Tensor> ins = {kv_lens, keep_lens, q_lens, ring_state};
-  const std::vector<at::Tensor> outs = {free_ring, kv_lens_out, ring_state_out, cu_q, slot_mapping, positions, status};
-  for (size_t i = 0; i < outs.size(); ++i) {
+  struct Range { uintptr_t at, end; };
+  const auto range = [](const at::Tensor& t) {
+    const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    return Range{at, at + t.nbytes()};
+  };
+  const auto meet = [](const Range& x, const Range& y) { return x.at < x.end && y.at < y.end && x.at < y.end && y.at < x.end; };
+  Range table = range(block_tables);
+  if (R > 0) table.end = table.at + ((R - 1) * stride + block_tables.size(1)) * 4;
+  const Range ins[] = {range(kv_lens), range(keep_lens), range(q_lens), range(ring_state)};
+  const Range outs[] = {range(kv_lens_out), range(ring_state_out), range(free_ring), range(cu_q), range(slot_mapping),
+                        range(positions), range(status), table};
+  for (size_t i = 0; i < std::size(outs); ++i) {
     for (const auto& x : ins)
-      TORCH_CHECK(!overlaps(outs[i], x) || (x.data_ptr() == outs[i].data_ptr() &&
-                                            ((i == 1 && x.data_ptr() == kv_lens.data_ptr()) ||
-                                             (i == 2 && x.data_ptr() == ring_state.data_ptr()))),
+      TORCH_CHECK(!meet(outs[i], x) || (x.at == outs[i].at && ((i == 0 && x.at == ins[0].at) || (i == 1 && x.at == ins[3].at))),
                   op, ": an output overlaps an input (kv_lens_out may be kv_lens, ring_state_out ring_state)");
-    for (size_t j = 0; j < i; ++j) TORCH_CHECK(!overlaps(outs[i], outs[j]), op, ": outputs overlap");
-    TORCH_CHECK(R == 0 || !extent_overlaps(block_tables, stride, block_tables.size(1), outs[i]), op,
-                ": block_tables overlaps another output");
+    for (size_t j = 0; j < i; ++j) TORCH_CHECK(!meet(outs[i], outs[j]), op, ": outputs overlap");
   }
-  for (const auto& x : ins)
-    TORCH_CHECK(R == 0 || !extent_overlaps(block_tables, stride, block_tables.size(1), x), op,
-                ": block_tables overlaps an input");
   c10::OptionalDeviceGuard guard(kv_lens.device());
   const auto p = [](const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
   check_rc(cek_kv_block_tables(p(kv_lens), p(keep_lens), p(q_lens), R, block_size, p(free_ring), free_ring.numel(),

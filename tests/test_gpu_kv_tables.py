@@ -70,6 +70,28 @@ def test_decode_across_block_ends(ops, dev):
     assert s.h_state[1] == 12 - 3 - 1
 
 
+def test_impossible_state_stays_in_bounds(ops, dev):
+    """Lengths of more blocks than there are, ring states out of range: nothing outside the arrays is touched."""
+    R, width, blocks = 6, 50, 16
+    guard = torch.full((3, 64 + blocks), 123, dtype=torch.int32, device=dev)
+    ring = guard[1, 32:32 + blocks]
+    ring.copy_(torch.arange(blocks))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    for state in ((0, 0), (5, 16), (-7, 99), (10 ** 9, -4)):
+        for lens, keep, q in (((800,) * 6, (0,) * 6, (0,) * 6), ((2 ** 31 - 1,) * 6, (5,) * 6, (2 ** 31 - 1, 1, 0, 40, 9, 3)),
+                              ((-5,) * 6, (3,) * 6, (16, 0, 17, -1, 100, 2 ** 31 - 1))):
+            tables = torch.zeros(R, width, dtype=torch.int32, device=dev)
+            cu, out, so = i32(*[0] * 7), i32(*[0] * 6), i32(0, 0)
+            slots, pos = (torch.zeros(20, dtype=torch.int64, device=dev) for _ in range(2))
+            ops.esimd_kv_block_tables(i32(*lens), i32(*keep), i32(*q), 16, ring, i32(*state), tables, out, so, cu, slots,
+                                      pos, i32(*[0] * 6))
+            head, count = so.tolist()
+            assert 0 <= head < blocks and 0 <= count <= blocks
+            assert (guard[0] == 123).all() and (guard[2] == 123).all()
+            assert (guard[1, :32] == 123).all() and (guard[1, 32 + blocks:] == 123).all()
+            assert 0 <= int(cu.max()) <= 20 and int(out.min()) >= 0
+
+
 def test_no_new_tokens_and_no_requests(ops, dev):
     s = State(2, 3, 16, 6, 0, dev)
     s.step(ops, [0, 0], [0, 0])
