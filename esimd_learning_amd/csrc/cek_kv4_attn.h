@@ -1,0 +1,146 @@
+// cek_kv4_attn.h -- what the attention kernels over the 4-bit cache share: their
+// arguments, the work list and the arithmetic's constants (cek_kv4_attn.hip says
+// what they mean).
+#pragma once
+
+#include "cek_kv4.h"
+
+namespace cek {
+
+struct Kv4AttnArgs {
+  const uint16_t* q;
+  uint16_t* out;
+  const uint8_t* cache;
+  const int32_t *tables, *kv_lens, *cu_q;
+  float* part;     // split keys: rows of hd sums
+  float* part_ml;  // and their (reference exponent, sum of weights)
+  int4* meta;      // per row of a kv head: first part's row, parts, rows a slot, rows a tile
+  int64_t T, q_stride, out_stride, table_stride;
+  Kv4Dims dm;
+  int R, group, max_blocks, window;
+  int rows_above, rows_upto;  // this launch serves requests with that many rows
+  int wgs;                    // workgroups per kv head that share the keys evenly; 0: keys stay whole
+  int part_row0;              // first partial row of this launch
+  int vec_q, vec_out;
+  float scale;
+};
+
+constexpr int kAttnWaves = 4;
+constexpr int kAttnHead = 6, kAttnBase = 9;  // exponents: lag of a maximum, where the largest weight lies
+constexpr float kAttnNone = -1e30f;
+
+typedef const __attribute__((address_space(4))) int32_t* const_i32;  // scalar loads
+
+// A stretch of work: units [unit, unit + units) of the keys of one tile of rows.
+struct Kv4Work {
+  int r, q0, rows, kv, n_new, lo, tile;
+  int unit, units, all;  // all: the tile's units
+  int first;             // the tile's first unit in the list
+};
+
+// The work list: every request has ceil(rows / BR) tiles of rows, and each tile its
+// keys (from the first that any row sees, down to a multiple of 32) in units of
+// `len` tokens, or in one.  Tiles lie one after another, a request's last one
+// first (its rows see most keys).  Every wave of the grid computes its place
+// from the lengths alone.
+template <int BR>
+struct Kv4List {
+  const Kv4AttnArgs& a;
+  int len = 0;    // tokens of a unit; 0: all of a tile's
+  int total = 0;  // units, where the keys are shared
+
+  struct Req { int q0, rows, kv, n_new, lo, tiles; };
+  __device__ inline Req request(int r) const {
+    Req x;
+    const int at = min(r, a.R - 1);
+    const int c0 = a.cu_q[at], c1 = a.cu_q[at + 1], kv = a.kv_lens[at];
+    x.q0 = max(0, c0);
+    x.n_new = (int)min((int64_t)c1, a.T) - x.q0;
+    const int64_t n = (int64_t)x.n_new * a.group;
+    const bool mine = (r < a.R) & (x.n_new > 0) & (n > a.rows_above) & (n <= a.rows_upto);
+    x.rows = mine ? (int)n : 0;
+    x.kv = (int)min((int64_t)max(kv, 0), (int64_t)a.max_blocks << a.dm.bs_log2);
+    x.lo = a.window > 0 ? max(0, x.kv - x.n_new - a.window + 1) & ~31 : 0;
+    x.tiles = (x.rows + BR - 1) / BR;
+    return x;
+  }
+  __device__ inline int units(const Req& x) const {
+    return len ? (int)(((unsigned)max(x.kv - x.lo, 1) + (unsigned)len - 1u) / (unsigned)len) : 1;
+  }
+  // Units of `step` tokens, or as many times that as keep their number in 30 bits.
+  __device__ inline void share(const Req& first, int step) {
+    const int lane = threadIdx.x & 63;
+    for (len = step;; len *= 2) {
+      float sum = (float)first.tiles * (float)units(first);
+      int n = first.tiles * units(first);
+      for (int base = 64; base < a.R; base += 64) {
+        const Req x = request(base + lane);
+        sum += (float)x.tiles * (float)units(x);
+        n += x.tiles * units(x);
+      }
+      total = __builtin_amdgcn_readlane(wave_scan_incl(n), 63);
+      if (wave_sum_dpp(sum) < 0x1p30f) return;
+    }
+  }
+  // Workgroup j of n gets each = total / n units, the first `more` one more.
+  int each = 0, more = 0;
+  __device__ inline void deal(int n) {
+    each = uniform((int)((unsigned)total / (unsigned)n));
+    more = total - each * n;
+  }
+  __device__ inline int begin_of(int j) const { return each * j + min(j, more); }
+  __device__ inline int owner_of(int u) const {
+    const int far = more * (each + 1);
+    return uniform(u < far ? (int)((unsigned)u / (unsigned)(each + 1)) : more + (int)((unsigned)(u - far) / (unsigned)max(each, 1)));
+  }
+  // The stretch that starts at unit u, up to unit `to`; false behind the last one.
+  __device__ inline bool find(const Req& first, int u, int to, Kv4Work& w) const {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int base = 0; base < a.R; base += 64) {
+      const Req x = base == 0 ? first : request(base + lane);
+      const int n = units(x);
+      const int incl = before + wave_scan_incl(x.tiles * n);
+      const uint64_t above = __ballot(incl > u);
+      if (above) {
+        const int at = __builtin_ctzll(above);
+        auto get = [&](int y) { return __builtin_amdgcn_readlane(y, at); };
+        w.r = base + at;
+        w.q0 = get(x.q0);
+        w.rows = get(x.rows);
+        w.kv = get(x.kv);
+        w.n_new = get(x.n_new);
+        w.lo = get(x.lo);
+        w.all = get(n);
+        const int tiles = get(x.tiles), start = get(incl) - tiles * w.all;
+        const int nth = uniform((u - start) / w.all);
+        w.tile = tiles - 1 - nth;
+        w.first = start + nth * w.all;
+        w.unit = u - w.first;
+        w.units = min(w.all - w.unit, to - u);
+        return true;
+      }
+      before = __builtin_amdgcn_readlane(incl, 63);
+    }
+    return false;
+  }
+};
+
+// v of lanes l, l ^ 16, l ^ 32, l ^ 48, joined by op.
+template <typename OP>
+__device__ inline float over_rows(float v, OP op) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ inline uint32_t pack_h2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});
+}
+
+// The kernel for many rows (cek_kv4_attn_rows.hip): tiles of attn_rows_br(hd) rows.
+constexpr int attn_rows_br(int hd) { return hd == 256 ? 64 : 128; }
+void launch_attn_rows(const Kv4AttnArgs& a, int hd, int io_dtype, dim3 grid, hipStream_t st);
+
+}  // namespace cek

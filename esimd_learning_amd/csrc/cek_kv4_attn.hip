@@ -32,144 +32,12 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "cek_kv4.h"
+#include "cek_kv4_attn.h"
 
 namespace cek {
 
-struct Kv4AttnArgs {
-  const uint16_t* q;
-  uint16_t* out;
-  const uint8_t* cache;
-  const int32_t *tables, *kv_lens, *cu_q;
-  float* part;     // split keys: rows of hd sums
-  float* part_ml;  // and their (reference exponent, sum of weights)
-  int4* meta;      // per row of a kv head: first part's row, parts, rows a slot, rows a tile
-  int64_t T, q_stride, out_stride, table_stride;
-  Kv4Dims dm;
-  int R, group, max_blocks, window;
-  int rows_above, rows_upto;  // this launch serves requests with that many rows
-  int wgs;                    // workgroups per kv head that share the keys evenly; 0: keys stay whole
-  int part_row0;              // first partial row of this launch
-  int vec_q, vec_out;
-  float scale;
-};
-
-constexpr int kAttnWaves = 4;
-constexpr int kAttnHead = 6, kAttnBase = 9;  // exponents: lag of a maximum, where the largest weight lies
-constexpr float kAttnNone = -1e30f;
-
-typedef const __attribute__((address_space(4))) int32_t* const_i32;  // scalar loads
-
-// A stretch of work: units [unit, unit + units) of the keys of one tile of rows.
-struct Kv4Work {
-  int r, q0, rows, kv, n_new, lo, tile;
-  int unit, units, all;  // all: the tile's units
-  int first;             // the tile's first unit in the list
-};
-
-// The work list: every request has ceil(rows / BR) tiles of rows, and each tile its
-// keys (from the first that any row sees, down to a multiple of 32) in units of
-// `len` tokens, or in one.  Tiles lie one after another, a request's last one
-// first (its rows see most keys).  Every wave of the grid computes its place
-// from the lengths alone.
-template <int BR>
-struct Kv4List {
-  const Kv4AttnArgs& a;
-  int len = 0;    // tokens of a unit; 0: all of a tile's
-  int total = 0;  // units, where the keys are shared
-
-  struct Req { int q0, rows, kv, n_new, lo, tiles; };
-  __device__ inline Req request(int r) const {
-    Req x;
-    const int at = min(r, a.R - 1);
-    const int c0 = a.cu_q[at], c1 = a.cu_q[at + 1], kv = a.kv_lens[at];
-    x.q0 = max(0, c0);
-    x.n_new = (int)min((int64_t)c1, a.T) - x.q0;
-    const int64_t n = (int64_t)x.n_new * a.group;
-    const bool mine = (r < a.R) & (x.n_new > 0) & (n > a.rows_above) & (n <= a.rows_upto);
-    x.rows = mine ? (int)n : 0;
-    x.kv = (int)min((int64_t)max(kv, 0), (int64_t)a.max_blocks << a.dm.bs_log2);
-    x.lo = a.window > 0 ? max(0, x.kv - x.n_new - a.window + 1) & ~31 : 0;
-    x.tiles = (x.rows + BR - 1) / BR;
-    return x;
-  }
-  __device__ inline int units(const Req& x) const {
-    return len ? (int)(((unsigned)max(x.kv - x.lo, 1) + (unsigned)len - 1u) / (unsigned)len) : 1;
-  }
-  // Units of `step` tokens, or as many times that as keep their number in 30 bits.
-  __device__ inline void share(const Req& first, int step) {
-    const int lane = threadIdx.x & 63;
-    for (len = step;; len *= 2) {
-      float sum = (float)first.tiles * (float)units(first);
-      int n = first.tiles * units(first);
-      for (int base = 64; base < a.R; base += 64) {
-        const Req x = request(base + lane);
-        sum += (float)x.tiles * (float)units(x);
-        n += x.tiles * units(x);
-      }
-      total = __builtin_amdgcn_readlane(wave_scan_incl(n), 63);
-      if (wave_sum_dpp(sum) < 0x1p30f) return;
-    }
-  }
-  // Workgroup j of n gets each = total / n units, the first `more` one more.
-  int each = 0, more = 0;
-  __device__ inline void deal(int n) {
-    each = uniform((int)((unsigned)total / (unsigned)n));
-    more = total - each * n;
-  }
-  __device__ inline int begin_of(int j) const { return each * j + min(j, more); }
-  __device__ inline int owner_of(int u) const {
-    const int far = more * (each + 1);
-    return uniform(u < far ? (int)((unsigned)u / (unsigned)(each + 1)) : more + (int)((unsigned)(u - far) / (unsigned)max(each, 1)));
-  }
-  // The stretch that starts at unit u, up to unit `to`; false behind the last one.
-  __device__ inline bool find(const Req& first, int u, int to, Kv4Work& w) const {
-    const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int base = 0; base < a.R; base += 64) {
-      const Req x = base == 0 ? first : request(base + lane);
-      const int n = units(x);
-      const int incl = before + wave_scan_incl(x.tiles * n);
-      const uint64_t above = __ballot(incl > u);
-      if (above) {
-        const int at = __builtin_ctzll(above);
-        auto get = [&](int y) { return __builtin_amdgcn_readlane(y, at); };
-        w.r = base + at;
-        w.q0 = get(x.q0);
-        w.rows = get(x.rows);
-        w.kv = get(x.kv);
-        w.n_new = get(x.n_new);
-        w.lo = get(x.lo);
-        w.all = get(n);
-        const int tiles = get(x.tiles), start = get(incl) - tiles * w.all;
-        const int nth = uniform((u - start) / w.all);
-        w.tile = tiles - 1 - nth;
-        w.first = start + nth * w.all;
-        w.unit = u - w.first;
-        w.units = min(w.all - w.unit, to - u);
-        return true;
-      }
-      before = __builtin_amdgcn_readlane(incl, 63);
-    }
-    return false;
-  }
-};
-
 // Parameters of tokens that do not exist: K's and, 4 bs bytes on, V's.
 __device__ const uint8_t kv4_zeros[4 * 256 + 64] __attribute__((aligned(16))) = {};
-
-// v of lanes l, l ^ 16, l ^ 32, l ^ 48, joined by op.
-template <typename OP>
-__device__ inline float over_rows(float v, OP op) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
-__device__ inline uint32_t pack_h2(float a, float b) {
-  return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});
-}
 
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
@@ -229,12 +97,12 @@ __device__ inline void read_params(uint32_t at, u4 (&k)[1], u4 (&v)[1]) {
 // Workgroups that a CU holds at once (waves a SIMD): by registers and LDS.
 constexpr int attn_held(int hd, int qt) { return hd == 256 ? 2 : (hd == 64 ? 5 - qt : 4 - qt); }
 
-// KVSPLIT: the workgroup's four waves share QT x 16 rows and take every fourth 32
-// tokens each; else each wave has QT x 16 rows of its own and all the tokens.
+// Few rows a request: the workgroup's four waves share QT x 16 rows and take every
+// fourth 32 tokens each.
 // FOLD: tiles of 8 rows, in the MFMA's columns twice, so that columns 0 .. 7 have
 // the scores of the first 16 tokens at hand and columns 8 .. 15 those of the second
 // 16: half the arithmetic between the two products.
-template <typename T, int HD, int QT, bool KVSPLIT, bool FOLD>
+template <typename T, int HD, int QT, bool FOLD>
 __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4AttnArgs a) {
   constexpr int ND = HD / 32;                    // 32-bit words per lane, part and 16 tokens
   constexpr int NP = HD >= 128 ? HD / 128 : 1;   // parts of a row: 128 values, or 64
@@ -242,14 +110,14 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   constexpr int PW = HD / NP;                    // values of a part
   constexpr int RT = FOLD ? 8 : 16;              // rows of a tile
   constexpr int NX = FOLD ? 1 : 2;               // groups of four tokens a lane has scores of
-  constexpr int BR = QT * RT * (KVSPLIT ? 1 : kAttnWaves);
+  constexpr int BR = QT * RT;
   constexpr int LSTR = HD + 4;                   // LDS row stride: rows 4 banks apart
   constexpr int CODES = HD >= 128 ? 4 * NP * 1024 : 2048;  // bytes of 32 tokens' codes
   constexpr int SLOT = CODES + 256;                        // and parameters
   constexpr int HALF = CODES / 2;                          // 16 tokens: K codes, V codes
   constexpr int DEPTH = 2;                 // slots a wave
   constexpr int LOADS = CODES / 1024 + 1;                  // load instructions of a slot
-  constexpr int OUT_BYTES = KVSPLIT ? kAttnWaves * 16 * (LSTR + 2) * 4 : 0;
+  constexpr int OUT_BYTES = kAttnWaves * 16 * (LSTR + 2) * 4;
   constexpr int RING_BYTES = kAttnWaves * DEPTH * SLOT;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[RING_BYTES > OUT_BYTES ? RING_BYTES : OUT_BYTES];
   float* const lds_o = reinterpret_cast<float*>(lds);
@@ -263,13 +131,13 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   const auto mine = list.request(lane);
   int u = blockIdx.x, u_end = u + 1;
   if (a.wgs > 0) {
-    list.share(mine, KVSPLIT ? 32 * kAttnWaves : 512);
+    list.share(mine, 32 * kAttnWaves);
     list.deal(a.wgs);
     u = list.begin_of(blockIdx.x);
     u_end = list.begin_of(blockIdx.x + 1);
   }
   for (Kv4Work w; u < u_end && list.find(mine, u, u_end, w); u += w.units) {
-  const int row0 = w.tile * BR + (KVSPLIT ? 0 : wave * QT * RT);  // this wave's first row in the request
+  const int row0 = w.tile * BR;  // the first row in the request
   // Partial rows: of a tile's first stretch in 2 wg + 1, of the others in 2 wg.
   const bool whole = w.units == w.all;
   const int64_t part0 =
@@ -301,10 +169,10 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   }
   const int window = a.window > 0 ? a.window : INT32_MAX;  // pos - window stays in range
   const int t_lo = a.window > 0 ? max(0, pmin - a.window + 1) & ~31 : 0;
-  const int begin = uniform((list.len ? max(t_lo, w.lo + w.unit * list.len) : t_lo) + (KVSPLIT ? 32 * wave : 0));
+  const int begin = uniform((list.len ? max(t_lo, w.lo + w.unit * list.len) : t_lo) + 32 * wave);
   const int end = uniform(
       list.len ? (int)min((int64_t)pmax + 1, (int64_t)w.lo + (int64_t)(w.unit + w.units) * list.len) : pmax + 1);
-  constexpr int STEP = KVSPLIT ? 32 * kAttnWaves : 32;
+  constexpr int STEP = 32 * kAttnWaves;
 
 
 
@@ -357,9 +225,9 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
       const uint64_t at = (uint64_t)(uint32_t)(out ? 0 : x.b[h]) * (uint32_t)a.dm.block_stride;
       const auto src = kv4_rsrc(head + at, out ? 0 : head_bytes);
       const int tok = (t0 + 16 * h) & (bs - 1);
-      // (aux 2: not kept in the caches where each code is read once, by KVSPLIT)
+      // (aux 2: not kept in the caches, since each code is read once)
 #define CEK_FETCH(lane_off, dst, bytes, off) \
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_ptr_t)(dst), bytes, lane_off, off, 0, KVSPLIT ? 2 : 0)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_ptr_t)(dst), bytes, lane_off, off, 0, 2)
       // a part of 128 values and 16 tokens: 64 bytes of each K row, 256 of each four tokens of V
       CEK_FETCH(k_lane, to + h * HALF, 16, tok * (HD / 2));
       if constexpr (HD == 256) CEK_FETCH(k_lane, to + h * HALF + 1024, 16, tok * (HD / 2) + 64);
@@ -653,7 +521,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     cut_to(end);
     wait_vmcnt<0>();  // loads in flight land in LDS that is about to be used, or given back
   }
-  if (KVSPLIT) __syncthreads();
+  __syncthreads();
 
   // ---- the end: sums over the lanes of a row, parts to the workspace, rows out ----
 #pragma unroll
@@ -665,111 +533,68 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     auto value = [&](int p, int e, int h, int b) {
       return fmaf(o[i][p][h][b][e], b & 1 ? 0x1p20f : 0x1p24f, off);
     };
-    if constexpr (KVSPLIT) {
-      if (i > 0) __syncthreads();
+    if (i > 0) __syncthreads();
 #pragma unroll
-      for (int p = 0; p < NP; ++p)
+    for (int p = 0; p < NP; ++p)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int h = 0; h < NH; ++h)
-            *reinterpret_cast<f4*>(&lds_o[(wave * 16 + c) * LSTR + p * PW + g * (PW / 4) + 4 * NH * e + 4 * h]) =
-                f4{value(p, e, h, 0), value(p, e, h, 1), value(p, e, h, 2), value(p, e, h, 3)};
-      if (g == 0) {
-        lds_ml[(wave * 16 + c) * 2] = ref[i];
-        lds_ml[(wave * 16 + c) * 2 + 1] = l[i];
+        for (int h = 0; h < NH; ++h)
+          *reinterpret_cast<f4*>(&lds_o[(wave * 16 + c) * LSTR + p * PW + g * (PW / 4) + 4 * NH * e + 4 * h]) =
+              f4{value(p, e, h, 0), value(p, e, h, 1), value(p, e, h, 2), value(p, e, h, 3)};
+    if (g == 0) {
+      lds_ml[(wave * 16 + c) * 2] = ref[i];
+      lds_ml[(wave * 16 + c) * 2 + 1] = l[i];
+    }
+    __syncthreads();
+    // thread (row, sixteenth of the row)
+    const int row = threadIdx.x >> 4, seg = threadIdx.x & 15;
+    const int rr = w.tile * BR + i * RT + row;
+    float top = kAttnNone, den = 0.f, y[HD / 16] = {};
+#pragma unroll
+    for (int v = 0; v < kAttnWaves; ++v) top = fmaxf(top, lds_ml[(v * 16 + row) * 2]);
+#pragma unroll
+    for (int v = 0; v < kAttnWaves; ++v) {
+      const float lv = lds_ml[(v * 16 + row) * 2 + 1];
+      const float f = __builtin_amdgcn_exp2f(lds_ml[(v * 16 + row) * 2] - top);
+      den = fmaf(lv, f, den);
+#pragma unroll
+      for (int e = 0; e < HD / 16; e += 4) {
+        const f4 s = *reinterpret_cast<const f4*>(&lds_o[(v * 16 + row) * LSTR + seg * (HD / 16) + e]);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) y[e + b] = fmaf(s[b], f, y[e + b]);
       }
-      __syncthreads();
-      // thread (row, sixteenth of the row)
-      const int row = threadIdx.x >> 4, seg = threadIdx.x & 15;
-      const int rr = w.tile * BR + i * RT + row;
-      float top = kAttnNone, den = 0.f, y[HD / 16] = {};
+    }
+    if (row < RT && rr < w.rows) {
+      if (!whole) {
+        const int64_t pr = part0 + i * RT + row;
 #pragma unroll
-      for (int v = 0; v < kAttnWaves; ++v) top = fmaxf(top, lds_ml[(v * 16 + row) * 2]);
-#pragma unroll
-      for (int v = 0; v < kAttnWaves; ++v) {
-        const float lv = lds_ml[(v * 16 + row) * 2 + 1];
-        const float f = __builtin_amdgcn_exp2f(lds_ml[(v * 16 + row) * 2] - top);
-        den = fmaf(lv, f, den);
-#pragma unroll
-        for (int e = 0; e < HD / 16; e += 4) {
-          const f4 s = *reinterpret_cast<const f4*>(&lds_o[(v * 16 + row) * LSTR + seg * (HD / 16) + e]);
-#pragma unroll
-          for (int b = 0; b < 4; ++b) y[e + b] = fmaf(s[b], f, y[e + b]);
+        for (int e = 0; e < HD / 16; e += 4)
+          *reinterpret_cast<f4*>(a.part + pr * HD + seg * (HD / 16) + e) = f4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+        if (seg == 0) {
+          a.part_ml[2 * pr] = top;
+          a.part_ml[2 * pr + 1] = den;
         }
-      }
-      if (row < RT && rr < w.rows) {
-        if (!whole) {
-          const int64_t pr = part0 + i * RT + row;
+      } else {
+        const float inv = den != 0.f ? 1.0f / den : 0.f;
+        uint16_t* dst = a.out + (int64_t)(w.q0 + rr / a.group) * a.out_stride +
+                        (int64_t)(kvh * a.group + rr % a.group) * HD + seg * (HD / 16);
+        uint32_t u[HD / 32];
 #pragma unroll
-          for (int e = 0; e < HD / 16; e += 4)
-            *reinterpret_cast<f4*>(a.part + pr * HD + seg * (HD / 16) + e) = f4{y[e], y[e + 1], y[e + 2], y[e + 3]};
-          if (seg == 0) {
-            a.part_ml[2 * pr] = top;
-            a.part_ml[2 * pr + 1] = den;
-          }
+        for (int e = 0; e < HD / 32; ++e)
+          u[e] = (uint32_t)T::from_f32(den != 0.f ? y[2 * e] * inv : 0.f) |
+                 ((uint32_t)T::from_f32(den != 0.f ? y[2 * e + 1] * inv : 0.f) << 16);
+        if (a.vec_out) {
+#pragma unroll
+          for (int e = 0; e < HD / 32; e += 2) *reinterpret_cast<uint2*>(dst + 2 * e) = uint2{u[e], u[e + 1]};
         } else {
-          const float inv = den != 0.f ? 1.0f / den : 0.f;
-          uint16_t* dst = a.out + (int64_t)(w.q0 + rr / a.group) * a.out_stride +
-                          (int64_t)(kvh * a.group + rr % a.group) * HD + seg * (HD / 16);
-          uint32_t u[HD / 32];
 #pragma unroll
-          for (int e = 0; e < HD / 32; ++e)
-            u[e] = (uint32_t)T::from_f32(den != 0.f ? y[2 * e] * inv : 0.f) |
-                   ((uint32_t)T::from_f32(den != 0.f ? y[2 * e + 1] * inv : 0.f) << 16);
-          if (a.vec_out) {
-#pragma unroll
-            for (int e = 0; e < HD / 32; e += 2) *reinterpret_cast<uint2*>(dst + 2 * e) = uint2{u[e], u[e + 1]};
-          } else {
-#pragma unroll
-            for (int e = 0; e < HD / 16; ++e) dst[e] = (uint16_t)(u[e / 2] >> (16 * (e & 1)));
-          }
-        }
-      }
-    } else {
-      const int rr = row0 + i * RT + c;
-      if (c < RT && rr < w.rows) {
-        if (!whole) {
-          const int64_t pr = part0 + wave * QT * RT + i * RT + c;
-#pragma unroll
-          for (int p = 0; p < NP; ++p)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-              for (int h = 0; h < NH; ++h)
-                *reinterpret_cast<f4*>(a.part + pr * HD + p * PW + g * (PW / 4) + 4 * NH * e + 4 * h) =
-                    f4{value(p, e, h, 0), value(p, e, h, 1), value(p, e, h, 2), value(p, e, h, 3)};
-          if (g == 0) {
-            a.part_ml[2 * pr] = ref[i];
-            a.part_ml[2 * pr + 1] = l[i];
-          }
-        } else {
-          const float inv = l[i] != 0.f ? 1.0f / l[i] : 0.f;
-          uint16_t* dst = a.out + (int64_t)(w.q0 + rr / a.group) * a.out_stride +
-                          (int64_t)(kvh * a.group + rr % a.group) * HD + g * (PW / 4);
-#pragma unroll
-          for (int p = 0; p < NP; ++p)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-              for (int h = 0; h < NH; ++h) {
-                uint16_t y[4];
-#pragma unroll
-                for (int b = 0; b < 4; ++b) y[b] = T::from_f32(l[i] != 0.f ? value(p, e, h, b) * inv : 0.f);
-                uint16_t* to = dst + p * PW + 4 * NH * e + 4 * h;
-                if (a.vec_out) {
-                  *reinterpret_cast<uint2*>(to) =
-                      uint2{(uint32_t)y[0] | ((uint32_t)y[1] << 16), (uint32_t)y[2] | ((uint32_t)y[3] << 16)};
-                } else {
-#pragma unroll
-                  for (int b = 0; b < 4; ++b) to[b] = y[b];
-                }
-              }
+          for (int e = 0; e < HD / 16; ++e) dst[e] = (uint16_t)(u[e / 2] >> (16 * (e & 1)));
         }
       }
     }
   }
-  if (KVSPLIT) __syncthreads();  // the rows have been read: LDS is free for the next stretch's codes
+  __syncthreads();  // the rows have been read: LDS is free for the next stretch's codes
   }
 }
 
@@ -861,7 +686,7 @@ constexpr int kAttnCus = 256;
 struct AttnPlan {
   bool few, many;
   bool fold;                      // tiles of 8 rows in the kernel for few rows
-  int qt_few, qt_many;
+  int qt_few;
   int64_t tiles_few, tiles_many;  // bounds of the row tiles per kv head
   int wgs_few, wgs_many;          // workgroups per kv head that share the keys; 0: one for each tile
   int64_t part_rows_few, part_rows;
@@ -880,11 +705,10 @@ AttnPlan attn_plan(int64_t T, int64_t R, int64_t n_q, int64_t n_kv, int64_t hd, 
   p.fold = few_rows <= 8;
   p.qt_few = few_rows <= 16 || hd == 256 ? 1 : 2;
   const int64_t br_few = p.fold ? 8 : 16 * p.qt_few;
-  p.qt_many = hd == 256 ? 1 : 2;
   const int64_t seqs = std::min(R, T);
   p.tiles_few = T * group / br_few + seqs;
   if (p.many) p.tiles_few = std::min(p.tiles_few, seqs * (kAttnFewRows / br_few));
-  p.tiles_many = T * group / (64 * p.qt_many) + seqs;
+  p.tiles_many = T * group / attn_rows_br((int)hd) + seqs;
   // As many workgroups as the CUs hold at once, each with an equal share of all
   // keys.  Not for short keys, where joining the parts would take longer than
   // they, nor for more row tiles than workgroups of the kernel for many rows.
@@ -893,7 +717,7 @@ AttnPlan attn_plan(int64_t T, int64_t R, int64_t n_q, int64_t n_kv, int64_t hd, 
   if (p.many && long_keys && p.tiles_many * n_kv < 2 * kAttnCus)
     p.wgs_many = (int)std::max<int64_t>(1, 2 * kAttnCus / n_kv);
   p.part_rows_few = (int64_t)2 * p.wgs_few * n_kv * br_few;
-  p.part_rows = p.part_rows_few + (int64_t)2 * p.wgs_many * n_kv * 64 * p.qt_many;
+  p.part_rows = p.part_rows_few + (int64_t)2 * p.wgs_many * n_kv * attn_rows_br((int)hd);
   if (p.part_rows > 0) p.bytes = p.part_rows * (hd + 2) * 4 + T * group * 16;
   return p;
 }
@@ -907,9 +731,9 @@ void launch_attn(const AttnPlan& p, Kv4AttnArgs a, int64_t n_kv, int64_t n_q, hi
     b.wgs = p.wgs_few;
     b.part_row0 = 0;
     const dim3 grid((unsigned)(p.wgs_few ? p.wgs_few : p.tiles_few), (unsigned)n_kv);
-    if (p.fold) kv4_attn_kernel<T, HD, 1, true, true><<<grid, 256, 0, st>>>(b);
-    else if (p.qt_few == 1) kv4_attn_kernel<T, HD, 1, true, false><<<grid, 256, 0, st>>>(b);
-    else if constexpr (HD != 256) kv4_attn_kernel<T, HD, 2, true, false><<<grid, 256, 0, st>>>(b);
+    if (p.fold) kv4_attn_kernel<T, HD, 1, true><<<grid, 256, 0, st>>>(b);
+    else if (p.qt_few == 1) kv4_attn_kernel<T, HD, 1, false><<<grid, 256, 0, st>>>(b);
+    else if constexpr (HD != 256) kv4_attn_kernel<T, HD, 2, false><<<grid, 256, 0, st>>>(b);
   }
   if (p.many) {
     Kv4AttnArgs b = a;
@@ -917,8 +741,8 @@ void launch_attn(const AttnPlan& p, Kv4AttnArgs a, int64_t n_kv, int64_t n_q, hi
     b.rows_upto = INT32_MAX;
     b.wgs = p.wgs_many;
     b.part_row0 = (int)p.part_rows_few;
-    const dim3 grid((unsigned)(p.wgs_many ? p.wgs_many : p.tiles_many), (unsigned)n_kv);
-    kv4_attn_kernel<T, HD, HD == 256 ? 1 : 2, false, false><<<grid, 256, 0, st>>>(b);
+    const dim3 grid((unsigned)((p.wgs_many ? p.wgs_many : p.tiles_many) * n_kv));
+    launch_attn_rows(b, HD, T::code, grid, st);
   }
   if (p.part_rows > 0) {
     const int64_t rows = a.T * n_q;
@@ -980,7 +804,7 @@ extern "C" int cek_kv4_attention(const void* q, const void* cache, const int32_t
     a.part_ml = a.part + p.part_rows * hd;
     a.meta = reinterpret_cast<int4*>(a.part_ml + p.part_rows * 2);
   }
-  if (p.tiles_few > INT32_MAX || p.tiles_many > INT32_MAX || p.part_rows > INT32_MAX || T * n_q > INT32_MAX)
+  if (p.tiles_few > INT32_MAX || p.tiles_many * n_kv > INT32_MAX || p.part_rows > INT32_MAX || T * n_q > INT32_MAX)
     return CEK_ERR_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
 #define CEK_GO(D)                                                       \
