@@ -131,7 +131,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
   u4 kc;              // KW words
   uint2 va, vb;       // four values of four tokens: of the first and the second 16
   uint32_t pw = 0;    // a token's parameters
-  float none = 0.f;   // -infinity where it lies in no block
+  float p_none = 0.f; // -infinity where it lies in no block
   auto load = [&](int t0, const Blocks& x) {
     auto tok = [&](int t) { return (t0 + t) & (bs - 1); };
     const uint8_t* kb = at_block(x.k) + tok(16 * k_run) * (HD / 2);
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
     if (wave < 2) {
       // parameters 0 for tokens that do not exist, whatever lies there
       const bool out = outside(x.p);
-      none = out ? -INFINITY : 0.f;
+      p_none = out ? -INFINITY : 0.f;
       pw = *reinterpret_cast<const uint32_t*>(at_block(x.p) + 4 * tok(p_tok) + p_base);
       pw = out | (t0 + p_tok >= end) ? 0u : pw;
     }
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
       const float s = kv4_step(pw) * qmul;
       par[buf][0][lane] = s;
       par[buf][1][lane] = fmaf(-7.5f, s, kv4_centre(pw) * qmul);
-      if (c == 0) gone[buf][g] = none;
+      if (c == 0) gone[buf][g] = p_none;
     }
     if (wave == 1 && lane < ST) {
       par[buf][2][lane] = kv4_step(pw);
@@ -249,38 +249,50 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
       const int t = t0 + 16 * h + 4 * g + e;
       return (t <= pos[i]) & (t < end) & (t > pos[i] - window);  // no branches
     };
-    f4 acc[QT][2];
+    // all reads of one product ahead of it: K's and the parameters first, V's behind
+    // the first product, so that they come while the weights are computed
+    u4 kf[2 * ND], vf[NV];
+    f4 acc[QT][2], sk[2], mk[2], sv[2], mv[2];
+    float none[2];
+#pragma unroll
+    for (int n = 0; n < 2 * ND; ++n) kf[n] = k_op[buf][2 * j * ND + n][lane];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = 32 * j + 16 * h + 4 * g;
+      sk[h] = *reinterpret_cast<const f4*>(&par[buf][0][at]);
+      mk[h] = *reinterpret_cast<const f4*>(&par[buf][1][at]);
+      sv[h] = *reinterpret_cast<const f4*>(&par[buf][2][at]);
+      none[h] = gone[buf][2 * j + h];
+    }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int i = 0; i < QT; ++i) acc[i][h] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int n = 0; n < ND; ++n) {
-        const u4 f = k_op[buf][(2 * j + h) * ND + n][lane];
+      for (int n = 0; n < ND; ++n)
 #pragma unroll
-        for (int i = 0; i < QT; ++i) acc[i][h] = mfma16x16x32<F16>(f, qf[i][n], acc[i][h]);
-      }
+        for (int i = 0; i < QT; ++i) acc[i][h] = mfma16x16x32<F16>(kf[h * ND + n], qf[i][n], acc[i][h]);
     }
+#pragma unroll
+    for (int x = 0; x < NV; ++x) vf[x] = v_op[buf][j * NV + x][lane];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) mv[h] = *reinterpret_cast<const f4*>(&par[buf][3][32 * j + 16 * h + 4 * g]);
+    __builtin_amdgcn_sched_barrier(0);
     // x - ref, in place of the sums
     float xm[QT], top = -1.f;
-    f4 sv[2], mv[2];
 #pragma unroll
     for (int i = 0; i < QT; ++i) xm[i] = -INFINITY;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int at = 32 * j + 16 * h + 4 * g;
-      const f4 sk = *reinterpret_cast<const f4*>(&par[buf][0][at]), mk = *reinterpret_cast<const f4*>(&par[buf][1][at]);
-      sv[h] = *reinterpret_cast<const f4*>(&par[buf][2][at]);
-      mv[h] = *reinterpret_cast<const f4*>(&par[buf][3][at]);
-      const float none = gone[buf][2 * j + h];
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = fmaxf(top, sv[h][e]);
 #pragma unroll
       for (int i = 0; i < QT; ++i) {
-        const float base = none - ref[i];
+        const float base = none[h] - ref[i];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float y = fmaf(sk[e], acc[i][h][e], fmaf(mk[e], qsum[i], base));
+          float y = fmaf(sk[h][e], acc[i][h][e], fmaf(mk[h][e], qsum[i], base));
           if constexpr (masked) y = sees(i, h, e) ? y : -INFINITY;
           acc[i][h][e] = y;
           xm[i] = fmaxf(xm[i], y);
@@ -346,12 +358,10 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < QT; ++i) wsum[i] = mfma16x16x32<F16>(halves, pf[i], wsum[i]);
 #pragma unroll
-    for (int x = 0; x < NV; ++x) {
-      const u4 f = v_op[buf][j * NV + x][lane];
+    for (int x = 0; x < NV; ++x)
 #pragma unroll
       for (int i = 0; i < QT; ++i)
-        o[i][x / (NH * 4)][x / 4 % NH][x % 4] = mfma16x16x32<F16>(f, pf[i], o[i][x / (NH * 4)][x / 4 % NH][x % 4]);
-    }
+        o[i][x / (NH * 4)][x / 4 % NH][x % 4] = mfma16x16x32<F16>(vf[x], pf[i], o[i][x / (NH * 4)][x / 4 % NH][x % 4]);
   };
 
   if (begin < end) {
