@@ -598,6 +598,15 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   }
 }
 
+// Largest of the 64 lanes, uniform, by DPP (wave_sum_dpp's pattern).
+__device__ inline float wave_max_dpp(float v) {
+  v = fmaxf(v, CEK_DPP_F32(v, 0xB1));
+  v = fmaxf(v, CEK_DPP_F32(v, 0x4E));
+  v = fmaxf(v, CEK_DPP_F32(v, 0x141));
+  v = fmaxf(v, CEK_DPP_F32(v, 0x140));
+  return over_rows(v, [](float p, float q) { return fmaxf(p, q); });
+}
+
 // Joins the parts of the rows that several workgroups share.  Part 0 of a row is
 // its first workgroup's, part p that of the p-th after it, two row tiles on each.
 // WIDE: few rows of many parts, a workgroup for 32 values of a row, eight groups of
@@ -637,11 +646,11 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4AttnArgs a, int n
         for (int e = 0; e < E; ++e) v[i][e] = row[e];
       }
       if (p0 == 0) {
-        nt = fmaxf(top, wave_max(r));
+        nt = fmaxf(top, wave_max_dpp(r));
         const float keep = __builtin_amdgcn_exp2f(top - nt);
         f = __builtin_amdgcn_exp2f(r - nt);
         top = nt;
-        den = fmaf(den, keep, wave_sum(f * l));
+        den = fmaf(den, keep, wave_sum_dpp(f * l));
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] *= keep;
       }
