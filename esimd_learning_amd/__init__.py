@@ -10,6 +10,8 @@ Layout:
   build.py, setup.py         build recipe (hipcc for libcek.so, PyTorch-ROCm
                              cpp_extension for the torch modules)
   cabi.py                    ctypes binding of include/cek.h
+  layer.py, kv4.py           a decoder layer's decode step, and the 4-bit key/value
+                             cache of a stack of them
   synthetic.py               seeded synthetic inputs (quantisation recipe)
 
 ``import esimd_learning_amd`` puts the drop-in package on ``sys.path`` so

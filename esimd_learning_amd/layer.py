@@ -1,10 +1,11 @@
-"""One Gemma-style decoder-layer decode step from the custom ops (BASELINE config 5).
+"""One Gemma-style decoder-layer decode step from the custom ops.
 
     h1, r1 = add_rmsnorm(hidden, residual, w_in)          esimd_fused_add_rms_norm_batched
     qkv    = h1 @ Wqkv^T * sqkv                           esimd_gemv_fp8_pern
                                    (the two as one launch: esimd_fused_add_rms_norm_gemv_fp8)
     q, k   = per-head RMSNorm + RoPE (in place in qkv)     esimd_qk_norm_rope
-    a      = attention(q, k, v)        -- out of scope: a copy of q stands in for its output
+    a      = attention(q, k, v)        with a key/value cache (``kv``): esimd_kv4_cache_write,
+                                       esimd_kv4_attention; without: a copy of q stands in
     o      = a @ Wo^T * so                                esimd_gemv_fp8_pern
     h2, r2 = add_rmsnorm(o, r1, w_post)                   esimd_fused_add_rms_norm_batched
     g      = gelu_tanh(h2 @ Wg^T * sg) * (h2 @ Wu^T * su) esimd_gemv_fp8_gelu_and_mul
@@ -26,9 +27,9 @@ workgroups of QKV and gate/up costs more than the norm launch it saves.
 
 With ``fuse_tails`` (the default; fp16/bf16 hand-offs, no ``fuse_norm``)
 QK-norm+RoPE runs in the QKV GEMV (esimd_gemv_fp8_qk_norm_rope: per head,
-the workgroup that finishes the head's rows last), which also writes the
-rotated q heads into the attention stand-in's output -- two launches fewer
-per step, the same values bit for bit.  Its arrival counters are allocated
+the workgroup that finishes the head's rows last), which without a cache also
+writes the rotated q heads into the attention stand-in's output -- two launches
+fewer per step, the same values bit for bit.  Its arrival counters are allocated
 (zeroed) once here and left zero by every call.
 
 With ``act_fp8=True`` the two norm -> GEMV hand-offs carry e4m3 activations
@@ -53,6 +54,12 @@ Two launches fewer per layer; the values match the unfused layer to within
 the rounding of the moved 1 / rms, not bit for bit (``defer_norm=False``
 gives the step that equals the separate ops bit for bit).
 
+With ``kv`` (a layer of a KV4Cache) the new tokens' k and v heads are
+quantised from their columns of qkv into the 4-bit cache and the q heads
+attend to it from theirs: two launches (three where the keys are split over
+workgroups), no copy.  Rows of a step that hold no token (behind cu_q's last)
+are padding: nothing is stored for them and their outputs mean nothing.
+
 The intermediate buffers and counters are allocated once in the
 constructor, so at decode sizes a step enqueues only kernels: it can be
 captured in a HIP graph (``capture``) and replayed, which removes host launch
@@ -60,7 +67,8 @@ overhead from the latency-bound small kernels between the GEMVs.  (One
 exception: with ``act_fp8`` at M = 64 the a8w8 op splits K where K exceeds
 5120 or N 16384 (a wide gate/up matrix) and takes its fp32 workspace from
 PyTorch's caching allocator on every call -- inside a captured graph, from the
-graph's memory pool.)
+graph's memory pool.  The attention's workspace, where keys are split, is taken
+the same way.)
 """
 
 import torch
@@ -85,7 +93,7 @@ class GemmaDecodeLayer:
         nqkv = self.Wqkv.shape[0]
         mk = lambda n: torch.empty(M, n, dtype=dtype, device=device)  # noqa: E731
         self.qkv = mk(nqkv)
-        self.attn = mk(self.nq * self.hd)
+        self.attn = mk(self.nq * self.hd).zero_()   # padding rows of an attention keep this
         self.o = mk(self.hidden)
         self.gu = mk(2 * self.mlp)
         self.act = mk(self.mlp)
@@ -130,8 +138,21 @@ class GemmaDecodeLayer:
     def weight_bytes(self):
         return sum(w.numel() for w in (self.Wqkv, self.Wo, self.Wgu, self.Wd))
 
-    def step(self, hidden, residual, positions, ss_in=None, next_norm=None):
+    def _attend(self, kv):
+        """The attention of the step's rows: over kv's cache, or its stand-in
+        (which fuse_tails has written already)."""
+        hd, nq, nk = self.hd, self.nq, self.nk
+        if kv is not None:
+            kv.attend(self.qkv[:, : nq * hd], self.qkv[:, nq * hd:(nq + nk) * hd],
+                      self.qkv[:, (nq + nk) * hd:(nq + 2 * nk) * hd], self.attn)
+        elif not self.fuse_tails:
+            self.attn.copy_(self.qkv[:, : nq * hd])
+
+    def step(self, hidden, residual, positions, ss_in=None, next_norm=None, kv=None):
         """hidden, residual: [M, hidden] (residual updated in place); returns out.
+
+        kv: this layer's KV4Layer, after its cache's advance() for the step, whose
+        positions the caller passes; None: no attention, its stand-in.
 
         defer_norm only: with ``ss_in`` (the previous layer's ss_d) hidden
         already holds residual * w_in * 2^-shift_in of the previous layer's
@@ -140,9 +161,9 @@ class GemmaDecodeLayer:
         produces that for the next layer and ss_d."""
         o, hd, nq, nk = self.ops, self.hd, self.nq, self.nk
         if self.fuse_norm:
-            return self._step_fused(hidden, residual, positions)
+            return self._step_fused(hidden, residual, positions, kv)
         if self.defer_norm:
-            return self._step_defer(hidden, residual, positions, ss_in, next_norm)
+            return self._step_defer(hidden, residual, positions, ss_in, next_norm, kv)
         if ss_in is not None or next_norm is not None:
             raise ValueError("ss_in / next_norm need defer_norm")
         if self.act_fp8:
@@ -150,15 +171,16 @@ class GemmaDecodeLayer:
             o.esimd_gemm_fp8_a8w8(self.q8.view(torch.uint8), self.s8, self.Wqkv8, self.sqkv32, self.qkv)
         else:
             o.esimd_fused_add_rms_norm_batched(hidden, residual, self.w_in, self.eps)
-            if self.fuse_tails:   # the tail also writes the attention stand-in's output
+            if self.fuse_tails:   # without a cache the tail also writes the attention stand-in's output
                 o.esimd_gemv_fp8_qk_norm_rope(hidden, self.Wqkv, self.sqkv, self.qkv, self.qw, self.kw, positions,
-                                              nq, nk, self.eps, self.theta, True, self.cnt_rope, self.attn)
+                                              nq, nk, self.eps, self.theta, True, self.cnt_rope,
+                                              self.attn if kv is None else None)
             else:
                 o.esimd_gemv_fp8_pern(hidden, self.Wqkv, self.sqkv, self.qkv, self.Wqkv.shape[0], self.hidden)
         if not self.fuse_tails:
             o.esimd_qk_norm_rope(self.qkv[:, : nq * hd], self.qkv[:, nq * hd:(nq + nk) * hd], self.qw, self.kw,
                                  positions, self.eps, self.theta, True)
-            self.attn.copy_(self.qkv[:, : nq * hd])                # attention stand-in
+        self._attend(kv)
         o.esimd_gemv_fp8_pern(self.attn, self.Wo, self.so, self.o, self.hidden, nq * hd)
         if self.act_fp8:
             o.esimd_fused_add_rms_norm_quant_fp8(self.o, residual, self.w_post, self.eps, self.q8, self.s8)
@@ -178,7 +200,7 @@ class GemmaDecodeLayer:
         o.esimd_gemv_fp8_pern(self.act, self.Wd, self.sd, self.out, self.hidden, self.mlp)
         return self.out
 
-    def _step_fused(self, hidden, residual, positions):
+    def _step_fused(self, hidden, residual, positions, kv):
         o, hd, nq, nk = self.ops, self.hd, self.nq, self.nk
         if self.act_fp8:
             o.esimd_fused_add_rms_norm_quant_gemv_fp8(hidden, residual, self.w_in, self.eps, self.r_mid, self.q8,
@@ -188,7 +210,7 @@ class GemmaDecodeLayer:
                                                 self.sqkv, self.qkv)
         o.esimd_qk_norm_rope(self.qkv[:, : nq * hd], self.qkv[:, nq * hd:(nq + nk) * hd], self.qw, self.kw,
                              positions, self.eps, self.theta, True)
-        self.attn.copy_(self.qkv[:, : nq * hd])                    # attention stand-in
+        self._attend(kv)
         o.esimd_gemv_fp8_pern(self.attn, self.Wo, self.so, self.o, self.hidden, nq * hd)
         glu = self.fuse_glu
         y = self.act if glu else self.gu
@@ -203,16 +225,18 @@ class GemmaDecodeLayer:
         o.esimd_gemv_fp8_pern(self.act, self.Wd, self.sd, self.out, self.hidden, self.mlp)
         return self.out
 
-    def _step_defer(self, hidden, residual, positions, ss_in, next_norm):
-        o, hd, nq, nk, eps = self.ops, self.hd, self.nq, self.nk, self.eps
+    def _step_defer(self, hidden, residual, positions, ss_in, next_norm, kv):
+        o, nq, nk, eps = self.ops, self.nq, self.nk, self.eps
+        q_out = self.attn if kv is None else None   # the attention stand-in's output
         if ss_in is None:
             o.esimd_fused_add_rms_norm_batched(hidden, residual, self.w_in, eps)
             o.esimd_gemv_fp8_qk_norm_rope(hidden, self.Wqkv, self.sqkv, self.qkv, self.qw, self.kw, positions,
-                                          nq, nk, eps, self.theta, True, self.cnt_rope, self.attn)
+                                          nq, nk, eps, self.theta, True, self.cnt_rope, q_out)
         else:
             o.esimd_gemv_fp8_qk_norm_rope_rs(hidden, self.Wqkv, self.sqkv, self.qkv, self.qw, self.kw, positions,
                                              nq, nk, eps, self.theta, True, self.cnt_rope, ss_in,
-                                             eps * 4.0 ** -self.shift_in, self.attn)
+                                             eps * 4.0 ** -self.shift_in, q_out)
+        self._attend(kv)
         o.esimd_gemv_fp8_add_rms_norm_defer(self.attn, self.Wo, self.so, residual, self.w_post, self.o, self.ss_o,
                                             self.shift_post)
         o.esimd_gemv_fp8_gelu_and_mul_rs(self.o, self.Wgu, self.sgu, self.act, self.ss_o,
@@ -225,13 +249,13 @@ class GemmaDecodeLayer:
                                                 shift_next)
         return self.out
 
-    def capture(self, hidden, residual, positions, stream=None):
+    def capture(self, hidden, residual, positions, stream=None, kv=None):
         """Capture one step on fixed input buffers in a HIP graph; replay with replay()."""
         s = stream or torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph, stream=s):
-            self.step(hidden, residual, positions)
+            self.step(hidden, residual, positions, kv=kv)
         torch.cuda.current_stream().wait_stream(s)
         return self.graph
 
@@ -240,7 +264,7 @@ class GemmaDecodeLayer:
         return self.out
 
 
-def forward(layers, hidden, residual, positions):
+def forward(layers, hidden, residual, positions, kv=None):
     """A decode forward over `layers` in sequence: each layer's output buffer
     is the next layer's hidden state (which that layer's first norm
     overwrites), and the residual stream is updated in place by every layer.
@@ -248,26 +272,41 @@ def forward(layers, hidden, residual, positions):
     deferred across the down projection and its QKV GEMV.  Returns the last
     layer's output buffer (for a deferred pair as for any other: the down
     projection's output is only the normed input of the next layer, the
-    last layer's is the plain one)."""
+    last layer's is the plain one).
+
+    kv: a KV4Cache with a layer for each of `layers` and M tokens a step, after
+    its advance(); positions are then its positions."""
+    if kv is not None and (len(kv.layers) != len(layers) or any(x.M != kv.tokens for x in layers)):
+        raise ValueError("kv must have a layer for each layer and as many tokens a step as they have rows")
     h, ss = hidden, None
     for i, layer in enumerate(layers):
         nxt = layers[i + 1] if i + 1 < len(layers) else None
         chain = nxt is not None and layer.defer_norm and nxt.defer_norm
+        kv_i = None if kv is None else kv.layers[i]
         if layer.defer_norm:
-            h = layer.step(h, residual, positions, ss_in=ss, next_norm=(nxt.w_in, nxt.shift_in) if chain else None)
+            h = layer.step(h, residual, positions, ss_in=ss, next_norm=(nxt.w_in, nxt.shift_in) if chain else None,
+                           kv=kv_i)
         else:
-            h = layer.step(h, residual, positions)
+            h = layer.step(h, residual, positions, kv=kv_i)
         ss = layer.ss_d if chain else None
     return h
 
 
-def capture_forward(layers, hidden, residual, positions, stream=None):
+def capture_forward(layers, hidden, residual, positions, stream=None, kv=None, q_lens=None, keep_lens=None,
+                    max_q_len=0, max_kv_len=0):
     """forward() over `layers` captured in one HIP graph, as a serving loop
-    captures a model's whole decode step (no launch gap between layers)."""
+    captures a model's whole decode step (no launch gap between layers).
+
+    With ``kv`` and ``q_lens`` the graph begins with kv.advance(q_lens, keep_lens,
+    max_q_len, max_kv_len) on these buffers, so that every replay is the next step:
+    the caller writes the tokens' hidden states (and, where they change, q_lens and
+    keep_lens) between replays.  Without ``q_lens`` the caller advances kv itself."""
     s = stream or torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g, stream=s):
-        forward(layers, hidden, residual, positions)
+        if kv is not None and q_lens is not None:
+            kv.advance(q_lens, keep_lens, max_q_len, max_kv_len)
+        forward(layers, hidden, residual, positions, kv)
     torch.cuda.current_stream().wait_stream(s)
     return g
