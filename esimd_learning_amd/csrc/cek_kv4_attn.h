@@ -21,6 +21,7 @@ struct Kv4AttnArgs {
   int rows_above, rows_upto;  // this launch serves requests with that many rows
   int wgs;                    // workgroups per kv head that share the keys evenly; 0: keys stay whole
   int part_row0;              // first partial row of this launch
+  int part_rows;              // of all
   int vec_q, vec_out;
   float scale;
 };
@@ -67,7 +68,8 @@ struct Kv4List {
   __device__ inline int units(const Req& x) const {
     return len ? (int)(((unsigned)max(x.kv - x.lo, 1) + (unsigned)len - 1u) / (unsigned)len) : 1;
   }
-  // Units of `step` tokens, or as many times that as keep their number in 30 bits.
+  // Units of `step` tokens, or as many times that as keep their number in 30 bits
+  // (offsets that do not ascend may count rows so often that none does: no work then).
   __device__ inline void share(const Req& first, int step) {
     const int lane = threadIdx.x & 63;
     for (len = step;; len *= 2) {
@@ -80,6 +82,10 @@ struct Kv4List {
       }
       total = __builtin_amdgcn_readlane(wave_scan_incl(n), 63);
       if (wave_sum_dpp(sum) < 0x1p30f) return;
+      if (len >= 1 << 29) {
+        total = 0;
+        return;
+      }
     }
   }
   // Workgroup j of n gets each = total / n units, the first `more` one more.

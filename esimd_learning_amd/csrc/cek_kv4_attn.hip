@@ -624,11 +624,13 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4AttnArgs a, int n
   const int kvh = h / a.group;
   const int c0 = a.cu_q[0], c1 = a.cu_q[a.R];
   const int4 mt = a.meta[t * a.group + h - kvh * a.group];
-  if (t < c0 || t >= c1 || mt.y <= 1) return;
+  // (rows that offsets out of order left without a worker: whatever the workspace held)
+  if (t < c0 || t >= c1 || mt.y <= 1 || mt.x < 0 || mt.z < 0 || mt.w < 0) return;
   const int parts = mt.y, grp = WIDE ? tid >> 5 : 0;
   const int d0 = WIDE ? (int)blockIdx.y * 32 + (tid & 31) : lane * E;
   const int64_t row0 = mt.x + (int64_t)kvh * mt.w;
   auto row_of = [&](int p) { return row0 + (int64_t)mt.z * (p > 0 ? 2 * p - 1 : 0); };
+  if (row_of(parts - 1) >= a.part_rows) return;
   float top = kAttnNone, den = 0.f, y[E] = {};
   for (int base = 0; base < parts; base += 64) {
     // a lane for a part: references and sums; then the parts' rows by their weights
@@ -785,7 +787,7 @@ extern "C" int cek_kv4_attention(const void* q, const void* cache, const int32_t
     return CEK_ERR_INVALID;
   if (T == 0 || R == 0) return CEK_OK;
   if (!q || !cache || !block_tables || !kv_lens || !cu_q || !out || !aligned(cache, 16)) return CEK_ERR_INVALID;
-  if (T * (n_q / n_kv) > INT32_MAX / 2) return CEK_ERR_UNSUPPORTED;  // rows of a kv head
+  if (T * (n_q / n_kv) > INT32_MAX / 4) return CEK_ERR_UNSUPPORTED;  // rows of a kv head
   if (workspace_bytes < 0 || (workspace && !aligned(workspace, 16))) return CEK_ERR_INVALID;
   a.q = static_cast<const uint16_t*>(q);
   a.out = static_cast<uint16_t*>(out);
@@ -812,6 +814,7 @@ extern "C" int cek_kv4_attention(const void* q, const void* cache, const int32_t
     a.part = static_cast<float*>(workspace);
     a.part_ml = a.part + p.part_rows * hd;
     a.meta = reinterpret_cast<int4*>(a.part_ml + p.part_rows * 2);
+    a.part_rows = (int)std::min<int64_t>(p.part_rows, INT32_MAX);
   }
   if (p.tiles_few > INT32_MAX || p.tiles_many * n_kv > INT32_MAX || p.part_rows > INT32_MAX || T * n_q > INT32_MAX)
     return CEK_ERR_UNSUPPORTED;

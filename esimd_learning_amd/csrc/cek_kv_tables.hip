@@ -159,8 +159,9 @@ __global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(KvTablesArgs 
     at[2] += (I)gone[j];
   }
   const int taken = (int)total[0], rows = (int)total[1];
-  // (lengths of more blocks than there are return no more than the ring has room for)
-  const int given = (int)min((int64_t)total[2], (int64_t)a.cap - count + taken);
+  // (lengths of more blocks than there are return no more than the ring has room for
+  // beside all that was free: no place is read and written)
+  const int given = (int)min((int64_t)total[2], (int64_t)a.cap - count);
   if (tid == 0) {
     at_need[a.R] = taken;
     a.cu_q[a.R] = at_q[a.R] = rows;

@@ -283,8 +283,10 @@ def esimd_kv_block_tables(
     new block is never refused for one.
 
     kv_lens_out may be kv_lens and ring_state_out ring_state (a captured step
-    replayed); no other two may share memory.  Lengths are taken within 0 ..
-    the table's reach, keep_lens within 0 .. kv_lens.  At most 4096 requests."""
+    replayed); no other output may share memory with another argument.  A block
+    is free or one request's: what several requests read is not shared here.
+    Lengths are taken within 0 .. the table's reach, keep_lens within 0 ..
+    kv_lens (2^31 - 1 keeps all).  At most 4096 requests."""
     _ops.esimd_kv_block_tables(kv_lens, keep_lens, q_lens, block_size, free_ring, ring_state, block_tables, kv_lens_out,
                                ring_state_out, cu_q, slot_mapping, positions, status)
 
@@ -324,8 +326,8 @@ def esimd_kv4_attention(
     keys and values lie in the blocks of block_tables[r].  Row at position p
     sees keys 0 .. p, with window > 0 keys p - window + 1 .. p; query head h
     reads kv head h / (n_q / n_kv).  out = sum softmax(scale q k) v; rows without
-    a key (kv_lens 0) are zero; rows of q before cu_q[0] or behind cu_q[R] are
-    left as they were.  Tokens whose table entry lies outside the cache count
+    a key (kv_lens 0) are zero; rows of out before cu_q[0] or behind cu_q[R] are
+    left as they were.  cu_q ascends; |q| up to 2^100.  Tokens whose table entry lies outside the cache count
     as absent.  max_q_len and max_kv_len, the longest of the batch (0: not
     known), choose the kernels; wrong ones cost time, not results."""
     _ops.esimd_kv4_attention(q, kv_cache, block_tables, kv_lens, cu_q, out, scale, max_q_len, max_kv_len, window)

@@ -390,8 +390,9 @@ int cek_qk_norm_rope(void* q, void* k, const void* qw, const void* kw, const int
  * cu_q [R + 1], slot_mapping and positions [T] (behind the last new token -1
  * and 0) and status [R] (0, or 1 not enough free blocks, 2 table too narrow, 3
  * more than T tokens: that request gets no token and takes no block).
- * kv_lens_out may be kv_lens and ring_state_out ring_state; other arrays must
- * not overlap.  R <= 4096.
+ * kv_lens_out may be kv_lens and ring_state_out ring_state; no other output may
+ * overlap an argument.  A block is free or one request's.  keep_lens beyond kv_lens
+ * keep all.  R <= 4096.
  *
  * cek_kv4_cache_write: k, v rows (strides in elements) quantised into the cache,
  * m = bf16((min + max) / 2), s = bf16(max(max - m, m - min) / 7.5), c =
@@ -403,7 +404,7 @@ int cek_qk_norm_rope(void* q, void* k, const void* qw, const void* kw, const int
  * q rows, the last tokens of request r, over its kv_lens[r] cached tokens; the
  * row at position p sees keys 0 .. p (window > 0: p - window + 1 .. p).  Rows
  * without a key are zero, rows outside cu_q[0] .. cu_q[R] left as they were.
- * Tokens in blocks outside the cache count as absent.  max_q_len and max_kv_len
+ * Tokens in blocks outside the cache count as absent.  cu_q ascends; |q| up to 2^100.  max_q_len and max_kv_len
  * (0: not known) choose the kernels and never change results beyond the order
  * of sums.  workspace: cek_kv4_attention_workspace_size bytes for the same
  * arguments, 16-byte aligned, no initialisation; with less the call does not
