@@ -607,78 +607,116 @@ __device__ inline float wave_max_dpp(float v) {
   return over_rows(v, [](float p, float q) { return fmaxf(p, q); });
 }
 
-// Joins the parts of the rows that several workgroups share.  Part 0 of a row is
-// its first workgroup's, part p that of the p-th after it, two row tiles on each.
-// WIDE: few rows of many parts, a workgroup for 32 values of a row, eight groups of
-// threads taking every eighth part; else a wave for a row.
-template <typename T, int HD, bool WIDE>
+// The parts of a row that several workgroups share.  Part 0 is its first
+// workgroup's, part p that of the p-th after it, two row tiles on each.
+struct Kv4Parts {
+  int64_t t, row0;
+  int h, n, step;
+  // Row t, head h of the call; n is 0 where there is nothing to join.
+  __device__ inline Kv4Parts(const Kv4AttnArgs& a, int64_t item, int n_q) {
+    t = item / n_q;
+    h = (int)(item - t * n_q);
+    n = 0;
+    if (t >= a.T) return;
+    const int kvh = h / a.group;
+    const int c0 = a.cu_q[0], c1 = a.cu_q[a.R];
+    const int4 mt = a.meta[t * a.group + h - kvh * a.group];
+    row0 = mt.x + (int64_t)kvh * mt.w;
+    step = mt.z;
+    n = mt.y;
+    // (rows that offsets out of order left without a worker: whatever the workspace held)
+    const bool no = (t < c0) | (t >= c1) | (mt.y <= 1) | (mt.x < 0) | (mt.z < 0) | (mt.w < 0);
+    if (no || row(n - 1) >= a.part_rows) n = 0;
+  }
+  __device__ inline int64_t row(int p) const { return row0 + (int64_t)step * (p > 0 ? 2 * p - 1 : 0); }
+};
+
+// Joins them: HD / 4 lanes a row, eight parts at a time on their way.
+template <typename T, int HD>
 __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4AttnArgs a, int n_q) {
-  constexpr int G = WIDE ? 8 : 1;         // groups of threads that share the parts
-  constexpr int E = WIDE ? 1 : HD / 64;   // values of a thread
-  constexpr int AHEAD = 8;                // parts of a group that are loaded at once
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int64_t item = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + (tid >> 6);
-  const int64_t t = item / n_q;
-  const int h = (int)(item - t * n_q);
-  if (t >= a.T) return;
-  const int kvh = h / a.group;
-  const int c0 = a.cu_q[0], c1 = a.cu_q[a.R];
-  const int4 mt = a.meta[t * a.group + h - kvh * a.group];
-  // (rows that offsets out of order left without a worker: whatever the workspace held)
-  if (t < c0 || t >= c1 || mt.y <= 1 || mt.x < 0 || mt.z < 0 || mt.w < 0) return;
-  const int parts = mt.y, grp = WIDE ? tid >> 5 : 0;
-  const int d0 = WIDE ? (int)blockIdx.y * 32 + (tid & 31) : lane * E;
-  const int64_t row0 = mt.x + (int64_t)kvh * mt.w;
-  auto row_of = [&](int p) { return row0 + (int64_t)mt.z * (p > 0 ? 2 * p - 1 : 0); };
-  if (row_of(parts - 1) >= a.part_rows) return;
-  float top = kAttnNone, den = 0.f, y[E] = {};
-  for (int base = 0; base < parts; base += 64) {
-    // a lane for a part: references and sums; then the parts' rows by their weights
-    const bool in = base + lane < parts;
-    const int64_t mine = row_of(in ? base + lane : 0);
-    const float r = in ? a.part_ml[2 * mine] : kAttnNone, l = in ? a.part_ml[2 * mine + 1] : 0.f;
-    const int n = min(64, parts - base);
-    float nt = 0.f, f = 0.f;
-    for (int p0 = 0; p0 < n; p0 += G * AHEAD) {  // the same for all lanes
-      float v[AHEAD][E];
+  constexpr int L = HD / 4, AHEAD = 8;
+  const Kv4Parts parts(a, (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L, n_q);
+  if (parts.n == 0) return;
+  const int d0 = (threadIdx.x % L) * 4;
+  float top = kAttnNone, den = 0.f;
+  f4 y = f4{0.f, 0.f, 0.f, 0.f};
+  for (int base = 0; base < parts.n; base += AHEAD) {
+    f4 v[AHEAD];
+    float2 ml[AHEAD];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const float* row = a.part + row_of(base + min(p0 + grp + G * i, n - 1)) * HD + d0;
+    for (int i = 0; i < AHEAD; ++i) {
+      const int64_t row = parts.row(min(base + i, parts.n - 1));
+      ml[i] = *reinterpret_cast<const float2*>(a.part_ml + 2 * row);
+      v[i] = *reinterpret_cast<const f4*>(a.part + row * HD + d0);
+    }
+    float nt = top;
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[i][e] = row[e];
-      }
-      if (p0 == 0) {
-        nt = fmaxf(top, wave_max_dpp(r));
-        const float keep = __builtin_amdgcn_exp2f(top - nt);
-        f = __builtin_amdgcn_exp2f(r - nt);
-        top = nt;
-        den = fmaf(den, keep, wave_sum_dpp(f * l));
+    for (int i = 0; i < AHEAD; ++i) nt = fmaxf(nt, ml[i].x);
+    const float keep = __builtin_amdgcn_exp2f(top - nt);
+    top = nt;
+    den *= keep;
+    y *= keep;
 #pragma unroll
-        for (int e = 0; e < E; ++e) y[e] *= keep;
-      }
+    for (int i = 0; i < AHEAD; ++i) {
+      const float f = base + i < parts.n ? __builtin_amdgcn_exp2f(ml[i].x - nt) : 0.f;
+      den = f != 0.f ? fmaf(f, ml[i].y, den) : den;
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const int p = p0 + grp + G * i;
-        const float w = __shfl(f, min(p, 63), 64), fp = p < n ? w : 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) y[e] = fp != 0.f ? fmaf(v[i][e], fp, y[e]) : y[e];
-      }
+      for (int e = 0; e < 4; ++e) y[e] = f != 0.f ? fmaf(v[i][e], f, y[e]) : y[e];
     }
   }
-  uint16_t* const dst = a.out + t * a.out_stride + (int64_t)h * HD;
-  if constexpr (WIDE) {
-    __shared__ float so[G][32];
-    so[grp][tid & 31] = y[0];
-    __syncthreads();
-    if (tid < 32) {
-      float v = 0.f;
+  const float inv = den != 0.f ? 1.0f / den : 0.f;
+  uint16_t u[4];
 #pragma unroll
-      for (int i = 0; i < G; ++i) v += so[i][tid];
-      dst[d0] = T::from_f32(den != 0.f ? v / den : 0.f);
-    }
+  for (int e = 0; e < 4; ++e) u[e] = T::from_f32(den != 0.f ? y[e] * inv : 0.f);
+  uint16_t* const dst = a.out + parts.t * a.out_stride + (int64_t)parts.h * HD + d0;
+  if (a.vec_out) {
+    *reinterpret_cast<uint2*>(dst) =
+        uint2{(uint32_t)u[0] | ((uint32_t)u[1] << 16), (uint32_t)u[2] | ((uint32_t)u[3] << 16)};
   } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) dst[d0 + e] = T::from_f32(den != 0.f ? y[e] / den : 0.f);
+    for (int e = 0; e < 4; ++e) dst[e] = u[e];
+  }
+}
+
+// Few rows of many parts: a workgroup for 32 values of a row, eight groups of
+// threads taking every eighth part.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void kv4_attn_join_wide_kernel(Kv4AttnArgs a, int n_q) {
+  constexpr int G = 8, AHEAD = 8;  // groups; parts of a group that are loaded at once
+  const int tid = threadIdx.x, lane = tid & 63, grp = tid >> 5;
+  const Kv4Parts parts(a, blockIdx.x, n_q);
+  if (parts.n == 0) return;
+  const int d0 = (int)blockIdx.y * 32 + (tid & 31);
+  float top = kAttnNone, den = 0.f, y = 0.f;
+  for (int base = 0; base < parts.n; base += 64) {
+    // a lane for a part: references and sums; then the parts' rows by their weights
+    const bool in = base + lane < parts.n;
+    const int64_t mine = parts.row(in ? base + lane : 0);
+    const float r = in ? a.part_ml[2 * mine] : kAttnNone, l = in ? a.part_ml[2 * mine + 1] : 0.f;
+    const int n = min(64, parts.n - base);
+    float v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) v[i] = a.part[parts.row(base + min(grp + G * i, n - 1)) * HD + d0];
+    const float nt = fmaxf(top, wave_max_dpp(r)), keep = __builtin_amdgcn_exp2f(top - nt);
+    const float f = __builtin_amdgcn_exp2f(r - nt);
+    top = nt;
+    den = fmaf(den, keep, wave_sum_dpp(f * l));
+    y *= keep;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int p = grp + G * i;
+      const float w = __shfl(f, p, 64), fp = p < n ? w : 0.f;
+      y = fp != 0.f ? fmaf(v[i], fp, y) : y;
+    }
+  }
+  __shared__ float so[G][32];
+  so[grp][tid & 31] = y;
+  __syncthreads();
+  if (tid < 32) {
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < G; ++i) v += so[i][tid];
+    a.out[parts.t * a.out_stride + (int64_t)parts.h * HD + d0] = T::from_f32(den != 0.f ? v / den : 0.f);
   }
 }
 
@@ -757,8 +795,8 @@ void launch_attn(const AttnPlan& p, Kv4AttnArgs a, int64_t n_kv, int64_t n_q, hi
   }
   if (p.part_rows > 0) {
     const int64_t rows = a.T * n_q;
-    if (rows <= 512) kv4_attn_join_kernel<T, HD, true><<<dim3((unsigned)rows, HD / 32), 256, 0, st>>>(a, (int)n_q);
-    else kv4_attn_join_kernel<T, HD, false><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a, (int)n_q);
+    if (rows <= 512) kv4_attn_join_wide_kernel<T, HD><<<dim3((unsigned)rows, HD / 32), 256, 0, st>>>(a, (int)n_q);
+    else kv4_attn_join_kernel<T, HD><<<(unsigned)((rows * (HD / 4) + 255) / 256), 256, 0, st>>>(a, (int)n_q);
   }
 }
 
