@@ -19,7 +19,7 @@ struct Kv4AttnArgs {
   Kv4Dims dm;
   int R, group, max_blocks, window;
   int rows_above, rows_upto;  // this launch serves requests with that many rows
-  int wgs;                    // workgroups per kv head that share the keys evenly; 0: keys stay whole
+  int wgs;                    // workgroups per kv head that share the keys; 0: keys stay whole
   int part_row0;              // first partial row of this launch
   int part_rows;              // of all
   int vec_q, vec_out;
@@ -36,7 +36,7 @@ typedef const __attribute__((address_space(4))) int32_t* const_i32;  // scalar l
 struct Kv4Work {
   int r, q0, rows, kv, n_new, lo, tile;
   int unit, units, all;  // all: the tile's units
-  int first;             // the tile's first unit in the list
+  int first, span;       // the tile's first unit in the list; how far the stretch reaches there
 };
 
 // The work list: every request has ceil(rows / BR) tiles of rows, and each tile its
@@ -44,11 +44,21 @@ struct Kv4Work {
 // `len` tokens, or in one.  Tiles lie one after another, a request's last one
 // first (its rows see most keys).  Every wave of the grid computes its place
 // from the lengths alone.
-template <int BR>
+//
+// Shared keys are dealt so that the workgroups end together, which equal shares do
+// not do (64 requests of 308 .. 16000 keys ended between 29 and 59 us):
+//   - a stretch costs its rows, its first loads and its sums' way out, as much as
+//     `cost` units: in the list every tile has that many more, without keys, ahead
+//     (62 -> 55 us);
+//   - of the HELD workgroups that a CU holds the first is served first.  The grid's
+//     first 256 workgroups are the first ones of their CUs, the next 256 the second
+//     ones: each such layer gets less than the one before it, by `lead` 32nds.
+template <int BR, int HELD>
 struct Kv4List {
   const Kv4AttnArgs& a;
   int len = 0;    // tokens of a unit; 0: all of a tile's
-  int total = 0;  // units, where the keys are shared
+  int cost = 0;   // units that a stretch costs
+  int total = 0;  // units and costs, where the keys are shared
 
   struct Req { int q0, rows, kv, n_new, lo, tiles; };
   __device__ inline Req request(int r) const {
@@ -70,15 +80,16 @@ struct Kv4List {
   }
   // Units of `step` tokens, or as many times that as keep their number in 30 bits
   // (offsets that do not ascend may count rows so often that none does: no work then).
-  __device__ inline void share(const Req& first, int step) {
+  __device__ inline void share(const Req& first, int step, int cost_) {
     const int lane = threadIdx.x & 63;
+    cost = cost_;
     for (len = step;; len *= 2) {
-      float sum = (float)first.tiles * (float)units(first);
-      int n = first.tiles * units(first);
+      float sum = (float)first.tiles * (float)(units(first) + cost);
+      int n = first.tiles * (units(first) + cost);
       for (int base = 64; base < a.R; base += 64) {
         const Req x = request(base + lane);
-        sum += (float)x.tiles * (float)units(x);
-        n += x.tiles * units(x);
+        sum += (float)x.tiles * (float)(units(x) + cost);
+        n += x.tiles * (units(x) + cost);
       }
       total = __builtin_amdgcn_readlane(wave_scan_incl(n), 63);
       if (wave_sum_dpp(sum) < 0x1p30f) return;
@@ -88,24 +99,61 @@ struct Kv4List {
       }
     }
   }
-  // Workgroup j of n gets each = total / n units, the first `more` one more.
-  int each = 0, more = 0;
-  __device__ inline void deal(int n) {
-    each = uniform((int)((unsigned)total / (unsigned)n));
-    more = total - each * n;
+  // Of n workgroups each layer has `size`, the last one the rest; layer l's units
+  // begin at base[l], its first more[l] workgroups have each[l] + 1, the others each[l].
+  // (Below four units a workgroup one layer has all: no workgroup without units lies
+  // between two with some, so that a tile's parts are those of consecutive ones.)
+  int size = 0, base[HELD], each[HELD], more[HELD];
+  __device__ inline void deal(int n, int lead) {
+    constexpr unsigned S = 32 * HELD;
+    const int lane = threadIdx.x & 63;
+    size = total / 4 < n ? 0 : n / HELD;
+    // a lane for a layer: one division for all of them
+    const unsigned whole = (unsigned)total / S, rest = (unsigned)total % S;
+    auto begin = [&](int l) {  // 32nds of an even share, of the layers before l
+      const unsigned upto = l * (32 + lead * (HELD - l));
+      return l < HELD ? (size ? (int)(whole * upto + rest * upto / S) : 0) : total;
+    };
+    const int l = min(lane, HELD - 1), from = begin(l), units = begin(l + 1) - from;
+    const int workers = l + 1 < HELD ? size : n - (HELD - 1) * size;
+    const int quot = (int)((unsigned)units / (unsigned)max(workers, 1)), over = units - quot * workers;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      base[i] = __builtin_amdgcn_readlane(from, i);
+      each[i] = __builtin_amdgcn_readlane(quot, i);
+      more[i] = __builtin_amdgcn_readlane(over, i);
+    }
   }
-  __device__ inline int begin_of(int j) const { return each * j + min(j, more); }
+  __device__ inline int begin_of(int j) const {
+    int u = 0;
+#pragma unroll
+    for (int l = 0; l < HELD; ++l) {
+      const int i = j - l * size;
+      u = l == 0 || i >= 0 ? base[l] + each[l] * i + min(i, more[l]) : u;
+    }
+    return u;
+  }
   __device__ inline int owner_of(int u) const {
-    const int far = more * (each + 1);
-    return uniform(u < far ? (int)((unsigned)u / (unsigned)(each + 1)) : more + (int)((unsigned)(u - far) / (unsigned)max(each, 1)));
+    int at = 0, b = base[0], e = each[0], m = more[0];
+#pragma unroll
+    for (int l = 1; l < HELD; ++l) {
+      const bool in = u >= base[l];
+      at = in ? l * size : at;
+      b = in ? base[l] : b;
+      e = in ? each[l] : e;
+      m = in ? more[l] : m;
+    }
+    const int i = u - b, far = m * (e + 1);
+    return uniform(at + (i < far ? (int)((unsigned)i / (unsigned)(e + 1)) : m + (int)((unsigned)(i - far) / (unsigned)max(e, 1))));
   }
-  // The stretch that starts at unit u, up to unit `to`; false behind the last one.
+  // The stretch that starts at unit u, up to unit `to` (without units where it has
+  // no more than costs); false behind the last one.
   __device__ inline bool find(const Req& first, int u, int to, Kv4Work& w) const {
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int base = 0; base < a.R; base += 64) {
       const Req x = base == 0 ? first : request(base + lane);
-      const int n = units(x);
+      const int n = units(x) + cost;
       const int incl = before + wave_scan_incl(x.tiles * n);
       const uint64_t above = __ballot(incl > u);
       if (above) {
@@ -117,13 +165,14 @@ struct Kv4List {
         w.kv = get(x.kv);
         w.n_new = get(x.n_new);
         w.lo = get(x.lo);
-        w.all = get(n);
-        const int tiles = get(x.tiles), start = get(incl) - tiles * w.all;
-        const int nth = uniform((u - start) / w.all);
+        const int all = get(n), tiles = get(x.tiles), start = get(incl) - tiles * all;
+        const int nth = uniform((u - start) / all);
         w.tile = tiles - 1 - nth;
-        w.first = start + nth * w.all;
-        w.unit = u - w.first;
-        w.units = min(w.all - w.unit, to - u);
+        w.all = all - cost;
+        w.first = start + nth * all + cost;
+        w.span = min(w.first + w.all, to) - u;
+        w.unit = max(u - w.first, 0);
+        w.units = max(u + w.span - w.first, 0) - w.unit;
         return true;
       }
       before = __builtin_amdgcn_readlane(incl, 63);

@@ -125,27 +125,30 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
 
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.y;
+  const int wg = uniform((int)(blockIdx.x / (unsigned)a.dm.n_kv)), kvh = blockIdx.x - wg * a.dm.n_kv;
   const int bs = 1 << a.dm.bs_log2;
-  Kv4List<BR> list{a};
+  Kv4List<BR, attn_held(HD, QT)> list{a};
   const auto mine = list.request(lane);
-  int u = blockIdx.x, u_end = u + 1;
+  int u = wg, u_end = u + 1;
   if (a.wgs > 0) {
-    list.share(mine, 32 * kAttnWaves);
-    list.deal(a.wgs);
-    u = list.begin_of(blockIdx.x);
-    u_end = list.begin_of(blockIdx.x + 1);
+    // (units of cost: 4, 5, 6, 8 on 64 ragged requests 56.2, 56.4, 55.3, 56.3 us; 2, 4, 5, 6
+    // on 16 with drafts, heads of 256, 45.0, 43.0, 44.2, 45.3; leads matter by 1 us)
+    list.share(mine, 32 * kAttnWaves, HD == 256 ? 4 : 6);
+    list.deal(a.wgs, attn_held(HD, QT) == 2 ? 8 : (attn_held(HD, QT) == 3 ? 6 : 4));
+    u = list.begin_of(wg);
+    u_end = list.begin_of(wg + 1);
   }
-  for (Kv4Work w; u < u_end && list.find(mine, u, u_end, w); u += w.units) {
+  for (Kv4Work w; u < u_end && list.find(mine, u, u_end, w); u += w.span) {
+  if (w.units == 0) continue;
   const int row0 = w.tile * BR;  // the first row in the request
   // Partial rows: of a tile's first stretch in 2 wg + 1, of the others in 2 wg.
   const bool whole = w.units == w.all;
   const int64_t part0 =
-      a.part_row0 + ((int64_t)(2 * blockIdx.x + (w.unit == 0)) * a.dm.n_kv + kvh) * BR;
+      a.part_row0 + ((int64_t)(2 * wg + (w.unit == 0)) * a.dm.n_kv + kvh) * BR;
   if (a.meta && kvh == 0 && w.unit == 0 && (int)threadIdx.x < BR) {
     // for the launch that joins the parts: the first one's row and their number
     const int rr = w.tile * BR + (int)threadIdx.x;
-    const int parts = whole ? 1 : list.owner_of(w.first + w.all - 1) - (int)blockIdx.x + 1;
+    const int parts = whole ? 1 : list.owner_of(w.first + w.all - 1) - wg + 1;
     if (rr < w.rows) a.meta[(int64_t)w.q0 * a.group + rr] = int4{(int)part0 + (int)threadIdx.x, parts, a.dm.n_kv * BR, BR};
   }
 
@@ -779,7 +782,7 @@ void launch_attn(const AttnPlan& p, Kv4AttnArgs a, int64_t n_kv, int64_t n_q, hi
     b.rows_upto = p.many ? kAttnFewRows : INT32_MAX;
     b.wgs = p.wgs_few;
     b.part_row0 = 0;
-    const dim3 grid((unsigned)(p.wgs_few ? p.wgs_few : p.tiles_few), (unsigned)n_kv);
+    const dim3 grid((unsigned)((p.wgs_few ? p.wgs_few : p.tiles_few) * n_kv));
     if (p.fold) kv4_attn_kernel<T, HD, 1, true><<<grid, 256, 0, st>>>(b);
     else if (p.qt_few == 1) kv4_attn_kernel<T, HD, 1, false><<<grid, 256, 0, st>>>(b);
     else if constexpr (HD != 256) kv4_attn_kernel<T, HD, 2, false><<<grid, 256, 0, st>>>(b);
@@ -854,7 +857,7 @@ extern "C" int cek_kv4_attention(const void* q, const void* cache, const int32_t
     a.meta = reinterpret_cast<int4*>(a.part_ml + p.part_rows * 2);
     a.part_rows = (int)std::min<int64_t>(p.part_rows, INT32_MAX);
   }
-  if (p.tiles_few > INT32_MAX || p.tiles_many * n_kv > INT32_MAX || p.part_rows > INT32_MAX || T * n_q > INT32_MAX)
+  if (p.tiles_few * n_kv > INT32_MAX || p.tiles_many * n_kv > INT32_MAX || p.part_rows > INT32_MAX || T * n_q > INT32_MAX)
     return CEK_ERR_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
 #define CEK_GO(D)                                                       \

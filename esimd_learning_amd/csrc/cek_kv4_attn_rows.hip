@@ -39,16 +39,17 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
   // heads side by side: the tiles that see most keys first, of all heads
   const int wg = uniform((int)(blockIdx.x / (unsigned)a.dm.n_kv)), kvh = blockIdx.x - wg * a.dm.n_kv;
   const int bs = 1 << a.dm.bs_log2;
-  Kv4List<BR> list{a};
+  Kv4List<BR, 1> list{a};
   const auto mine = list.request(lane);
   int u = wg, u_end = u + 1;
   if (a.wgs > 0) {
-    list.share(mine, 512);
-    list.deal(a.wgs);
+    list.share(mine, 512, 0);  // (costs and leads made it slower: 71 -> 73 .. 78 us)
+    list.deal(a.wgs, 0);
     u = list.begin_of(wg);
     u_end = list.begin_of(wg + 1);
   }
-  for (Kv4Work w; u < u_end && list.find(mine, u, u_end, w); u += w.units) {
+  for (Kv4Work w; u < u_end && list.find(mine, u, u_end, w); u += w.span) {
+  if (w.units == 0) continue;
   const int row0 = w.tile * BR + wave * QT * 16;  // this wave's first row in the request
   // Partial rows: of a tile's first stretch in 2 wg + 1, of the others in 2 wg.
   const bool whole = w.units == w.all;
@@ -148,7 +149,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
       const bool out = outside(x.p);
       p_none = out ? -INFINITY : 0.f;
       pw = *reinterpret_cast<const uint32_t*>(at_block(x.p) + 4 * tok(p_tok) + p_base);
-      pw = out | (t0 + p_tok >= end) ? 0u : pw;
+      pw = (out | (t0 + p_tok >= end)) ? 0u : pw;
     }
   };
   if (begin < end) {
