@@ -9,7 +9,8 @@
 // is read after it was overwritten.  Offsets are prefix sums over the requests.
 //
 // All integer work on a few kilobytes: what it costs is latency, of the launch,
-// two rounds of loads and four barriers.  One workgroup, no larger than the
+// two rounds of loads and four barriers (8 requests 3.5 us, a pass among others 6.0;
+// 256 requests with prompts 8.5 and the second launch 3.9).  One workgroup, no larger than the
 // requests and tokens need, holds up to four requests a thread, scans their
 // counts by DPP, keeps the offsets in LDS and hands the moved blocks and the
 // tokens out evenly, each finding its request by bisection there; a new token's
