@@ -837,7 +837,8 @@ extern "C" int cek_kv4_attention(const void* q, const void* cache, const int32_t
     return CEK_ERR_INVALID;
   if (T == 0 || R == 0) return CEK_OK;
   if (!q || !cache || !block_tables || !kv_lens || !cu_q || !out || !aligned(cache, 16)) return CEK_ERR_INVALID;
-  if (T * (n_q / n_kv) > INT32_MAX / 4) return CEK_ERR_UNSUPPORTED;  // rows of a kv head
+  // rows of a kv head, and requests: their tiles with what each costs stay below 2^30
+  if (T * (n_q / n_kv) > INT32_MAX / 4 || R > 1 << 26) return CEK_ERR_UNSUPPORTED;
   if (workspace_bytes < 0 || (workspace && !aligned(workspace, 16))) return CEK_ERR_INVALID;
   a.q = static_cast<const uint16_t*>(q);
   a.out = static_cast<uint16_t*>(out);

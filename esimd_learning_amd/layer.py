@@ -56,8 +56,8 @@ gives the step that equals the separate ops bit for bit).
 
 With ``kv`` (a layer of a KV4Cache) the new tokens' k and v heads are
 quantised from their columns of qkv into the 4-bit cache and the q heads
-attend to it from theirs: two launches (three where the keys are split over
-workgroups), no copy.  Rows of a step that hold no token (behind cu_q's last)
+attend to it from theirs, without a copy: one launch and one to three (tokens
+alone, prompt chunks beside them, the join of keys shared by workgroups).  Rows of a step that hold no token (behind cu_q's last)
 are padding: nothing is stored for them and their outputs mean nothing.
 
 The intermediate buffers and counters are allocated once in the

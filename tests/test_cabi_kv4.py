@@ -54,6 +54,7 @@ ATTN = dict(q=P, cache=P, tables=P, lens=P, cu=P, out=P, T=4, R=2, n_q=8, n_kv=2
     (dict(mq=-1), INVALID), (dict(mk=-1), INVALID), (dict(window=-1), INVALID), (dict(window=2 ** 31), INVALID),
     (dict(io=7), INVALID), (dict(ws=ODD), INVALID), (dict(ws_bytes=-1), INVALID),
     (dict(T=2 ** 28), UNSUPPORTED),                       # 2^30 rows of a kv head
+    (dict(R=2 ** 26 + 1), UNSUPPORTED),
     (dict(T=0, q=N, out=N), OK), (dict(R=0, lens=N), OK),
 ])
 def test_attention(change, rc):
