@@ -78,6 +78,19 @@ struct Kv4List {
   __device__ inline int units(const Req& x) const {
     return len ? (int)(((unsigned)max(x.kv - x.lo, 1) + (unsigned)len - 1u) / (unsigned)len) : 1;
   }
+  // Tokens of a unit, from `least` to `most`, that give n workgroups four units each.
+  __device__ inline int unit_for(const Req& first, int n, int least, int most) const {
+    const int lane = threadIdx.x & 63;
+    float keys = (float)first.tiles * (float)(first.kv - first.lo);
+    for (int base = 64; base < a.R; base += 64) {
+      const Req x = request(base + lane);
+      keys += (float)x.tiles * (float)(x.kv - x.lo);
+    }
+    keys = wave_sum_dpp(keys);
+    int step = least;
+    while (step < most && keys > 4.f * (float)n * (float)step) step *= 2;
+    return uniform(step);
+  }
   // Units of `step` tokens, or as many times that as keep their number in 30 bits
   // (offsets that do not ascend may count rows so often that none does: no work then).
   __device__ inline void share(const Req& first, int step, int cost_) {

@@ -49,7 +49,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
   const auto mine = list.request(lane);
   int u = wg, u_end = u + 1;
   if (a.wgs > 0) {
-    list.share(mine, 512, 0);  // (costs and leads made it slower: 71 -> 73 .. 78 us)
+    // (costs and leads made a chunk of 1000 on 4000 keys slower: 71 -> 73 .. 78 us)
+    list.share(mine, list.unit_for(mine, a.wgs, 256, 512), 0);
     list.deal(a.wgs, 0);
     u = list.begin_of(wg);
     u_end = list.begin_of(wg + 1);
@@ -393,6 +394,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
     };
     auto idle = [&]() {};
     auto cut = [&]() {
+#pragma unroll 1
       for (int j = 0; j < NG; ++j)
         if (t0 + 32 * j < to && t0 + 32 * j + 32 > from) step(t0 + 32 * j, buf, j, std::true_type{});
     };
