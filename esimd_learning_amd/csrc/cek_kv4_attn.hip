@@ -186,8 +186,6 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
       list.len ? (int)min((int64_t)pmax + 1, (int64_t)w.lo + (int64_t)(w.unit + w.units) * list.len) : pmax + 1);
   constexpr int STEP = 32 * kAttnWaves;
 
-
-
   // ---- q: this lane's 16-bit values of its row of each tile, in the order of K's
   // words; on their way while the codes' addresses are found ----
   uint32_t raw[QT][ND][4];
@@ -244,7 +242,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
       CEK_FETCH(k_lane, to + h * HALF, 16, tok * (HD / 2));
       if constexpr (HD == 256) CEK_FETCH(k_lane, to + h * HALF + 1024, 16, tok * (HD / 2) + 64);
       if constexpr (HD >= 128) CEK_FETCH(v_lane, to + h * HALF + NP * 1024, 16, tok * (HD / 2));
-      if constexpr (HD == 256) CEK_FETCH(v_lane, to + h * HALF + 3072, 16, tok * (HD / 2) + 256);
+      if constexpr (HD == 256) CEK_FETCH(v_lane, to + h * HALF + 3 * 1024, 16, tok * (HD / 2) + 256);
 #undef CEK_FETCH
       par[h] = out ? kv4_zeros : head + at + kv4_k_params(bs, HD) + 4 * tok;
     }
@@ -301,7 +299,6 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     qsum[i] = sum * 0x1p-24f;
     qmul[i] = ldexpf(a.scale * 1.4426950408889634f, 24 - k);
   }
-
 
   f4 o[QT][NP][NH][4];
   f4 wsum[QT];
