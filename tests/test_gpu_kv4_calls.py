@@ -27,6 +27,20 @@ def test_wrong_hints(ops, dev, nq, nk, hd, window, mq, mk):
     b.check(b.run(ops, window=window, mq=mq, mk=mk), window)
 
 
+@pytest.mark.parametrize("nq,nk,hd,chunk", [(8, 2, 64, 1), (4, 4, 128, 1), (8, 2, 64, 40), (2, 1, 256, 33)])
+def test_many_requests(ops, dev, nq, nk, hd, chunk):
+    """More requests than a wave has lanes, most of them short or empty, a few long; some with rows for the other kernel."""
+    _say("requests", nq, nk, hd, chunk)
+    lens = [(7 * i) % 50 for i in range(700)]
+    qlens = [min(n, 1) for n in lens]
+    for i, n in ((3, 2000), (64, 1500), (65, 900), (333, 3000), (699, 700)):
+        lens[i], qlens[i] = n, chunk if i % 2 else 1
+    b = Batch(lens, qlens, nq, nk, hd, 16, torch.bfloat16, dev, seed=chunk)
+    b.check(b.run(ops))
+    b.check(b.run(ops, hints=False))
+    b.check(b.run(ops, window=30), 30)
+
+
 def test_two_streams_at_once(ops, dev):
     """Calls of two batches in flight together, each on its stream, give what they give alone."""
     pair = [Batch([3000, 20, 5000], [1, 40, 2], 16, 4, 128, 32, torch.bfloat16, dev, seed=s) for s in (1, 2)]
