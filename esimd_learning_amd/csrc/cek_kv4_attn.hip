@@ -6,14 +6,15 @@
 // with k = mk + sk (ck - 7.5), v = mv + sv (cv - 7.5) per token and head:
 //
 //   q . k       = sk (q . ck) + (mk - 7.5 sk) sum(q)
-//   sum_j w v   = sum_j (w sv)(cv) - 7.5 sum_j (w sv) + sum_j w mv
+//   sum_j w v   = sum_j (w sv)(cv - 8) + sum_j (w sv) / 2 + sum_j w mv
 //
 // so the matrix products run on the codes themselves and the parameters are
-// applied to scores and weights, one value a token instead of hd.  Codes enter
-// the fp16 MFMA as they lie: a 32-bit word & 0x000F000F is a pair of fp16
+// applied to scores and weights, one value a token instead of hd.  K's codes
+// enter the fp16 MFMA as they lie: a 32-bit word & 0x000F000F is a pair of fp16
 // subnormals c 2^-24, & 0x00F000F0 a pair c 2^-20 -- exact, one AND (and a shift
 // for every second pair) where a conversion would take three operations.  The
-// powers of two are taken back in q (2^-4 for the second kind) and in the sums.
+// powers of two are taken back in q (2^-4 for the second kind) and in the scores.
+// V's take an OR and a packed subtraction more (v_pair).
 //
 // Layout: everything stays in registers.  A wave takes 32 tokens at a time and
 // QT tiles of 16 rows (row = query token x query head of the kv head).  It forms
@@ -26,7 +27,7 @@
 // far, P = exp2(x - M - E + 9) makes P sv at most 2^9 as it comes and 2^15 with
 // the 2^6 that a maximum may lag behind (it moves, and the sums are rescaled,
 // only where a score exceeds it by more): fp16 holds P sv to half a step (2^-12
-// of the value) down to 2^-23 of the largest.  Sums are fp32; 7.5 sum(P sv) is
+// of the value) down to 2^-23 of the largest.  Sums are fp32; sum(P sv) / 2 is
 // taken by an MFMA over the rounded weights, so that a weight's rounding acts
 // on v's distance from its centre alone.
 //
@@ -485,7 +486,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     read_v();
     refill(t0);
     // O^T: values 4 (NH c + h) + b of each part, in rows c
-    const u4 halves = u4{0x47804780u, 0x47804780u, 0x47804780u, 0x47804780u};  // 7.5
+    const u4 halves = u4{0x38003800u, 0x38003800u, 0x38003800u, 0x38003800u};  // 0.5
 #pragma unroll
     for (int i = 0; i < QT; ++i) wsum[i] = mfma16x16x32<F16>(halves, pf[i], wsum[i]);
 #pragma unroll
@@ -494,11 +495,9 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
       for (int h = 0; h < NH; ++h) {
         const int n = (p * NH + h) * 2;
         const uint32_t a0 = vc[0][n], a1 = vc[0][n + 1], b0 = vc[1][n], b1 = vc[1][n + 1];
-        u4 f[4];
-        f[0] = u4{a0 & 0x000F000Fu, a1 & 0x000F000Fu, b0 & 0x000F000Fu, b1 & 0x000F000Fu};
-        f[1] = u4{a0 & 0x00F000F0u, a1 & 0x00F000F0u, b0 & 0x00F000F0u, b1 & 0x00F000F0u};
-        f[2] = u4{(a0 >> 8) & 0x000F000Fu, (a1 >> 8) & 0x000F000Fu, (b0 >> 8) & 0x000F000Fu, (b1 >> 8) & 0x000F000Fu};
-        f[3] = u4{(a0 >> 8) & 0x00F000F0u, (a1 >> 8) & 0x00F000F0u, (b0 >> 8) & 0x00F000F0u, (b1 >> 8) & 0x00F000F0u};
+        const u4 f[4] = {v_operand<0>(a0, a1, b0, b1), v_operand<4>(a0, a1, b0, b1),
+                         v_operand<0>(a0 >> 8, a1 >> 8, b0 >> 8, b1 >> 8),
+                         v_operand<4>(a0 >> 8, a1 >> 8, b0 >> 8, b1 >> 8)};
 #pragma unroll
         for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -537,10 +536,10 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   for (int i = 0; i < QT; ++i) {
     l[i] = over_row(l[i], [](float p, float q) { return p + q; });
     z[i] = over_row(z[i], [](float p, float q) { return p + q; });
-    const float off = z[i] - wsum[i][0];  // every row of the MFMA's result holds 7.5 sum(P sv)
+    const float off = z[i] + wsum[i][0];  // every row of the MFMA's result holds sum(P sv) / 2
     // lane (c, g): values p PW + g PW / 4 + 4 NH e + 4 h + b of row c
     auto value = [&](int p, int e, int h, int b) {
-      return fmaf(o[i][p][h][b][e], b & 1 ? 0x1p20f : 0x1p24f, off);
+      return fmaf(o[i][p][h][b][e], b & 1 ? 0.0625f : 1.0f, off);
     };
     if (i > 0) __syncthreads();
 #pragma unroll

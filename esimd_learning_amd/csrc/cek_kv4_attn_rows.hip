@@ -214,14 +214,13 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
           u4{x & 0x000F000Fu, x & 0x00F000F0u, x8 & 0x000F000Fu, x8 & 0x00F000F0u};
     }
     u4* const to = &v_op[buf][v_grp * NV + (v_part * NH + v_run) * 4][lane];
-    const u4 y = u4{va.x, va.y, vb.x, vb.y};
     if (HD != 64 || (wave & 1) == 0) {
-      to[0] = y & 0x000F000Fu;
-      to[64] = y & 0x00F000F0u;
+      to[0] = v_operand<0>(va.x, va.y, vb.x, vb.y);
+      to[64] = v_operand<4>(va.x, va.y, vb.x, vb.y);
     }
     if (HD != 64 || (wave & 1) == 1) {
-      to[128] = (y >> 8) & 0x000F000Fu;
-      to[192] = (y >> 8) & 0x00F000F0u;
+      to[128] = v_operand<0>(va.x >> 8, va.y >> 8, vb.x >> 8, vb.y >> 8);
+      to[192] = v_operand<4>(va.x >> 8, va.y >> 8, vb.x >> 8, vb.y >> 8);
     }
     if (wave == 0 && lane < ST) {
       const float s = kv4_step(pw) * qmul;
@@ -362,7 +361,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
         pf[i][2 * h] = pack_h2(pv[0], pv[1]);
         pf[i][2 * h + 1] = pack_h2(pv[2], pv[3]);
       }
-    const u4 halves = u4{0x47804780u, 0x47804780u, 0x47804780u, 0x47804780u};  // 7.5
+    const u4 halves = u4{0x38003800u, 0x38003800u, 0x38003800u, 0x38003800u};  // 0.5
 #pragma unroll
     for (int i = 0; i < QT; ++i) wsum[i] = mfma16x16x32<F16>(halves, pf[i], wsum[i]);
 #pragma unroll
@@ -417,10 +416,10 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
   for (int i = 0; i < QT; ++i) {
     l[i] = over_rows(l[i], [](float p, float q) { return p + q; });
     z[i] = over_rows(z[i], [](float p, float q) { return p + q; });
-    const float off = z[i] - wsum[i][0];  // every row of the MFMA's result holds 7.5 sum(P sv)
+    const float off = z[i] + wsum[i][0];  // every row of the MFMA's result holds sum(P sv) / 2
     // lane (c, g): values p PW + g PW / 4 + 4 NH e + 4 h + b of row c
     auto value = [&](int p, int e, int h, int b) {
-      return fmaf(o[i][p][h][b][e], b & 1 ? 0x1p20f : 0x1p24f, off);
+      return fmaf(o[i][p][h][b][e], b & 1 ? 0.0625f : 1.0f, off);
     };
     const int rr = row0 + i * 16 + c;
     if (rr >= w.rows) continue;

@@ -4,6 +4,7 @@ and the tolerance are tests/test_gpu_kv4.py's."""
 import pytest
 import torch
 
+from oracle import kv4
 from test_gpu_kv4 import Batch, _say
 
 pytestmark = pytest.mark.gpu
@@ -39,6 +40,23 @@ def test_many_requests(ops, dev, nq, nk, hd, chunk):
     b.check(b.run(ops))
     b.check(b.run(ops, hints=False))
     b.check(b.run(ops, window=30), 30)
+
+
+@pytest.mark.parametrize("nq,nk,hd,rows", [(2, 2, 128, 1), (4, 2, 64, 1), (2, 1, 256, 1), (8, 2, 128, 20), (8, 1, 64, 20)])
+def test_flat_weights_over_many_keys(ops, dev, nq, nk, hd, rows):
+    """The mean of 40000 values is a two hundredth of each: what sums lose must be small against it, not against them.
+
+    Of the outputs' norm: the output's rounding is at most 2^-11 of a value, uniformly distributed 2^-11 / sqrt(3); the
+    weights' rounding the same, independently for each key, on values whose sum is what the output is made of: the
+    root of both squares is 2^-11 sqrt(2 / 3) = 0.0004.  Half as much again is left for the sample."""
+    _say("flat", nq, nk, hd, rows)
+    b = Batch([40000], [rows], nq, nk, hd, 64, torch.float16, dev, seed=hd + rows)
+    b.q = b.q * 0.01
+    b.qd = b.q.to(dev)
+    ref = kv4.attention(b.q, b.keys[0], b.vals[0], b.scale)
+    for hints in (dict(mq=rows, mk=1), dict(mq=rows, mk=40000), dict(mq=0, mk=0)):
+        err = b.run(ops, **hints).cpu().double() - ref
+        assert float(err.norm() / ref.norm()) <= 6e-4, hints
 
 
 def test_two_streams_at_once(ops, dev):
