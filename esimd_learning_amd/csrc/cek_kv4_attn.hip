@@ -32,10 +32,10 @@
 // on v's distance from its centre alone.
 //
 // What bounds it: the codes' bytes from HBM, and for short keys the latency of one
-// launch.  64 requests of 308 .. 16000 keys, 32 / 8 heads of 128, bf16: 55.2 us for
-// 288 MB (5.2 TB/s; a kernel that only reads them 40); one of 131071 keys 32.1 us
+// launch.  64 requests of 308 .. 16000 keys, 32 / 8 heads of 128, bf16: 56.4 us for
+// 288 MB (5.1 TB/s; a kernel that only reads them 40); one of 131071 keys 32.9 us
 // (143 MB; 20); 16 of 5 drafts on up to 6000 keys, window 4096, 16 heads of 256,
-// fp16: 42.6 us (174 MB; 24); one of 700 keys 9.5 us, of which 5 in the six tiles
+// fp16: 43.6 us (174 MB; 24); one of 700 keys 10.2 us, of which 5 in the six tiles
 // that each wave takes one after another.  What lies between: launch, work list,
 // table and first tiles before the loop, 5 us; the join's launch, 5; and workgroups
 // that end up to 10 us before the last one.

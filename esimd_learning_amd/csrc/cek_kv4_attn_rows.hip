@@ -12,8 +12,8 @@
 // stage.  Two workgroups a CU: while one's waves are in the products the other's
 // may be in the softmax.
 //
-// Four chunks of 1900 tokens on 1900 .. 4100 keys, 32 / 8 heads of 128, fp16: 385 us,
-// 690 TFLOP/s.  Of a SIMD's cycles the matrix cores are busy 30%, vector instructions
+// Four chunks of 1900 tokens on 1900 .. 4100 keys, 32 / 8 heads of 128, fp16: 394 us,
+// 673 TFLOP/s.  Of a SIMD's cycles the matrix cores are busy 30%, vector instructions
 // 43% and exponentials 11%, and hardly at the same time: 84% together.  No gain came
 // from priorities for the products, from products and softmax of different rows
 // interleaved, from fewer maxima, nor from the next product's operands read ahead.
