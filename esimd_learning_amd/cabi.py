@@ -57,6 +57,8 @@ SIGNATURES = {
                                           _i64, _f, _i64, _i64, _i64, _i, _i, _i, _p]),
     "cek_kv_block_tables": (_i, [_p, _p, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p,
                                  _p]),
+    "cek_kv_block_tables_fixed_rows": (_i, [_p, _p, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _p, _p,
+                                            _i64, _p, _p]),
     "cek_kv4_cache_write": (_i, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _p]),
     "cek_kv4_cache_read": (_i, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _p]),
     "cek_kv4_attention_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),

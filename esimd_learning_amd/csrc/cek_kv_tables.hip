@@ -16,7 +16,9 @@
 // tokens out evenly, each finding its request by bisection there; a new token's
 // block comes from the ring itself, so that nothing waits for the tables that are
 // being written.  Above kTablesOneLaunch tokens a second launch fills the slots.
-// kv_lens_out and ring_state_out are written behind the barrier that follows the
+// With fixed_rows a request's rows lie where the wishes (q) of those before it put
+// them, granted or not: cu_q follows the wishes, and rows that were not granted have
+// no slot.  kv_lens_out and ring_state_out are written behind the barrier that follows the
 // last read of kv_lens and ring_state, so that they may be the same memory.
 #include <algorithm>
 
@@ -34,6 +36,7 @@ struct KvTablesArgs {
   int64_t *slots, *positions;
   int64_t table_stride, T;
   int R, cap, width, bs_log2;
+  int fixed_rows;
 };
 
 __device__ inline int64_t wave_scan_incl(int64_t x) {
@@ -82,7 +85,7 @@ template <typename I>
 __global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(KvTablesArgs a, int fill_slots) {
   constexpr int N = kTablesMaxRequests;
   __shared__ I sh2[kTablesThreads / 64][2], sh3[kTablesThreads / 64][3];
-  // offsets of the requests' new tokens, taken and returned blocks; kept tokens, blocks held and wanted
+  // offsets of the requests' new tokens, taken and returned blocks; kept tokens (-1: refused), blocks held and wanted
   __shared__ int32_t at_q[N + 1], at_need[N + 1], at_gone[N + 1], keep_s[N], have_s[N], want_s[N];
   const int tid = threadIdx.x, nt = blockDim.x;
   const int per = (a.R + nt - 1) / nt;  // requests per thread, consecutive
@@ -100,6 +103,7 @@ __global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(KvTablesArgs 
   };
 
   int64_t q[4];
+  I rows_of[4];  // rows that the request's new tokens take
   int len[4], keep[4], have[4], need[4], st[4];
   I sum[2] = {0, 0}, total2[2];
 #pragma unroll
@@ -107,16 +111,18 @@ __global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(KvTablesArgs 
     const int r = tid * per + j;
     len[j] = keep[j] = have[j] = need[j] = st[j] = 0;
     q[j] = 0;
+    rows_of[j] = 0;
     if (j < per && r < a.R) {
       len[j] = (int)min((int64_t)max(a.kv_lens[r], 0), reach);
       keep[j] = min(max(a.keep_lens[r], 0), len[j]);
       q[j] = max(a.q_lens[r], 0);
-      if (keep[j] + q[j] > reach) st[j] = 2, q[j] = 0;
+      rows_of[j] = (I)min(q[j], a.T + 1);
+      if (keep[j] + q[j] > reach) st[j] = 2, q[j] = 0, rows_of[j] = a.fixed_rows ? rows_of[j] : 0;
       have[j] = (len[j] + bs - 1) >> a.bs_log2;
       need[j] = max((int)((keep[j] + q[j] + bs - 1) >> a.bs_log2) - have[j], 0);
       // (counts beyond what there is are as good as one more than that)
       sum[0] += (I)min(need[j], a.cap + 1);
-      sum[1] += (I)min(q[j], a.T + 1);
+      sum[1] += rows_of[j];
     }
   }
   const I own[2] = {sum[0], sum[1]};
@@ -129,13 +135,13 @@ __global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(KvTablesArgs 
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     sum[0] += (I)min(need[j], a.cap + 1);
-    sum[1] += (I)min(q[j], a.T + 1);
+    sum[1] += rows_of[j];
     if (st[j] == 0) st[j] = need[j] > 0 && sum[0] > (I)count ? 1 : (q[j] > 0 && sum[1] > (I)a.T ? 3 : 0);
-    if (st[j]) need[j] = 0, q[j] = 0;
+    if (st[j]) need[j] = 0, q[j] = 0, rows_of[j] = a.fixed_rows ? rows_of[j] : 0;
     want[j] = (int)((keep[j] + q[j] + bs - 1) >> a.bs_log2);
     gone[j] = min(max(have[j] - want[j], 0), a.cap + 1);
     at[0] += (I)need[j];
-    at[1] += (I)q[j];
+    at[1] += rows_of[j];
     at[2] += (I)gone[j];
   }
   const I mine[3] = {at[0], at[1], at[2]};
@@ -147,19 +153,19 @@ __global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(KvTablesArgs 
     const int r = tid * per + j;
     if (j < per && r < a.R) {
       at_need[r] = (int)at[0];
-      a.cu_q[r] = at_q[r] = (int)at[1];
+      a.cu_q[r] = at_q[r] = (int)min(at[1], (I)a.T);
       at_gone[r] = (int)at[2];
-      keep_s[r] = keep[j];
+      keep_s[r] = st[j] ? -1 : keep[j];
       have_s[r] = have[j];
       want_s[r] = want[j];
       a.kv_lens_out[r] = keep[j] + (int)q[j];
       a.status[r] = st[j];
     }
     at[0] += (I)need[j];
-    at[1] += (I)q[j];
+    at[1] += rows_of[j];
     at[2] += (I)gone[j];
   }
-  const int taken = (int)total[0], rows = (int)total[1];
+  const int taken = (int)total[0], rows = (int)min(total[1], (I)a.T);
   // (lengths of more blocks than there are return no more than the ring has room for
   // beside all that was free: no place is read and written)
   const int given = (int)min((int64_t)total[2], (int64_t)a.cap - count);
@@ -186,11 +192,13 @@ __global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(KvTablesArgs 
     int64_t pos = 0, slot = -1;
     if (t < rows) {
       const int r = find_in(at_q, a.R, t);
-      pos = keep_s[r] + t - at_q[r];
-      const int i = (int)(pos >> a.bs_log2);
-      const int32_t blk = i < have_s[r] ? a.tables[(int64_t)r * a.table_stride + i]
-                                        : a.ring[place((int64_t)at_need[r] + i - have_s[r])];
-      slot = blk < 0 ? -1 : ((int64_t)blk << a.bs_log2) + (pos & (bs - 1));
+      if (keep_s[r] >= 0) {
+        pos = keep_s[r] + t - at_q[r];
+        const int i = (int)(pos >> a.bs_log2);
+        const int32_t blk = i < have_s[r] ? a.tables[(int64_t)r * a.table_stride + i]
+                                          : a.ring[place((int64_t)at_need[r] + i - have_s[r])];
+        slot = blk < 0 ? -1 : ((int64_t)blk << a.bs_log2) + (pos & (bs - 1));
+      }
     }
     a.slots[t] = slot;
     a.positions[t] = pos;
@@ -208,9 +216,11 @@ __global__ __launch_bounds__(256) void kv_slots_kernel(KvTablesArgs a) {
   int64_t pos = 0, slot = -1;
   if (t < at_q[a.R]) {
     const int r = find_in(at_q, a.R, (int)t);
-    pos = (int64_t)a.kv_lens_out[r] - at_q[r + 1] + t;
-    const int32_t blk = a.tables[(int64_t)r * a.table_stride + (pos >> a.bs_log2)];
-    slot = blk < 0 ? -1 : ((int64_t)blk << a.bs_log2) + (pos & ((1 << a.bs_log2) - 1));
+    if (a.status[r] == 0) {
+      pos = (int64_t)a.kv_lens_out[r] - at_q[r + 1] + t;
+      const int32_t blk = a.tables[(int64_t)r * a.table_stride + (pos >> a.bs_log2)];
+      slot = blk < 0 ? -1 : ((int64_t)blk << a.bs_log2) + (pos & ((1 << a.bs_log2) - 1));
+    }
   }
   a.slots[t] = slot;
   a.positions[t] = pos;
@@ -220,11 +230,11 @@ __global__ __launch_bounds__(256) void kv_slots_kernel(KvTablesArgs a) {
 
 using namespace cek;
 
-extern "C" int cek_kv_block_tables(const int32_t* kv_lens, const int32_t* keep_lens, const int32_t* q_lens, int64_t R,
-                                   int64_t block_size, int32_t* free_ring, int64_t num_blocks, const int32_t* ring_state,
-                                   int32_t* block_tables, int64_t table_stride, int64_t max_blocks,
-                                   int32_t* kv_lens_out, int32_t* ring_state_out, int32_t* cu_q, int64_t* slot_mapping,
-                                   int64_t* positions, int64_t T, int32_t* status, void* stream) {
+static int block_tables_call(const int32_t* kv_lens, const int32_t* keep_lens, const int32_t* q_lens, int64_t R,
+                             int64_t block_size, int32_t* free_ring, int64_t num_blocks, const int32_t* ring_state,
+                             int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* kv_lens_out,
+                             int32_t* ring_state_out, int32_t* cu_q, int64_t* slot_mapping, int64_t* positions,
+                             int64_t T, int32_t* status, int fixed_rows, void* stream) {
   if (R < 0 || T < 0 || T > INT32_MAX || num_blocks <= 0 || num_blocks > INT32_MAX || max_blocks <= 0 ||
       table_stride < max_blocks)
     return CEK_ERR_INVALID;
@@ -235,7 +245,7 @@ extern "C" int cek_kv_block_tables(const int32_t* kv_lens, const int32_t* keep_l
     return CEK_ERR_INVALID;
   const KvTablesArgs a{kv_lens, keep_lens, q_lens, ring_state, free_ring, block_tables, kv_lens_out, ring_state_out, cu_q,
                        status, slot_mapping, positions, table_stride, T, (int)R, (int)num_blocks, (int)max_blocks,
-                       __builtin_ctzll((unsigned long long)block_size)};
+                       __builtin_ctzll((unsigned long long)block_size), fixed_rows};
   hipStream_t st = (hipStream_t)stream;
   const int one = T <= kTablesOneLaunch;
   // a thread for each request and, where they are few, for each token
@@ -247,4 +257,25 @@ extern "C" int cek_kv_block_tables(const int32_t* kv_lens, const int32_t* keep_l
   if (rc != CEK_OK || one) return rc;
   kv_slots_kernel<<<(unsigned)((T + 255) / 256), 256, 0, st>>>(a);
   return check_launch();
+}
+
+extern "C" int cek_kv_block_tables(const int32_t* kv_lens, const int32_t* keep_lens, const int32_t* q_lens, int64_t R,
+                                   int64_t block_size, int32_t* free_ring, int64_t num_blocks, const int32_t* ring_state,
+                                   int32_t* block_tables, int64_t table_stride, int64_t max_blocks,
+                                   int32_t* kv_lens_out, int32_t* ring_state_out, int32_t* cu_q, int64_t* slot_mapping,
+                                   int64_t* positions, int64_t T, int32_t* status, void* stream) {
+  return block_tables_call(kv_lens, keep_lens, q_lens, R, block_size, free_ring, num_blocks, ring_state, block_tables,
+                           table_stride, max_blocks, kv_lens_out, ring_state_out, cu_q, slot_mapping, positions, T,
+                           status, 0, stream);
+}
+
+extern "C" int cek_kv_block_tables_fixed_rows(const int32_t* kv_lens, const int32_t* keep_lens, const int32_t* q_lens,
+                                              int64_t R, int64_t block_size, int32_t* free_ring, int64_t num_blocks,
+                                              const int32_t* ring_state, int32_t* block_tables, int64_t table_stride,
+                                              int64_t max_blocks, int32_t* kv_lens_out, int32_t* ring_state_out,
+                                              int32_t* cu_q, int64_t* slot_mapping, int64_t* positions, int64_t T,
+                                              int32_t* status, void* stream) {
+  return block_tables_call(kv_lens, keep_lens, q_lens, R, block_size, free_ring, num_blocks, ring_state, block_tables,
+                           table_stride, max_blocks, kv_lens_out, ring_state_out, cu_q, slot_mapping, positions, T,
+                           status, 1, stream);
 }

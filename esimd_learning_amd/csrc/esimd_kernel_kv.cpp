@@ -101,7 +101,7 @@ int64_t check_tables(const at::Tensor& t, const at::Tensor& ref, int64_t R, cons
 void esimd_kv_block_tables(at::Tensor kv_lens, at::Tensor keep_lens, at::Tensor q_lens, int64_t block_size,
                            at::Tensor free_ring, at::Tensor ring_state, at::Tensor block_tables, at::Tensor kv_lens_out,
                            at::Tensor ring_state_out, at::Tensor cu_q, at::Tensor slot_mapping, at::Tensor positions,
-                           at::Tensor status) {
+                           at::Tensor status, bool fixed_rows) {
   const char* op = "esimd_kv_block_tables";
   const auto i32 = at::ScalarType::Int, i64 = at::ScalarType::Long;
   TORCH_CHECK(kv_lens.dim() == 1, op, ": kv_lens must be int32, one-dimensional");
@@ -144,10 +144,11 @@ void esimd_kv_block_tables(at::Tensor kv_lens, at::Tensor keep_lens, at::Tensor 
   }
   c10::OptionalDeviceGuard guard(kv_lens.device());
   const auto p = [](const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
-  check_rc(cek_kv_block_tables(p(kv_lens), p(keep_lens), p(q_lens), R, block_size, p(free_ring), free_ring.numel(),
-                               p(ring_state), p(block_tables), stride, block_tables.size(1), p(kv_lens_out),
-                               p(ring_state_out), p(cu_q), static_cast<int64_t*>(slot_mapping.data_ptr()),
-                               static_cast<int64_t*>(positions.data_ptr()), T, p(status), current_stream(kv_lens)),
+  const auto call = fixed_rows ? cek_kv_block_tables_fixed_rows : cek_kv_block_tables;
+  check_rc(call(p(kv_lens), p(keep_lens), p(q_lens), R, block_size, p(free_ring), free_ring.numel(), p(ring_state),
+                p(block_tables), stride, block_tables.size(1), p(kv_lens_out), p(ring_state_out), p(cu_q),
+                static_cast<int64_t*>(slot_mapping.data_ptr()), static_cast<int64_t*>(positions.data_ptr()), T,
+                p(status), current_stream(kv_lens)),
            op);
 }
 

@@ -85,7 +85,7 @@ TORCH_LIBRARY(custom_esimd_kernels_vllm, m) {
   m.def("esimd_kv_block_tables(Tensor(a!) kv_lens, Tensor keep_lens, Tensor q_lens, int block_size, "
         "Tensor(b!) free_ring, Tensor(c!) ring_state, Tensor(d!) block_tables, Tensor(a!) kv_lens_out, "
         "Tensor(c!) ring_state_out, Tensor(e!) cu_q, Tensor(f!) slot_mapping, Tensor(g!) positions, "
-        "Tensor(h!) status) -> ()");
+        "Tensor(h!) status, bool fixed_rows=False) -> ()");
   m.impl("esimd_kv_block_tables", c10::DispatchKey::CUDA, &esimd_kv_block_tables);
 
   m.def("esimd_kv4_cache_write(Tensor k, Tensor v, Tensor(a!) kv_cache, Tensor slot_mapping) -> ()");

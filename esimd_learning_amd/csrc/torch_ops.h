@@ -81,7 +81,7 @@ void esimd_gemv_fp8_qk_norm_rope_rs(at::Tensor input, at::Tensor weight, at::Ten
 void esimd_kv_block_tables(at::Tensor kv_lens, at::Tensor keep_lens, at::Tensor q_lens, int64_t block_size,
                            at::Tensor free_ring, at::Tensor ring_state, at::Tensor block_tables, at::Tensor kv_lens_out,
                            at::Tensor ring_state_out, at::Tensor cu_q, at::Tensor slot_mapping, at::Tensor positions,
-                           at::Tensor status);
+                           at::Tensor status, bool fixed_rows);
 void esimd_kv4_cache_write(at::Tensor k, at::Tensor v, at::Tensor kv_cache, at::Tensor slot_mapping);
 void esimd_kv4_cache_read(at::Tensor kv_cache, at::Tensor slot_mapping, at::Tensor k, at::Tensor v);
 void esimd_kv4_attention(at::Tensor q, at::Tensor kv_cache, at::Tensor block_tables, at::Tensor kv_lens, at::Tensor cu_q,

@@ -3,7 +3,8 @@
     kv = KV4Cache(layers, num_blocks, n_kv, head_dim, requests, tokens, max_len)
     each step:
       kv.advance(q_lens)                    esimd_kv_block_tables: room, slots and
-                                            positions of the step's new tokens
+                                            positions of the step's new tokens, by
+                                            rows as cu_q says
       per layer i: kv.layers[i].attend(q, k, v, out)
                                             esimd_kv4_cache_write, then
                                             esimd_kv4_attention over old and new
@@ -35,7 +36,8 @@ class KV4Layer:
         """Store the step's k and v rows; out = causal attention of q over the cache.
 
         Rows behind the step's last token are padding: not stored, and left as
-        they were in out."""
+        they were in out.  So are a refused request's rows where they stay
+        (``fixed_rows`` of advance), but for out, which holds nothing of use."""
         o = self.owner
         self.write(k, v)
         o.ops.esimd_kv4_attention(q, self.cache, o.block_tables, o.lens, o.cu_q, out,
@@ -72,10 +74,16 @@ class KV4Cache:
         self.positions = torch.zeros(tokens, dtype=torch.int64, device=device)
         self.max_q_len = self.max_kv_len = 0
 
-    def advance(self, q_lens, keep_lens=None, max_q_len=0, max_kv_len=0):
+    def advance(self, q_lens, keep_lens=None, max_q_len=0, max_kv_len=0, fixed_rows=False):
         """Begin a step: q_lens [requests] int32 new tokens of each request, whose
         rows stand one request after another; positions, slots, tables and lens
         follow.
+
+        A request that gets no room has no token in the step.  Its rows are closed
+        up: request r's are cu_q[r] .. cu_q[r + 1] - 1, known after the call.  With
+        ``fixed_rows`` they stay, as padding, and everyone's rows are where q_lens
+        puts them: for a caller that lays out its rows without reading status or
+        cu_q back, as around a captured step.
 
         keep_lens [requests] int32: how many of its cached tokens each request
         keeps (None, or beyond its length: all) -- fewer after rejected drafts, 0
@@ -85,7 +93,8 @@ class KV4Cache:
         attention choose its kernels without looking; wrong ones cost only time."""
         self.ops.esimd_kv_block_tables(self.lens, self.keep_all if keep_lens is None else keep_lens, q_lens,
                                        self.block_size, self.free_ring, self.ring_state, self.block_tables, self.lens,
-                                       self.ring_state, self.cu_q, self.slot_mapping, self.positions, self.status)
+                                       self.ring_state, self.cu_q, self.slot_mapping, self.positions, self.status,
+                                       fixed_rows)
         self.max_q_len, self.max_kv_len = max_q_len, max_kv_len
 
     def slots(self, request, start, count):

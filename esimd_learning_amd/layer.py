@@ -57,7 +57,8 @@ gives the step that equals the separate ops bit for bit).
 With ``kv`` (a layer of a KV4Cache) the new tokens' k and v heads are
 quantised from their columns of qkv into the 4-bit cache and the q heads
 attend to it from theirs, without a copy: one launch and one to three (tokens
-alone, prompt chunks beside them, the join of keys shared by workgroups).  Rows of a step that hold no token (behind cu_q's last)
+alone, prompt chunks beside them, the join of keys shared by workgroups).  Rows of a step that hold no token (behind cu_q's last, or of a
+request that got no room, where its rows stay)
 are padding: nothing is stored for them and their outputs mean nothing.
 
 The intermediate buffers and counters are allocated once in the
@@ -275,7 +276,8 @@ def forward(layers, hidden, residual, positions, kv=None):
     last layer's is the plain one).
 
     kv: a KV4Cache with a layer for each of `layers` and M tokens a step, after
-    its advance(); positions are then its positions."""
+    its advance(); positions are then its positions, and the rows of hidden and
+    residual lie as its cu_q says."""
     if kv is not None and (len(kv.layers) != len(layers) or any(x.M != kv.tokens for x in layers)):
         raise ValueError("kv must have a layer for each layer and as many tokens a step as they have rows")
     h, ss = hidden, None
@@ -298,15 +300,17 @@ def capture_forward(layers, hidden, residual, positions, stream=None, kv=None, q
     captures a model's whole decode step (no launch gap between layers).
 
     With ``kv`` and ``q_lens`` the graph begins with kv.advance(q_lens, keep_lens,
-    max_q_len, max_kv_len) on these buffers, so that every replay is the next step:
-    the caller writes the tokens' hidden states (and, where they change, q_lens and
-    keep_lens) between replays.  Without ``q_lens`` the caller advances kv itself."""
+    max_q_len, max_kv_len, fixed_rows=True) on these buffers, so that every replay is
+    the next step: the caller writes the tokens' hidden states (and, where they change,
+    q_lens and keep_lens) between replays, each request's rows behind those that q_lens
+    gives the ones before it.  A request that gets no room (kv.status, after the replay)
+    shifts no one's rows: its own are padding.  Without ``q_lens`` the caller advances kv itself."""
     s = stream or torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g, stream=s):
         if kv is not None and q_lens is not None:
-            kv.advance(q_lens, keep_lens, max_q_len, max_kv_len)
+            kv.advance(q_lens, keep_lens, max_q_len, max_kv_len, fixed_rows=True)
         forward(layers, hidden, residual, positions, kv)
     torch.cuda.current_stream().wait_stream(s)
     return g

@@ -258,7 +258,7 @@ def esimd_kv_block_tables(
     kv_lens: torch.Tensor, keep_lens: torch.Tensor, q_lens: torch.Tensor, block_size: int,
     free_ring: torch.Tensor, ring_state: torch.Tensor, block_tables: torch.Tensor,
     kv_lens_out: torch.Tensor, ring_state_out: torch.Tensor, cu_q: torch.Tensor,
-    slot_mapping: torch.Tensor, positions: torch.Tensor, status: torch.Tensor,
+    slot_mapping: torch.Tensor, positions: torch.Tensor, status: torch.Tensor, fixed_rows: bool = False,
 ) -> None:
     """Block tables, slots and positions of one step, from the lengths alone.
 
@@ -282,13 +282,21 @@ def esimd_kv_block_tables(
     wishes of all requests before, refused ones too; a request that needs no
     new block is never refused for one.
 
+    A refused request closes up the rows: those behind it begin where cu_q says,
+    earlier than q_lens alone would put them, so that a caller lays out its rows
+    by cu_q, or sees from status that nobody was refused.  With ``fixed_rows``
+    the rows do not depend on who was refused (a captured step, whose rows are
+    laid out before it runs): cu_q are the offsets of q_lens (negative ones as 0,
+    no further than T), and a refused request's rows are padding, slot -1 and
+    position 0.  Status 3 then counts the wishes of requests with status 2 too.
+
     kv_lens_out may be kv_lens and ring_state_out ring_state (a captured step
     replayed); no other output may share memory with another argument.  A block
     is free or one request's: what several requests read is not shared here.
     Lengths are taken within 0 .. the table's reach, keep_lens within 0 ..
     kv_lens (2^31 - 1 keeps all).  At most 4096 requests."""
     _ops.esimd_kv_block_tables(kv_lens, keep_lens, q_lens, block_size, free_ring, ring_state, block_tables, kv_lens_out,
-                               ring_state_out, cu_q, slot_mapping, positions, status)
+                               ring_state_out, cu_q, slot_mapping, positions, status, fixed_rows)
 
 
 def esimd_kv4_cache_write(

@@ -393,6 +393,11 @@ int cek_qk_norm_rope(void* q, void* k, const void* qw, const void* kw, const int
  * kv_lens_out may be kv_lens and ring_state_out ring_state; no other output may
  * overlap an argument.  A block is free or one request's.  keep_lens beyond kv_lens
  * keep all.  R <= 4096.
+ * cek_kv_block_tables_fixed_rows: the same, but that a refused request's tokens keep
+ * their rows (slot -1, position 0): cu_q are the offsets of q_lens, negative ones
+ * taken as 0, no further than T, whatever was granted.  Status 3 then counts the
+ * tokens of requests with status 2 too.  For callers that lay out the step's rows
+ * without having seen status.
  *
  * cek_kv4_cache_write: k, v rows (strides in elements) quantised into the cache,
  * m = bf16((min + max) / 2), s = bf16(max(max - m, m - min) / 7.5), c =
@@ -415,6 +420,11 @@ int cek_kv_block_tables(const int32_t* kv_lens, const int32_t* keep_lens, const 
                         int32_t* block_tables, int64_t table_stride, int64_t max_blocks, int32_t* kv_lens_out,
                         int32_t* ring_state_out, int32_t* cu_q, int64_t* slot_mapping, int64_t* positions, int64_t T,
                         int32_t* status, void* stream);
+int cek_kv_block_tables_fixed_rows(const int32_t* kv_lens, const int32_t* keep_lens, const int32_t* q_lens, int64_t R,
+                                   int64_t block_size, int32_t* free_ring, int64_t num_blocks,
+                                   const int32_t* ring_state, int32_t* block_tables, int64_t table_stride,
+                                   int64_t max_blocks, int32_t* kv_lens_out, int32_t* ring_state_out, int32_t* cu_q,
+                                   int64_t* slot_mapping, int64_t* positions, int64_t T, int32_t* status, void* stream);
 int cek_kv4_cache_write(const void* k, const void* v, void* cache, const int64_t* slot_mapping, int64_t T, int64_t n_kv,
                         int64_t head_dim, int64_t block_size, int64_t num_blocks, int64_t k_stride, int64_t v_stride,
                         int64_t block_stride, int io_dtype, void* stream);

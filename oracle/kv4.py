@@ -92,9 +92,9 @@ def attention(q, keys, vals, scale, window=0, weigh=()):
     return (outs[0], outs[1:]) if weigh else outs[0]
 
 
-def block_tables(kv_lens, keep_lens, q_lens, bs, ring, state, tables, T):
+def block_tables(kv_lens, keep_lens, q_lens, bs, ring, state, tables, T, fixed_rows=False):
     """One step on Python lists; tables is a list of rows, changed like ring in place.  Returns (kv_lens_out,
-    ring_state_out, cu_q, slots, positions, status)."""
+    ring_state_out, cu_q, slots, positions, status).  fixed_rows: refused requests keep their rows, as padding."""
     cap, width = len(ring), len(tables[0]) if tables else 0
     head, count = state
     taken = given = wish = rows = 0
@@ -103,9 +103,10 @@ def block_tables(kv_lens, keep_lens, q_lens, bs, ring, state, tables, T):
     for r, (n, keep, q) in enumerate(zip(kv_lens, keep_lens, q_lens)):
         n = min(max(n, 0), width * bs)
         keep, q = min(max(keep, 0), n), max(q, 0)
-        have, want, st = -(-n // bs), -(-(keep + q) // bs), 0
+        have, want, st, wished = -(-n // bs), -(-(keep + q) // bs), 0, q
         if want > width:
             st = 2
+            rows += q if fixed_rows else 0
         else:
             need = max(0, want - have)
             wish += need
@@ -125,7 +126,10 @@ def block_tables(kv_lens, keep_lens, q_lens, bs, ring, state, tables, T):
         for p in range(keep, keep + q):
             pos.append(p)
             slots.append(tables[r][p // bs] * bs + p % bs)
-        cu.append(cu[-1] + q)
+        end = min(cu[-1] + wished, T) if fixed_rows else cu[-1] + q
+        pos += [0] * (end - len(pos))
+        slots += [-1] * (end - len(slots))
+        cu.append(end)
         lens.append(keep + q)
         status.append(st)
     slots += [-1] * (T - len(slots))
