@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   f4 wsum[QT];
   float l[QT], z[QT], m[QT], ref[QT];
   int ev = -80;
-  float sv_top = -1.f;  // 2^ev, or -1 before the first tokens
+  float sv_top = 0x1p-80f;  // 2^ev
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     l[i] = z[i] = 0.f;
@@ -420,16 +420,19 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     return over_rows(v, op);
   };
   // New references, and the sums so far brought to them.
-  auto rescale = [&]() {
+  auto rescale = [&](auto mask) {
+    constexpr bool masked = decltype(mask)::value;
     top = over_row(top, [](float p, float q) { return fmaxf(p, q); });
+    const int was = ev;
     ev = max(ev, (int)((__float_as_uint(fmaxf(top, 0.f)) >> 23) & 255) - 126);
     sv_top = __uint_as_float((uint32_t)(ev + 127) << 23);
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-      float t = fmaxf(m[i], xm[i] * qmul[i]);
-      t = over_row(t, [](float p, float q) { return fmaxf(p, q); });
-      m[i] = t;
-      const float nr = t + (float)(ev - kAttnBase);
+      const float t = over_row(xm[i], [](float p, float q) { return fmaxf(p, q); }) * qmul[i];
+      // a row moves for what it has seen itself, whatever the others saw
+      const bool move = masked | (ev > was) | (t > m[i] + (float)kAttnHead);
+      m[i] = move ? fmaxf(m[i], t) : m[i];
+      const float nr = move ? m[i] + (float)(ev - kAttnBase) : ref[i];
       const float f = __builtin_amdgcn_exp2f(ref[i] - nr);
       ref[i] = nr;
       l[i] *= f;
@@ -515,7 +518,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
       for (; t0 < to; t0 += STEP) {
         read_k();
         scores(t0, std::true_type{});
-        rescale();
+        rescale(std::true_type{});
         accumulate(t0, std::true_type{});
       }
     };
@@ -523,7 +526,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     for (; t0 <= full; t0 += STEP) {
       read_k();
       scores(t0, std::false_type{});
-      if (grows()) rescale();
+      if (grows()) rescale(std::false_type{});
       accumulate(t0, std::false_type{});
     }
     cut_to(end);

@@ -38,7 +38,6 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
   __shared__ u4 k_op[2][NS * ND][64], v_op[2][NG * NV][64];
   __shared__ float par[2][4][ST];  // K step and offset, V step and centre, of a stage's tokens
   __shared__ float gone[2][NS];    // -infinity for 16 tokens in no block
-  __shared__ float wave_top[kAttnWaves];
 
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -165,28 +164,25 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
     nb = blocks_of(min(begin + ST, last));
   }
 
-  // ---- q as MFMA operands: all rows of the tile times one power of two ----
+  // ---- q as MFMA operands: each row times its own power of two, so that what
+  // other rows hold (an infinity, values far larger) leaves it as it is ----
+  __syncthreads();  // (of the stretch before, nothing is read any more)
   u4 qf[QT][ND];
-  float qsum[QT], top_q = 0.f;
+  float qsum[QT], qmul[QT];
 #pragma unroll
-  for (int i = 0; i < QT; ++i)
+  for (int i = 0; i < QT; ++i) {
+    float top_q = 0.f;
 #pragma unroll
     for (int n = 0; n < 4 * ND; ++n) {
       if (!real[i]) raw[i][n / 4][n % 4] = 0;
       const uint32_t x = raw[i][n / 4][n % 4];
       top_q = fmaxf(top_q, fmaxf(fabsf(T::to_f32(x & 0xFFFF)), fabsf(T::to_f32(x >> 16))));
     }
-  top_q = wave_max(top_q);
-  __syncthreads();  // (of the stretch before, nothing is read any more)
-  if (lane == 0) wave_top[wave] = top_q;
-  __syncthreads();
-  top_q = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
-  int k2 = 0;
-  if (top_q > 0.f) k2 = min(120, 140 - (int)((__float_as_uint(top_q) >> 23) & 255));
-  k2 = uniform(k2);
-  const float up = ldexpf(1.f, k2), qmul = ldexpf(a.scale * 1.4426950408889634f, 24 - k2);
-#pragma unroll
-  for (int i = 0; i < QT; ++i) {
+    top_q = over_rows(top_q, [](float p, float q) { return fmaxf(p, q); });
+    int k2 = 0;
+    if (top_q > 0.f) k2 = min(120, 140 - (int)((__float_as_uint(top_q) >> 23) & 255));
+    const float up = ldexpf(1.f, k2);
+    qmul[i] = ldexpf(a.scale * 1.4426950408889634f, 24 - k2);
     float sum = 0.f;
 #pragma unroll
     for (int n = 0; n < ND; ++n) {
@@ -223,9 +219,9 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
       to[192] = v_operand<4>(va.x >> 8, va.y >> 8, vb.x >> 8, vb.y >> 8);
     }
     if (wave == 0 && lane < ST) {
-      const float s = kv4_step(pw) * qmul;
+      const float s = kv4_step(pw);
       par[buf][0][lane] = s;
-      par[buf][1][lane] = fmaf(-7.5f, s, kv4_centre(pw) * qmul);
+      par[buf][1][lane] = fmaf(-7.5f, s, kv4_centre(pw));
       if (c == 0) gone[buf][g] = p_none;
     }
     if (wave == 1 && lane < ST) {
@@ -236,14 +232,13 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
 
   f4 o[QT][NP][NH][4];
   f4 wsum[QT];
-  float l[QT], z[QT], m[QT], ref[QT];  // ref: 0 while m is none
+  float l[QT], z[QT], m[QT], ref[QT];
   int ev = -80;
-  float sv_top = -1.f;       // 2^ev, or -1 before the first tokens
-  float limit = -INFINITY;   // of x - ref, beyond which a maximum moves
+  float sv_top = 0x1p-80f;  // 2^ev
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
-    l[i] = z[i] = ref[i] = 0.f;
-    m[i] = kAttnNone;
+    l[i] = z[i] = 0.f;
+    m[i] = ref[i] = kAttnNone;
     wsum[i] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < NP * NH * 4; ++x) o[i][x / (NH * 4)][x / 4 % NH][x % 4] = f4{0.f, 0.f, 0.f, 0.f};
@@ -286,7 +281,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) mv[h] = *reinterpret_cast<const f4*>(&par[buf][3][32 * j + 16 * h + 4 * g]);
     __builtin_amdgcn_sched_barrier(0);
-    // x - ref, in place of the sums
+    // the exponents / qmul, in place of the sums
     float xm[QT], top = -1.f;
 #pragma unroll
     for (int i = 0; i < QT; ++i) xm[i] = -INFINITY;
@@ -296,32 +291,33 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
       for (int e = 0; e < 4; ++e) top = fmaxf(top, sv[h][e]);
 #pragma unroll
       for (int i = 0; i < QT; ++i) {
-        const float base = none[h] - ref[i];
+        float xh = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float y = fmaf(sk[h][e], acc[i][h][e], fmaf(mk[h][e], qsum[i], base));
+          float y = fmaf(sk[h][e], acc[i][h][e], mk[h][e] * qsum[i]);
           if constexpr (masked) y = sees(i, h, e) ? y : -INFINITY;
           acc[i][h][e] = y;
-          xm[i] = fmaxf(xm[i], y);
+          xh = fmaxf(xh, y);
         }
+        xm[i] = fmaxf(xm[i], xh + none[h]);
       }
     }
     bool grow = masked | (top > sv_top);
 #pragma unroll
-    for (int i = 0; i < QT; ++i) grow = grow | (xm[i] > limit);
+    for (int i = 0; i < QT; ++i) grow = grow | (xm[i] * qmul[i] > m[i] + (float)kAttnHead);
     if (masked || __any(grow)) {
       top = over_rows(top, [](float p, float q) { return fmaxf(p, q); });
+      const int was = ev;
       ev = max(ev, (int)((__float_as_uint(fmaxf(top, 0.f)) >> 23) & 255) - 126);
       sv_top = __uint_as_float((uint32_t)(ev + 127) << 23);
-      limit = (float)(kAttnHead + kAttnBase - ev);
 #pragma unroll
       for (int i = 0; i < QT; ++i) {
-        const float x = over_rows(xm[i], [](float p, float q) { return fmaxf(p, q); });
-        const bool was = m[i] != kAttnNone;
-        const float t = fmaxf(m[i], x + ref[i]);
-        const float nr = t != kAttnNone ? t + (float)(ev - kAttnBase) : 0.f;
-        const float move = ref[i] - nr, f = was ? __builtin_amdgcn_exp2f(move) : 1.f;
-        m[i] = t;
+        const float x = over_rows(xm[i], [](float p, float q) { return fmaxf(p, q); }) * qmul[i];
+        // a row moves for what it has seen itself, whatever the others saw
+        const bool move = masked | (ev > was) | (x > m[i] + (float)kAttnHead);
+        m[i] = move ? fmaxf(m[i], x) : m[i];
+        const float nr = move ? m[i] + (float)(ev - kAttnBase) : ref[i];
+        const float f = __builtin_amdgcn_exp2f(ref[i] - nr);
         ref[i] = nr;
         l[i] *= f;
         z[i] *= f;
@@ -332,10 +328,6 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
           for (int h = 0; h < NH; ++h)
 #pragma unroll
             for (int b = 0; b < 4; ++b) o[i][p][h][b] *= f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][h][e] += move;
       }
     }
     u4 pf[QT];
@@ -344,9 +336,10 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float pv[4];
+        const float off = none[h] - ref[i];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(acc[i][h][e]);
+          const float p = __builtin_amdgcn_exp2f(fmaf(acc[i][h][e], qmul[i], off));
           pv[e] = p * sv[h][e];
           if constexpr (masked) {
             const bool ok = sees(i, h, e);
@@ -405,7 +398,6 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
     const int e0 = down(max(min(from, end), begin)), e1 = max(full0 > begin ? down(full0 + ST - 1) : begin, e0);
     stages(min(e0, end), idle);
     stages(min(min(e1, to), end), cut);
-    limit = -INFINITY;  // rows that have seen no token yet take their reference now
     stages(down(max(full1, begin)), all);
     stages(to, cut);
     stages(end, idle);
@@ -434,7 +426,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
             *reinterpret_cast<f4*>(a.part + pr * HD + p * PW + g * (PW / 4) + 4 * NH * e + 4 * h) =
                 f4{value(p, e, h, 0), value(p, e, h, 1), value(p, e, h, 2), value(p, e, h, 3)};
       if (g == 0) {
-        a.part_ml[2 * pr] = m[i] != kAttnNone ? ref[i] : kAttnNone;
+        a.part_ml[2 * pr] = ref[i];
         a.part_ml[2 * pr + 1] = l[i];
       }
     } else {
