@@ -203,6 +203,13 @@ __device__ inline float over_rows(float v, OP op) {
   return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// The least power of two above a step; kAttnStep at least.
+constexpr float kAttnStep = 0x1p-80f;
+__device__ inline float above_step(float s) {
+  return fmaxf(kAttnStep, __uint_as_float((__float_as_uint(s) & 0x7F800000u) + 0x00800000u));
+}
+__device__ inline float exponent_of(float power) { return (float)((int)(__float_as_uint(power) >> 23) - 127); }
+
 __device__ inline uint32_t pack_h2(float a, float b) {
   return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});
 }

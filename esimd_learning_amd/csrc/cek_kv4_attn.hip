@@ -23,8 +23,8 @@
 // contraction is free -- the operand of O^T = V^T P^T; V's words hold four tokens
 // side by side for that.  Each code byte is read once, 1 KB a load instruction.
 //
-// Weights: with M a running maximum of the exponents and 2^E above every sv so
-// far, P = exp2(x - M - E + 9) makes P sv at most 2^9 as it comes and 2^15 with
+// Weights: with M a running maximum of a row's exponents and 2^E above every sv that
+// the row has seen, P = exp2(x - M - E + 9) makes P sv at most 2^9 as it comes and 2^15 with
 // the 2^6 that a maximum may lag behind (it moves, and the sums are rescaled,
 // only where a score exceeds it by more): fp16 holds P sv to half a step (2^-12
 // of the value) down to 2^-23 of the largest.  Sums are fp32; sum(P sv) / 2 is
@@ -304,12 +304,12 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   f4 o[QT][NP][NH][4];
   f4 wsum[QT];
   float l[QT], z[QT], m[QT], ref[QT];
-  int ev = -80;
-  float sv_top = 0x1p-80f;  // 2^ev
+  float sv_top[QT];  // 2^E, above every V step that the row has seen
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     l[i] = z[i] = 0.f;
     m[i] = ref[i] = kAttnNone;
+    sv_top[i] = kAttnStep;
     wsum[i] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < NP * NH * 4; ++x) o[i][x / (NH * 4)][x / 4 % NH][x % 4] = f4{0.f, 0.f, 0.f, 0.f};
@@ -351,8 +351,8 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     slot = slot + 1 == DEPTH ? 0 : slot + 1;
   };
 
-  // Scores of 32 tokens: x (exponents / qmul), their maxima xm and that of the V steps.
-  float x[QT][NX][4], xm[QT], top;
+  // Scores of 32 tokens: x (exponents / qmul), their maxima xm and those of the V steps.
+  float x[QT][NX][4], xm[QT], top[QT];
   auto scores = [&](int t0, auto mask) {
     constexpr bool masked = decltype(mask)::value;
     if constexpr (masked) {
@@ -379,9 +379,12 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
         for (int i = 0; i < QT; ++i) acc[i][h] = mfma16x16x32<F16>(f, qf[i][n], acc[i][h]);
       }
     }
-    top = -1.f;
+    float step_top = 0.f;  // of the lane's tokens, where all rows see them
 #pragma unroll
-    for (int i = 0; i < QT; ++i) xm[i] = -INFINITY;
+    for (int i = 0; i < QT; ++i) {
+      xm[i] = -INFINITY;
+      top[i] = 0.f;
+    }
     if constexpr (FOLD) {
 #pragma unroll
       for (int i = 0; i < QT; ++i)
@@ -396,22 +399,29 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float sk = kv4_step(kp[h][e]), mk = fmaf(-7.5f, sk, kv4_centre(kp[h][e]));
-        top = fmaxf(top, kv4_step(vp[h][e]));
+        if constexpr (!masked) step_top = fmaxf(step_top, kv4_step(vp[h][e]));
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
           x[i][h][e] = fmaf(sk, acc[i][h][e], mk * qsum[i]);
-          if constexpr (masked) x[i][h][e] = sees(i, t0, h, e) ? x[i][h][e] : -INFINITY;
+          if constexpr (masked) {
+            const bool ok = sees(i, t0, h, e);
+            x[i][h][e] = ok ? x[i][h][e] : -INFINITY;
+            top[i] = fmaxf(top[i], ok ? kv4_step(vp[h][e]) : 0.f);
+          }
           xh[i] = fmaxf(xh[i], x[i][h][e]);
         }
       }
 #pragma unroll
       for (int i = 0; i < QT; ++i) xm[i] = fmaxf(xm[i], xh[i] + none[h]);
     }
+    if constexpr (!masked)
+#pragma unroll
+      for (int i = 0; i < QT; ++i) top[i] = step_top;
   };
   auto grows = [&]() {
-    bool y = top > sv_top;
+    bool y = false;
 #pragma unroll
-    for (int i = 0; i < QT; ++i) y = y | (xm[i] * qmul[i] > m[i] + (float)kAttnHead);
+    for (int i = 0; i < QT; ++i) y = y | (top[i] > sv_top[i]) | (xm[i] * qmul[i] > m[i] + (float)kAttnHead);
     return __any(y);
   };
   // Over the lanes that hold one row.
@@ -422,17 +432,15 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
   // New references, and the sums so far brought to them.
   auto rescale = [&](auto mask) {
     constexpr bool masked = decltype(mask)::value;
-    top = over_row(top, [](float p, float q) { return fmaxf(p, q); });
-    const int was = ev;
-    ev = max(ev, (int)((__float_as_uint(fmaxf(top, 0.f)) >> 23) & 255) - 126);
-    sv_top = __uint_as_float((uint32_t)(ev + 127) << 23);
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
       const float t = over_row(xm[i], [](float p, float q) { return fmaxf(p, q); }) * qmul[i];
       // a row moves for what it has seen itself, whatever the others saw
-      const bool move = masked | (ev > was) | (t > m[i] + (float)kAttnHead);
+      top[i] = over_row(top[i], [](float p, float q) { return fmaxf(p, q); });
+      const bool move = masked | (top[i] > sv_top[i]) | (t > m[i] + (float)kAttnHead);
+      sv_top[i] = move ? fmaxf(sv_top[i], above_step(top[i])) : sv_top[i];
       m[i] = move ? fmaxf(m[i], t) : m[i];
-      const float nr = move ? m[i] + (float)(ev - kAttnBase) : ref[i];
+      const float nr = move ? m[i] + (exponent_of(sv_top[i]) - (float)kAttnBase) : ref[i];
       const float f = __builtin_amdgcn_exp2f(ref[i] - nr);
       ref[i] = nr;
       l[i] *= f;

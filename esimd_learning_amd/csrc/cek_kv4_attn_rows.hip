@@ -224,21 +224,24 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
       par[buf][1][lane] = fmaf(-7.5f, s, kv4_centre(pw));
       if (c == 0) gone[buf][g] = p_none;
     }
-    if (wave == 1 && lane < ST) {
-      par[buf][2][lane] = kv4_step(pw);
-      par[buf][3][lane] = kv4_centre(pw);
+    if (wave == 1) {
+      float s = kv4_step(pw);
+      if (lane < ST) {
+        par[buf][2][lane] = s;
+        par[buf][3][lane] = kv4_centre(pw);
+      }
     }
   };
 
   f4 o[QT][NP][NH][4];
   f4 wsum[QT];
   float l[QT], z[QT], m[QT], ref[QT];
-  int ev = -80;
-  float sv_top = 0x1p-80f;  // 2^ev
+  float sv_top[QT];  // 2^E, above every V step that the row has seen
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     l[i] = z[i] = 0.f;
     m[i] = ref[i] = kAttnNone;
+    sv_top[i] = kAttnStep;
     wsum[i] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < NP * NH * 4; ++x) o[i][x / (NH * 4)][x / 4 % NH][x % 4] = f4{0.f, 0.f, 0.f, 0.f};
@@ -256,6 +259,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
     u4 kf[2 * ND], vf[NV];
     f4 acc[QT][2], sk[2], mk[2], sv[2], mv[2];
     float none[2];
+    float step_top = 0.f;
 #pragma unroll
     for (int n = 0; n < 2 * ND; ++n) kf[n] = k_op[buf][2 * j * ND + n][lane];
 #pragma unroll
@@ -282,41 +286,50 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
     for (int h = 0; h < 2; ++h) mv[h] = *reinterpret_cast<const f4*>(&par[buf][3][32 * j + 16 * h + 4 * g]);
     __builtin_amdgcn_sched_barrier(0);
     // the exponents / qmul, in place of the sums
-    float xm[QT], top = -1.f;
+    float xm[QT], top[QT];
 #pragma unroll
-    for (int i = 0; i < QT; ++i) xm[i] = -INFINITY;
+    for (int i = 0; i < QT; ++i) {
+      xm[i] = -INFINITY;
+      top[i] = 0.f;
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      if constexpr (!masked)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top = fmaxf(top, sv[h][e]);
+        for (int e = 0; e < 4; ++e) step_top = fmaxf(step_top, sv[h][e]);
 #pragma unroll
       for (int i = 0; i < QT; ++i) {
         float xh = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float y = fmaf(sk[h][e], acc[i][h][e], mk[h][e] * qsum[i]);
-          if constexpr (masked) y = sees(i, h, e) ? y : -INFINITY;
+          if constexpr (masked) {
+            const bool ok = sees(i, h, e);
+            y = ok ? y : -INFINITY;
+            top[i] = fmaxf(top[i], ok ? sv[h][e] : 0.f);
+          }
           acc[i][h][e] = y;
           xh = fmaxf(xh, y);
         }
         xm[i] = fmaxf(xm[i], xh + none[h]);
       }
     }
-    bool grow = masked | (top > sv_top);
+    if constexpr (!masked)
 #pragma unroll
-    for (int i = 0; i < QT; ++i) grow = grow | (xm[i] * qmul[i] > m[i] + (float)kAttnHead);
+      for (int i = 0; i < QT; ++i) top[i] = step_top;
+    bool grow = masked;
+#pragma unroll
+    for (int i = 0; i < QT; ++i) grow = grow | (top[i] > sv_top[i]) | (xm[i] * qmul[i] > m[i] + (float)kAttnHead);
     if (masked || __any(grow)) {
-      top = over_rows(top, [](float p, float q) { return fmaxf(p, q); });
-      const int was = ev;
-      ev = max(ev, (int)((__float_as_uint(fmaxf(top, 0.f)) >> 23) & 255) - 126);
-      sv_top = __uint_as_float((uint32_t)(ev + 127) << 23);
 #pragma unroll
       for (int i = 0; i < QT; ++i) {
+        top[i] = over_rows(top[i], [](float p, float q) { return fmaxf(p, q); });
         const float x = over_rows(xm[i], [](float p, float q) { return fmaxf(p, q); }) * qmul[i];
         // a row moves for what it has seen itself, whatever the others saw
-        const bool move = masked | (ev > was) | (x > m[i] + (float)kAttnHead);
+        const bool move = masked | (top[i] > sv_top[i]) | (x > m[i] + (float)kAttnHead);
+        sv_top[i] = move ? fmaxf(sv_top[i], above_step(top[i])) : sv_top[i];
         m[i] = move ? fmaxf(m[i], x) : m[i];
-        const float nr = move ? m[i] + (float)(ev - kAttnBase) : ref[i];
+        const float nr = move ? m[i] + (exponent_of(sv_top[i]) - (float)kAttnBase) : ref[i];
         const float f = __builtin_amdgcn_exp2f(ref[i] - nr);
         ref[i] = nr;
         l[i] *= f;

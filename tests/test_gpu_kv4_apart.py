@@ -1,11 +1,13 @@
-"""GPU: a row of the attention over the 4-bit cache beside others that are far larger or smaller, or not finite.  The
-batch and the tolerance are tests/test_gpu_kv4.py's; where nothing that a row may see has changed, its bits have not."""
+"""GPU: a row of the attention over the 4-bit cache beside others that are far larger or smaller, or not finite, and
+before tokens that it must not see.  The batch and the tolerance are tests/test_gpu_kv4.py's; where nothing that a row
+may see has changed, its bits have not."""
 
 import math
 
 import pytest
 import torch
 
+from oracle import kv4
 from test_gpu_kv4 import Batch, _say
 
 pytestmark = pytest.mark.gpu
@@ -14,6 +16,33 @@ HEADS = [(8, 2, 64), (8, 2, 128), (8, 2, 256), (4, 4, 128), (7, 1, 64)]
 # hints: true ones, none (keys shared by the workgroups), and two that name the kernel for few and for many rows
 HINTS = [dict(mq=45, mk=160), dict(mq=0, mk=0), dict(mq=1, mk=160), dict(mq=45, mk=5000), dict(mq=1, mk=5000)]
 LENS, QLENS = [160, 45, 90, 7], [45, 45, 3, 1]
+
+
+def _slots(b, r, first, n):
+    t = torch.arange(first, first + n)
+    return (b.host_tables[r].long()[t // b.bs] * b.bs + t % b.bs).to(b.tables.device)
+
+
+def _store(b, ops, r, first, k=None, v=None):
+    """Tokens first .. of request r take the rows k, v [n, nk, hd] (None: as they are)."""
+    n = len(v if k is None else k)
+    slots = _slots(b, r, first, n)
+    old = [torch.empty(n, *b.heads[1:], dtype=b.dtype, device=b.tables.device) for _ in range(2)]
+    keep = b.cache.clone()
+    ops.esimd_kv4_cache_read(b.cache, slots, *old)
+    new = [o if x is None else x.to(o) for o, x in zip(old, (k, v))]
+    ops.esimd_kv4_cache_write(*new, b.cache, slots)
+    nk, bs, hd = b.heads[1], b.bs, b.heads[2]
+    for x, a, z, vals in ((k, 0, bs * hd // 2, b.keys), (v, bs * hd // 2, bs * hd, b.vals)):
+        p = bs * hd + (0 if vals is b.keys else 4 * bs)
+        if x is None:       # the bytes as they were
+            now, was = b.cache.flatten(2), keep.flatten(2)
+            now[..., a:z], now[..., p:p + 4 * bs] = was[..., a:z], was[..., p:p + 4 * bs]
+            continue
+        c, s, m = kv4.quantise(x)
+        vals[r][first:first + n] = kv4.values(c, s, m)
+        if vals is b.vals:
+            b.spread[r][first:first + n] = 7.5 * s.double()[..., None]
 
 
 def _set_q(b, q):
@@ -71,3 +100,23 @@ def test_one_row_that_is_not_finite(ops, dev, nq, nk, hd, bad, dtype):
             same = (out == ref).all(-1).cpu()
             same[tuple(zip(*spoilt))] = True
             assert same.all(), (h, (~same).nonzero()[:8].tolist())
+
+
+@pytest.mark.parametrize("nq,nk,hd", HEADS)
+@pytest.mark.parametrize("far", [1.0, 2.0 ** 20, 2.0 ** 60, -2.0 ** 90])
+def test_tokens_behind_a_row_change_nothing(ops, dev, nq, nk, hd, far):
+    """One token of a chunk with another key, and a value far larger: the rows before it keep their bits, the others are right."""
+    _say("behind", nq, nk, hd, far)
+    b = Batch(LENS, QLENS, nq, nk, hd, 16, torch.bfloat16, dev, seed=nq + hd)
+    refs = [b.run(ops, **h) for h in HINTS]
+    g = torch.Generator().manual_seed(1)
+    # position 140 of request 0 is its row 25, position 30 of request 1 its row 30, 88 of request 2 its row 1
+    for r, at in ((0, 140), (1, 30), (2, 88)):
+        _store(b, ops, r, at, k=torch.randn(1, nk, hd, generator=g).bfloat16(),
+               v=(torch.randn(1, nk, hd, generator=g) * far).bfloat16())
+    for h, ref in zip(HINTS, refs):
+        out = b.run(ops, **h)
+        assert torch.equal(out[:25], ref[:25]), h
+        assert torch.equal(out[45:75], ref[45:75]), h
+        assert torch.equal(out[90], ref[90]) and torch.equal(out[93], ref[93]), h
+        b.check(out)
