@@ -203,6 +203,11 @@ __device__ inline float over_rows(float v, OP op) {
   return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// V's step as the products take it: of a row that is one value throughout (step 0)
+// 2^-40 of that value, which changes nothing that fp32 holds and keeps the weights,
+// up to 2^15 over the largest step, times the value in fp32's range.
+__device__ inline float v_step_of(uint32_t p) { return fmaxf(kv4_step(p), fabsf(kv4_centre(p)) * 0x1p-40f); }
+
 // The least power of two above a step; kAttnStep at least.
 constexpr float kAttnStep = 0x1p-80f;
 __device__ inline float above_step(float s) {

@@ -399,14 +399,14 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float sk = kv4_step(kp[h][e]), mk = fmaf(-7.5f, sk, kv4_centre(kp[h][e]));
-        if constexpr (!masked) step_top = fmaxf(step_top, kv4_step(vp[h][e]));
+        if constexpr (!masked) step_top = fmaxf(step_top, v_step_of(vp[h][e]));
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
           x[i][h][e] = fmaf(sk, acc[i][h][e], mk * qsum[i]);
           if constexpr (masked) {
             const bool ok = sees(i, t0, h, e);
             x[i][h][e] = ok ? x[i][h][e] : -INFINITY;
-            top[i] = fmaxf(top[i], ok ? kv4_step(vp[h][e]) : 0.f);
+            top[i] = fmaxf(top[i], ok ? v_step_of(vp[h][e]) : 0.f);
           }
           xh[i] = fmaxf(xh[i], x[i][h][e]);
         }
@@ -465,7 +465,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
       for (int i = 0; i < QT; ++i) off[i] = none[h] - ref[i];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float sv = kv4_step(vp[h][e]), mv = kv4_centre(vp[h][e]);
+        const float sv = v_step_of(vp[h][e]), mv = kv4_centre(vp[h][e]);
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
           const float p = __builtin_amdgcn_exp2f(fmaf(x[i][h][e], qmul[i], off[i]));

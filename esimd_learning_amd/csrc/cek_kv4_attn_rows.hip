@@ -224,12 +224,9 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
       par[buf][1][lane] = fmaf(-7.5f, s, kv4_centre(pw));
       if (c == 0) gone[buf][g] = p_none;
     }
-    if (wave == 1) {
-      float s = kv4_step(pw);
-      if (lane < ST) {
-        par[buf][2][lane] = s;
-        par[buf][3][lane] = kv4_centre(pw);
-      }
+    if (wave == 1 && lane < ST) {
+      par[buf][2][lane] = v_step_of(pw);
+      par[buf][3][lane] = kv4_centre(pw);
     }
   };
 

@@ -120,3 +120,17 @@ def test_tokens_behind_a_row_change_nothing(ops, dev, nq, nk, hd, far):
         assert torch.equal(out[45:75], ref[45:75]), h
         assert torch.equal(out[90], ref[90]) and torch.equal(out[93], ref[93]), h
         b.check(out)
+
+
+@pytest.mark.parametrize("hints", HINTS)
+@pytest.mark.parametrize("nq,nk,hd", HEADS)
+@pytest.mark.parametrize("size", [2.0 ** 40, -2.0 ** 100, 2.0 ** -60, 0.0])
+def test_values_without_spread(ops, dev, nq, nk, hd, hints, size):
+    """V rows that are one value throughout (step 0), large and small."""
+    _say("no spread", nq, nk, hd, hints, size)
+    b = Batch(LENS, QLENS, nq, nk, hd, 16, torch.bfloat16, dev, seed=nq + hd)
+    g = torch.Generator().manual_seed(2)
+    for r, n in enumerate(LENS):
+        _store(b, ops, r, 0, v=(torch.rand(n, nk, 1, generator=g) + 0.5).mul(size).expand(-1, -1, hd).bfloat16())
+        assert (b.spread[r] == 0).all()
+    b.check(b.run(ops, **hints))
