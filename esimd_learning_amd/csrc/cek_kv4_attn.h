@@ -28,7 +28,7 @@ struct Kv4AttnArgs {
 
 constexpr int kAttnWaves = 4;
 constexpr int kAttnHead = 6, kAttnBase = 9;  // exponents: lag of a maximum, where the largest weight lies
-constexpr float kAttnNone = -1e30f;
+constexpr float kAttnNone = -3e38f;
 
 typedef const __attribute__((address_space(4))) int32_t* const_i32;  // scalar loads
 
@@ -213,7 +213,12 @@ constexpr float kAttnStep = 0x1p-80f;
 __device__ inline float above_step(float s) {
   return fmaxf(kAttnStep, __uint_as_float((__float_as_uint(s) & 0x7F800000u) + 0x00800000u));
 }
-__device__ inline float exponent_of(float power) { return (float)((int)(__float_as_uint(power) >> 23) - 127); }
+// A row's reference, from its maximum m and 2^E.  From 2^22 on fp32 has no room for E
+// beside m: the reference is m alone, and the largest weight 1.
+__device__ inline float attn_ref(float m, float power) {
+  const int e = (int)(__float_as_uint(power) >> 23) - 127;
+  return fabsf(m) < 0x1p22f ? m + (float)(e - kAttnBase) : m;
+}
 
 __device__ inline uint32_t pack_h2(float a, float b) {
   return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});

@@ -13,7 +13,8 @@
 // enter the fp16 MFMA as they lie: a 32-bit word & 0x000F000F is a pair of fp16
 // subnormals c 2^-24, & 0x00F000F0 a pair c 2^-20 -- exact, one AND (and a shift
 // for every second pair) where a conversion would take three operations.  The
-// powers of two are taken back in q (2^-4 for the second kind) and in the scores.
+// powers of two are taken back in q (2^-4 for the second kind) and in the scores --
+// exactly, so that a row's largest score less its maximum is 0 at any size.
 // V's take an OR and a packed subtraction more (v_pair).
 //
 // Layout: everything stays in registers.  A wave takes 32 tokens at a time and
@@ -298,7 +299,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     }
     sum = over_rows(sum, [](float p, float q) { return p + q; });
     qsum[i] = sum * 0x1p-24f;
-    qmul[i] = ldexpf(a.scale * 1.4426950408889634f, 24 - k);
+    qmul[i] = ldexpf(1.f, 24 - k);
   }
 
   f4 o[QT][NP][NH][4];
@@ -398,7 +399,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
       for (int i = 0; i < QT; ++i) xh[i] = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float sk = kv4_step(kp[h][e]), mk = fmaf(-7.5f, sk, kv4_centre(kp[h][e]));
+        const float sk = kv4_step(kp[h][e]) * a.scale, mk = fmaf(-7.5f, sk, kv4_centre(kp[h][e]) * a.scale);
         if constexpr (!masked) step_top = fmaxf(step_top, v_step_of(vp[h][e]));
 #pragma unroll
         for (int i = 0; i < QT; ++i) {
@@ -440,7 +441,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
       const bool move = masked | (top[i] > sv_top[i]) | (t > m[i] + (float)kAttnHead);
       sv_top[i] = move ? fmaxf(sv_top[i], above_step(top[i])) : sv_top[i];
       m[i] = move ? fmaxf(m[i], t) : m[i];
-      const float nr = move ? m[i] + (exponent_of(sv_top[i]) - (float)kAttnBase) : ref[i];
+      const float nr = move ? attn_ref(m[i], sv_top[i]) : ref[i];
       const float f = __builtin_amdgcn_exp2f(ref[i] - nr);
       ref[i] = nr;
       l[i] *= f;
@@ -861,7 +862,7 @@ extern "C" int cek_kv4_attention(const void* q, const void* cache, const int32_t
   a.group = (int)(n_q / n_kv);
   a.max_blocks = (int)max_blocks;
   a.window = (int)window;
-  a.scale = scale;
+  a.scale = scale * 1.4426950408889634f;  // weights are powers of two
   a.vec_q = aligned(q, 16) && q_stride % 8 == 0;
   a.vec_out = aligned(out, 8) && out_stride % 4 == 0;
   AttnPlan p = attn_plan(T, R, n_q, n_kv, hd, max_q_len, max_kv_len);

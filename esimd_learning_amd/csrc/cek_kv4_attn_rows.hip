@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
     int k2 = 0;
     if (top_q > 0.f) k2 = min(120, 140 - (int)((__float_as_uint(top_q) >> 23) & 255));
     const float up = ldexpf(1.f, k2);
-    qmul[i] = ldexpf(a.scale * 1.4426950408889634f, 24 - k2);
+    qmul[i] = ldexpf(1.f, 24 - k2);
     float sum = 0.f;
 #pragma unroll
     for (int n = 0; n < ND; ++n) {
@@ -219,9 +219,9 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
       to[192] = v_operand<4>(va.x >> 8, va.y >> 8, vb.x >> 8, vb.y >> 8);
     }
     if (wave == 0 && lane < ST) {
-      const float s = kv4_step(pw);
+      const float s = kv4_step(pw) * a.scale;
       par[buf][0][lane] = s;
-      par[buf][1][lane] = fmaf(-7.5f, s, kv4_centre(pw));
+      par[buf][1][lane] = fmaf(-7.5f, s, kv4_centre(pw) * a.scale);
       if (c == 0) gone[buf][g] = p_none;
     }
     if (wave == 1 && lane < ST) {
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
         const bool move = masked | (top[i] > sv_top[i]) | (x > m[i] + (float)kAttnHead);
         sv_top[i] = move ? fmaxf(sv_top[i], above_step(top[i])) : sv_top[i];
         m[i] = move ? fmaxf(m[i], x) : m[i];
-        const float nr = move ? m[i] + (exponent_of(sv_top[i]) - (float)kAttnBase) : ref[i];
+        const float nr = move ? attn_ref(m[i], sv_top[i]) : ref[i];
         const float f = __builtin_amdgcn_exp2f(ref[i] - nr);
         ref[i] = nr;
         l[i] *= f;

@@ -134,3 +134,30 @@ def test_values_without_spread(ops, dev, nq, nk, hd, hints, size):
         _store(b, ops, r, 0, v=(torch.rand(n, nk, 1, generator=g) + 0.5).mul(size).expand(-1, -1, hd).bfloat16())
         assert (b.spread[r] == 0).all()
     b.check(b.run(ops, **hints))
+
+
+@pytest.mark.parametrize("nq,nk,hd", HEADS)
+@pytest.mark.parametrize("hints", HINTS)
+def test_rows_of_all_sizes(ops, dev, nq, nk, hd, hints):
+    """bf16 rows of a tile 2^130 apart, tokens and heads: each as if it were alone.  (Rows of 2^24 and more have one key
+    left: what fp32 loses of a score of 2^26, some 2^4, is a 2^22th of the distance between two.)"""
+    _say("sizes", nq, nk, hd, hints)
+    b = Batch(LENS, QLENS, nq, nk, hd, 16, torch.bfloat16, dev, seed=nq + hd)
+    size = torch.tensor([0, 40, -30, 100, 24, -3])
+    t, h = torch.arange(b.cu[-1])[:, None], torch.arange(nq)[None]
+    _set_q(b, (b.q.float() * torch.exp2(size[(t + 2 * h) % 6].float())[..., None]).bfloat16())
+    b.check(b.run(ops, **hints))
+
+
+@pytest.mark.parametrize("hints", HINTS)
+@pytest.mark.parametrize("nq,nk,hd", HEADS)
+def test_scores_far_below_zero(ops, dev, nq, nk, hd, hints):
+    """q of 2^100 against the only key there is, its negative: the key's value, however small the score."""
+    _say("far below", nq, nk, hd, hints)
+    b = Batch([1, 1, 45], [1, 1, 45], nq, nk, hd, 16, torch.bfloat16, dev, seed=nq + hd)
+    k = torch.ones(1, nk, hd).bfloat16()
+    for r in (0, 1):
+        _store(b, ops, r, 0, k=k)
+    _store(b, ops, 2, 0, k=k.expand(45, -1, -1))
+    _set_q(b, torch.full_like(b.q, -2.0 ** 100))
+    b.check(b.run(ops, **hints))
