@@ -678,10 +678,12 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4AttnArgs a, int n
     y *= keep;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      const float f = base + i < parts.n ? __builtin_amdgcn_exp2f(ml[i].x - nt) : 0.f;
-      den = f != 0.f ? fmaf(f, ml[i].y, den) : den;
+      // (a part of weight 0 counts too: what it holds may be NaN)
+      const bool in = base + i < parts.n;
+      const float f = __builtin_amdgcn_exp2f(ml[i].x - nt);
+      den = in ? fmaf(f, ml[i].y, den) : den;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = f != 0.f ? fmaf(v[i][e], f, y[e]) : y[e];
+      for (int e = 0; e < 4; ++e) y[e] = in ? fmaf(v[i][e], f, y[e]) : y[e];
     }
   }
   const float inv = den != 0.f ? 1.0f / den : 0.f;
@@ -725,8 +727,8 @@ __global__ __launch_bounds__(256) void kv4_attn_join_wide_kernel(Kv4AttnArgs a, 
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int p = grp + G * i;
-      const float w = __shfl(f, p, 64), fp = p < n ? w : 0.f;
-      y = fp != 0.f ? fmaf(v[i], fp, y) : y;
+      const float w = __shfl(f, p, 64);
+      y = p < n ? fmaf(v[i], w, y) : y;
     }
   }
   __shared__ float so[G][32];

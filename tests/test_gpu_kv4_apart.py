@@ -161,3 +161,18 @@ def test_scores_far_below_zero(ops, dev, nq, nk, hd, hints):
     _store(b, ops, 2, 0, k=k.expand(45, -1, -1))
     _set_q(b, torch.full_like(b.q, -2.0 ** 100))
     b.check(b.run(ops, **hints))
+
+
+def test_parts_whose_keys_are_all_nan(ops, dev):
+    """Keys split over workgroups: NaN keys that fill a workgroup's share reach the rows like any others, whichever of
+    the joins has them."""
+    nq, nk, hd, n = 8, 8, 128, 20000
+    for rows in (1, 70):
+        _say("nan parts", rows)
+        b = Batch([n], [rows], nq, nk, hd, 64, torch.float16, dev, seed=3)
+        nan = torch.full((128, nk, hd), math.nan, dtype=torch.float16, device=dev)
+        one = torch.ones_like(nan)
+        for first in range(0, 6400, 128):
+            ops.esimd_kv4_cache_write(nan, one, b.cache, _slots(b, 0, first, 128))
+            for h in (dict(mq=rows), dict(mq=0, mk=0), dict(mq=1)):
+                assert b.run(ops, **h).isnan().all(), (first, h)
