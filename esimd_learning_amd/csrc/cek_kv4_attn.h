@@ -22,6 +22,7 @@ struct Kv4AttnArgs {
   int wgs;                    // workgroups per kv head that share the keys; 0: keys stay whole
   int part_row0;              // first partial row of this launch
   int part_rows;              // of all
+  int max_parts;              // of a row
   int vec_q, vec_out;
   float scale;
 };

@@ -644,8 +644,9 @@ struct Kv4Parts {
     row0 = mt.x + (int64_t)kvh * mt.w;
     step = mt.z;
     n = mt.y;
-    // (rows that offsets out of order left without a worker: whatever the workspace held)
-    const bool no = (t < c0) | (t >= c1) | (mt.y <= 1) | (mt.x < 0) | (mt.z < 0) | (mt.w < 0);
+    // (rows that offsets out of order left without a worker: whatever the workspace
+    // held -- no more parts than workgroups share a tile, each in a row of its own)
+    const bool no = (t < c0) | (t >= c1) | (mt.y <= 1) | (mt.y > a.max_parts) | (mt.x < 0) | (mt.z <= 0) | (mt.w < 0);
     if (no || row(n - 1) >= a.part_rows) n = 0;
   }
   __device__ inline int64_t row(int p) const { return row0 + (int64_t)step * (p > 0 ? 2 * p - 1 : 0); }
@@ -876,6 +877,7 @@ extern "C" int cek_kv4_attention(const void* q, const void* cache, const int32_t
     a.part_ml = a.part + p.part_rows * hd;
     a.meta = reinterpret_cast<int4*>(a.part_ml + p.part_rows * 2);
     a.part_rows = (int)std::min<int64_t>(p.part_rows, INT32_MAX);
+    a.max_parts = std::max(p.wgs_few, p.wgs_many);
   }
   if (p.tiles_few * n_kv > INT32_MAX || p.tiles_many * n_kv > INT32_MAX || p.part_rows > INT32_MAX || T * n_q > INT32_MAX)
     return CEK_ERR_UNSUPPORTED;
