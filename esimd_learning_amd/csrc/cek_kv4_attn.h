@@ -40,6 +40,10 @@ struct Kv4Work {
   int first, span;       // the tile's first unit in the list; how far the stretch reaches there
 };
 
+// The position of a request's new row t.  Rows before position 0 see no key: -1, from
+// which a window of up to 2^31 - 1 can be taken without an overflow.
+__device__ inline int kv4_pos(int kv, int n_new, int t) { return max(kv - n_new + t, -1); }
+
 // The work list: every request has ceil(rows / BR) tiles of rows, and each tile its
 // keys (from the first that any row sees, down to a multiple of 32) in units of
 // `len` tokens, or in one.  Tiles lie one after another, a request's last one
@@ -72,7 +76,7 @@ struct Kv4List {
     const bool mine = (r < a.R) & (x.n_new > 0) & (n > a.rows_above) & (n <= a.rows_upto);
     x.rows = mine ? (int)n : 0;
     x.kv = (int)min((int64_t)max(kv, 0), (int64_t)a.max_blocks << a.dm.bs_log2);
-    x.lo = a.window > 0 ? max(0, x.kv - x.n_new - a.window + 1) & ~31 : 0;
+    x.lo = a.window > 0 ? max(0, kv4_pos(x.kv, x.n_new, 0) - a.window + 1) & ~31 : 0;
     x.tiles = (x.rows + BR - 1) / BR;
     return x;
   }

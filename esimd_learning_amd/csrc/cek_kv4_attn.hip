@@ -174,11 +174,11 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
     real[i] = rr < w.rows;
     const int t = rr / a.group, h = kvh * a.group + rr % a.group;
     qsrc[i] = a.q + (int64_t)(w.q0 + (real[i] ? t : 0)) * a.q_stride + (int64_t)(real[i] ? h : 0) * HD;
-    pos[i] = real[i] ? w.kv - w.n_new + t : INT32_MAX - 1;
+    pos[i] = real[i] ? kv4_pos(w.kv, w.n_new, t) : INT32_MAX - 1;
     if (row0 + i * RT < w.rows) {
       // uniform: rows are in order of position
-      pmin = uniform(min(pmin, w.kv - w.n_new + (row0 + i * RT) / a.group));
-      pmax = uniform(max(pmax, w.kv - w.n_new + (min(row0 + i * RT + RT, w.rows) - 1) / a.group));
+      pmin = uniform(min(pmin, kv4_pos(w.kv, w.n_new, (row0 + i * RT) / a.group)));
+      pmax = uniform(max(pmax, kv4_pos(w.kv, w.n_new, (min(row0 + i * RT + RT, w.rows) - 1) / a.group)));
     }
   }
   const int window = a.window > 0 ? a.window : INT32_MAX;  // pos - window stays in range

@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
   int pos[QT];          // position of the row; padding rows see everything
   const uint16_t* qsrc[QT];
   bool real[QT];
-  auto pos_of = [&](int rr) { return w.kv - w.n_new + rr / a.group; };
+  auto pos_of = [&](int rr) { return kv4_pos(w.kv, w.n_new, rr / a.group); };
   const int tile_end = min(w.rows, (w.tile + 1) * BR), wave_end = min(tile_end, row0 + QT * 16);
   const int pmin = uniform(row0 < w.rows ? pos_of(row0) : INT32_MAX - 1), pmax = uniform(row0 < w.rows ? pos_of(wave_end - 1) : -1);
 #pragma unroll
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
     real[i] = rr < w.rows;
     const int t = rr / a.group, h = kvh * a.group + rr % a.group;
     qsrc[i] = a.q + (int64_t)(w.q0 + (real[i] ? t : 0)) * a.q_stride + (int64_t)(real[i] ? h : 0) * HD;
-    pos[i] = real[i] ? w.kv - w.n_new + t : INT32_MAX - 1;
+    pos[i] = real[i] ? kv4_pos(w.kv, w.n_new, t) : INT32_MAX - 1;
   }
   const int window = a.window > 0 ? a.window : INT32_MAX;  // pos - window stays in range
   const int first_pos = uniform(pos_of(w.tile * BR)), last_pos = uniform(pos_of(tile_end - 1));

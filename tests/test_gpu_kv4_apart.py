@@ -176,3 +176,17 @@ def test_parts_whose_keys_are_all_nan(ops, dev):
             ops.esimd_kv4_cache_write(nan, one, b.cache, _slots(b, 0, first, 128))
             for h in (dict(mq=rows), dict(mq=0, mk=0), dict(mq=1)):
                 assert b.run(ops, **h).isnan().all(), (first, h)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 8, 2 ** 30, 1])
+@pytest.mark.parametrize("nq,nk,hd", HEADS)
+def test_windows_beyond_everything(ops, dev, nq, nk, hd, window):
+    """Requests with fewer keys than new rows: the rows that have keys see them, up to the largest window there is."""
+    _say("windows", nq, nk, hd, window)
+    b = Batch([3, 40, 0, 1, 17], [10, 45, 4, 2, 17], nq, nk, hd, 16, torch.float16, dev, seed=nq + hd)
+    for h in HINTS:
+        out = b.run(ops, window=window, **h)
+        b.check(out, window)
+        assert (out[:7] == 0).all() and (out[55:60] == 0).all()
+        if window > 40:
+            assert torch.equal(out, b.run(ops, **h))
