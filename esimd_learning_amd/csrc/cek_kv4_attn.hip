@@ -828,6 +828,10 @@ void launch_attn(const AttnPlan& p, Kv4AttnArgs a, int64_t n_kv, int64_t n_q, hi
 extern "C" int64_t cek_kv4_attention_workspace_size(int64_t T, int64_t R, int64_t n_q, int64_t n_kv, int64_t hd,
                                                     int64_t max_q_len, int64_t max_kv_len) {
   if (T <= 0 || R <= 0 || n_kv <= 0 || n_q <= 0 || n_q % n_kv || (hd != 64 && hd != 128 && hd != 256)) return 0;
+  // sizes that the call refuses
+  if (T > INT32_MAX || n_q > 65535 || n_kv > 4096 || max_q_len < 0 || max_kv_len < 0 ||
+      T * (n_q / n_kv) > INT32_MAX / 4 || R > 1 << 26)
+    return 0;
   return attn_plan(T, R, n_q, n_kv, hd, max_q_len, max_kv_len).bytes;
 }
 
