@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import kv4
-from test_gpu_kv4 import Batch, _say
+from test_gpu_kv4 import EPS, Batch, _say
 
 pytestmark = pytest.mark.gpu
 
@@ -190,3 +190,33 @@ def test_windows_beyond_everything(ops, dev, nq, nk, hd, window):
         assert (out[:7] == 0).all() and (out[55:60] == 0).all()
         if window > 40:
             assert torch.equal(out, b.run(ops, **h))
+
+
+@pytest.mark.parametrize("hints", HINTS)
+@pytest.mark.parametrize("nq,nk,hd", HEADS)
+@pytest.mark.parametrize("far", [2.0 ** 14, 2.0 ** 24, 2.0 ** 80])
+def test_large_values_of_no_weight(ops, dev, nq, nk, hd, far, hints):
+    """Tokens with far larger values that a row sees, but hardly weighs: a weight times its step is rounded to 2^-34 of
+    the largest weight times the largest step at worst, which is beside tests/test_gpu_kv4.py's bound
+
+        n 2^-34 max_j p_j 2 max_j s_j 8
+
+    of n keys (the power of two above a step is at most twice it, and a code at most 8 from the products' zero)."""
+    _say("no weight", nq, nk, hd, far, hints)
+    b = Batch(LENS, QLENS, nq, nk, hd, 16, torch.bfloat16, dev, seed=nq + hd)
+    g = torch.Generator().manual_seed(3)
+    _set_q(b, (torch.ones_like(b.q.float()) + 0.1 * b.q.float()).bfloat16())
+    at = {0: (1, 60, 118), 1: (0, 20), 2: (50,), 3: (2,)}
+    for r, tokens in at.items():
+        for t in tokens:
+            _store(b, ops, r, t, k=torch.full((1, nk, hd), -60 / hd ** 0.5).bfloat16(),
+                   v=(torch.randn(1, nk, hd, generator=g) * far).bfloat16())
+    out = b.run(ops, **hints).cpu().double()
+    for r, n in enumerate(LENS):
+        a, z = b.cu[r], b.cu[r + 1]
+        one = torch.eye(n, dtype=torch.float64)[:, None].expand(-1, nk, -1)
+        ref, (spread, size, p) = kv4.attention(b.q[a:z], b.keys[r], b.vals[r], b.scale, weigh=(b.spread[r], b.vals[r].abs(), one))
+        step = b.spread[r].amax() / 7.5
+        tol = EPS[b.dtype] / 2 * ref.abs() + 2.0 ** -11 * spread + 2.0 ** -13 * size
+        tol = tol + n * 2.0 ** -34 * p.amax(-1, keepdim=True) * 2 * step * 8
+        assert ((out[a:z] - ref).abs() <= tol).all(), f"request {r}: {float(((out[a:z] - ref).abs() / tol).max()):.3g} tolerances"
