@@ -7,9 +7,10 @@
 // wave has 8, 4 or 2 tokens.  V's 16-bit accesses of neighbouring tokens meet in the
 // same cache lines.
 //
-// The write is bound by its arithmetic, about 18 vector operations a value: one row
-// of K or V a wave, so that some waves load while others compute (8000 rows of 8 x
-// 128 13.9 us; with four rows in flight a wave 16.0).  The read is bound by its 16-bit
+// The write takes its loads and its arithmetic, about 18 vector operations a value, half
+// of its time each and hardly at the same time: one row of K or V a wave, so that some
+// waves load while others compute (8000 rows of 8 x 128 14.3 us; with four rows in
+// flight a wave 16.0).  The read is bound by its 16-bit
 // rows, stored past the caches (32768 rows of 8 x 128 27.1 us, 6.3 TB/s; 42 us through
 // them): ROWS rows a wave in flight, four, or one where that leaves the GPU part
 // empty (8 rows 4.0 -> 2.5 us).

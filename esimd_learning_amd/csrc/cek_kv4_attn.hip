@@ -22,21 +22,24 @@
 // S^T = K Q^T (MFMA rows: tokens, columns: rows), so that a lane holds eight
 // weights of one row, which are -- without a shuffle, since the order within a
 // contraction is free -- the operand of O^T = V^T P^T; V's words hold four tokens
-// side by side for that.  Each code byte is read once, 1 KB a load instruction.
+// side by side for that.  Each tile of rows reads each code byte once, 1 KB a load
+// instruction; the tiles of one request read them again, from HBM or the L2.
 //
 // Weights: with M a running maximum of a row's exponents and 2^E above every sv that
-// the row has seen, P = exp2(x - M - E + 9) makes P sv at most 2^9 as it comes and 2^15 with
-// the 2^6 that a maximum may lag behind (it moves, and the sums are rescaled,
-// only where a score exceeds it by more): fp16 holds P sv to half a step (2^-12
-// of the value) down to 2^-23 of the largest.  Sums are fp32; sum(P sv) / 2 is
-// taken by an MFMA over the rounded weights, so that a weight's rounding acts
-// on v's distance from its centre alone.
+// the row has seen, P = exp2(x - M - E + 9) makes P sv at most 2^9 as it comes and
+// 2^15 with the 2^6 that a maximum may lag behind (it moves, and the sums are
+// rescaled, only where a score exceeds it by more): fp16 holds P sv to half a step
+// (2^-12 of the value) down to 2^-23 of the largest, and to 2^-34 of that below.
+// M, E and the power of two of q are the row's own and move for what it sees itself:
+// no other row, and no token that it does not see, changes its bits.  Sums are fp32;
+// sum(P sv) / 2 is taken by an MFMA over the rounded weights, so that a weight's
+// rounding acts on v's distance from its centre alone.
 //
 // What bounds it: the codes' bytes from HBM, and for short keys the latency of one
-// launch.  64 requests of 308 .. 16000 keys, 32 / 8 heads of 128, bf16: 56.4 us for
-// 288 MB (5.1 TB/s; a kernel that only reads them 40); one of 131071 keys 32.9 us
+// launch.  64 requests of 308 .. 16000 keys, 32 / 8 heads of 128, bf16: 57.8 us for
+// 288 MB (5.0 TB/s; a kernel that only reads them 40); one of 131071 keys 33.1 us
 // (143 MB; 20); 16 of 5 drafts on up to 6000 keys, window 4096, 16 heads of 256,
-// fp16: 43.6 us (174 MB; 24); one of 700 keys 10.2 us, of which 5 in the six tiles
+// fp16: 43.8 us (174 MB; 24); one of 700 keys 10.4 us, of which 5 in the six tiles
 // that each wave takes one after another.  What lies between: launch, work list,
 // table and first tiles before the loop, 5 us; the join's launch, 5; and workgroups
 // that end up to 10 us before the last one.
@@ -237,7 +240,7 @@ __global__ __launch_bounds__(256, attn_held(HD, QT)) void kv4_attn_kernel(Kv4Att
       const uint64_t at = (uint64_t)(uint32_t)(out ? 0 : x.b[h]) * (uint32_t)a.dm.block_stride;
       const auto src = kv4_rsrc(head + at, out ? 0 : head_bytes);
       const int tok = (t0 + 16 * h) & (bs - 1);
-      // (aux 2: not kept in the caches, since each code is read once)
+      // (aux 2: not kept in the caches, since a tile of rows reads each code once)
 #define CEK_FETCH(lane_off, dst, bytes, off) \
   __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_ptr_t)(dst), bytes, lane_off, off, 0, 2)
       // a part of 128 values and 16 tokens: 64 bytes of each K row, 256 of each four tokens of V
@@ -751,7 +754,10 @@ namespace {
 
 // What the host knows of a call: which kernels, their tiles, and whether the keys
 // are shared.  Requests with more than kAttnFewRows rows (query tokens x heads of a
-// kv head) go to the kernel whose waves have rows of their own.
+// kv head) go to the kernel whose waves have rows of their own.  16 requests of 4000
+// keys, bf16, us at 16 / 32 / 64 / 128 rows in this kernel and in that one: 8 kv heads
+// of 128, 29 / 36 / 53 / 90 and 62 / 64 / 69 / 80; 4 of 64, 20 / 24 / 30 / 42 and 31 /
+// 33 / 35 / 42; 4 of 256, 30 / 42 / 67 / 108 and 46 / 49 / 58 / 87.
 constexpr int kAttnFewRows = 64;
 constexpr int kAttnCus = 256;
 

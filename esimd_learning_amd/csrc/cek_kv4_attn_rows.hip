@@ -2,8 +2,8 @@
 // (prompt chunks), gfx950.  The mathematics is cek_kv4_attn.hip's.
 //
 // What bounds it: arithmetic.  Per 16 rows and 32 tokens the matrix products take
-// 272 cycles of a SIMD (17 MFMA), the softmax between them about 60 vector
-// operations and 8 exponentials, 330.  Unpacking codes and parameters (130 more)
+// 272 cycles of a SIMD (17 MFMA), the softmax between them about 70 vector
+// operations and 8 exponentials, 370.  Unpacking codes and parameters (130 more)
 // does not depend on the rows: a workgroup of four waves, each with QT x 16 rows of
 // its own, does it once for all of them.  The tokens come in stages of 64 (32 at head
 // size 256); the waves load a share of a stage's codes two stages ahead, unpack it
@@ -12,11 +12,14 @@
 // stage.  Two workgroups a CU: while one's waves are in the products the other's
 // may be in the softmax.
 //
-// Four chunks of 1900 tokens on 1900 .. 4100 keys, 32 / 8 heads of 128, fp16: 394 us,
-// 673 TFLOP/s.  Of a SIMD's cycles the matrix cores are busy 30%, vector instructions
-// 43% and exponentials 11%, and hardly at the same time: 84% together.  No gain came
-// from priorities for the products, from products and softmax of different rows
-// interleaved, from fewer maxima, nor from the next product's operands read ahead.
+// Four chunks of 1900 tokens on 1900 .. 4100 keys, 32 / 8 heads of 128, fp16: 415 us,
+// 639 TFLOP/s.  Of a SIMD's cycles the matrix cores are busy 27%, vector instructions
+// 48% and exponentials 10%, and hardly at the same time: 85% together.  (With one
+// power of two for all rows of a tile, which saves a multiplication a score but mixes
+// the rows' ranges, 394.)  No gain came from priorities for the products, from products
+// and softmax of different rows interleaved, from fewer maxima, nor from the next
+// product's operands read ahead; the largest step of 32 tokens found while unpacking,
+// once for all waves, cost 12 us.
 #include <type_traits>
 
 #include "cek_kv4_attn.h"
@@ -48,7 +51,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_rows_kernel(Kv4AttnArgs a) {
   const auto mine = list.request(lane);
   int u = wg, u_end = u + 1;
   if (a.wgs > 0) {
-    // (costs and leads made a chunk of 1000 on 4000 keys slower: 71 -> 73 .. 78 us)
+    // (costs and leads made a chunk of 1000 on 4000 keys slower, by 2 .. 7 us of 71)
     list.share(mine, list.unit_for(mine, a.wgs, 256, 512), 0);
     list.deal(a.wgs, 0);
     u = list.begin_of(wg);

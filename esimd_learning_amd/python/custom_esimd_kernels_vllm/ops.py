@@ -335,9 +335,14 @@ def esimd_kv4_attention(
     sees keys 0 .. p, with window > 0 keys p - window + 1 .. p; query head h
     reads kv head h / (n_q / n_kv).  out = sum softmax(scale q k) v; rows without
     a key (kv_lens 0) are zero; rows of out before cu_q[0] or behind cu_q[R] are
-    left as they were.  cu_q ascends; |q| up to 2^100.  Tokens whose table entry lies outside the cache count
-    as absent.  max_q_len and max_kv_len, the longest of the batch (0: not
-    known), choose the kernels; wrong ones cost time, not results."""
+    left as they were.  Tokens whose table entry lies outside the cache count
+    as absent.  cu_q ascends.  |q| and |v| up to 2^100, and V steps up to 2^9
+    where scores pass 2^22; weights times V steps are rounded to 2^-12 of
+    themselves, or 2^-34 of the largest that the row sees.  Other rows, finite or
+    not, and tokens that a row does not see leave it as it is.  max_q_len and
+    max_kv_len, the longest of the batch (0: not known), choose the kernels;
+    wrong ones cost time, and change results by that rounding and the order of
+    sums alone."""
     _ops.esimd_kv4_attention(q, kv_cache, block_tables, kv_lens, cu_q, out, scale, max_q_len, max_kv_len, window)
 
 

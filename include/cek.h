@@ -409,9 +409,12 @@ int cek_qk_norm_rope(void* q, void* k, const void* qw, const void* kw, const int
  * q rows, the last tokens of request r, over its kv_lens[r] cached tokens; the
  * row at position p sees keys 0 .. p (window > 0: p - window + 1 .. p).  Rows
  * without a key are zero, rows outside cu_q[0] .. cu_q[R] left as they were.
- * Tokens in blocks outside the cache count as absent.  cu_q ascends; |q| up to 2^100.  max_q_len and max_kv_len
- * (0: not known) choose the kernels and never change results beyond the order
- * of sums.  workspace: cek_kv4_attention_workspace_size bytes for the same
+ * Tokens in blocks outside the cache count as absent.  cu_q ascends.  |q| and |v|
+ * up to 2^100, and V steps up to 2^9 where scores pass 2^22; weights times V steps
+ * are rounded to 2^-12 of themselves, or 2^-34 of the largest that the row sees.
+ * Other rows, finite or not, and tokens that a row does not see leave it as it is.
+ * max_q_len and max_kv_len (0: not known) choose the kernels and never change
+ * results beyond that rounding and the order of sums.  workspace: cek_kv4_attention_workspace_size bytes for the same
  * arguments, 16-byte aligned, no initialisation; with less the call does not
  * split the keys.
  */
