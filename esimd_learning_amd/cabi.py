@@ -15,6 +15,7 @@ HEADER = PKG_DIR.parent / "include" / "cek.h"
 
 CEK_F16, CEK_BF16, CEK_F32 = 0, 1, 2
 CEK_E4M3, CEK_E5M2 = 0, 1
+CEK_GELU_TANH, CEK_SILU = 0, 1
 CEK_OK, CEK_ERR_INVALID, CEK_ERR_UNSUPPORTED, CEK_ERR_HIP, CEK_ERR_SCRATCH = 0, 1, 2, 3, 4
 
 _p, _i64, _i, _f = C.c_void_p, C.c_int64, C.c_int, C.c_float
@@ -64,6 +65,12 @@ SIGNATURES = {
     "cek_kv4_attention_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     "cek_kv4_attention": (_i, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                _i64, _f, _i64, _i64, _i64, _i, _p, _i64, _p]),
+    "cek_per_token_quant_int8": (_i, [_p, _i64, _i64, _i, _p, _p, _p]),
+    "cek_fused_add_rms_norm_quant_int8": (_i, [_p, _p, _p, _i64, _i64, _f, _i, _p, _p, _p]),
+    "cek_gemm_int8_a8w8_workspace_size": (_i64, [_i64, _i64, _i64]),
+    "cek_gemm_int8_a8w8": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p, _i64, _p]),
+    "cek_gemm_int8_a8w8_glu_workspace_size": (_i64, [_i64, _i64, _i64]),
+    "cek_gemm_int8_a8w8_glu": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _i, _p, _i64, _p]),
     "cek_hbm_read_probe": (_i, [_p, _i64, _p, _p]),
 }
 

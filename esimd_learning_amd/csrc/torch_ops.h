@@ -93,3 +93,11 @@ at::Tensor esimd_gemm_fp8_a8w8(at::Tensor a, at::Tensor a_scale, at::Tensor b, a
 // The a8w8 form of esimd_gemv_fp8_gelu_and_mul (e4m3 activations and weights).
 void esimd_gemm_fp8_a8w8_gelu_and_mul(at::Tensor a, at::Tensor a_scale, at::Tensor b, at::Tensor b_scale,
                                       at::Tensor output);
+
+// The int8 path (cek_int8.h).
+void esimd_per_token_quant_int8(at::Tensor input, at::Tensor out_q, at::Tensor out_scale);
+void esimd_fused_add_rms_norm_quant_int8(at::Tensor hidden_states, at::Tensor residual, at::Tensor weight, double eps,
+                                         at::Tensor out_q, at::Tensor out_scale);
+at::Tensor esimd_gemm_int8_a8w8(at::Tensor a, at::Tensor a_scale, at::Tensor b, at::Tensor b_scale, at::Tensor output);
+void esimd_gemm_int8_a8w8_glu(at::Tensor a, at::Tensor a_scale, at::Tensor b, at::Tensor b_scale, at::Tensor output,
+                              c10::string_view activation);

@@ -42,4 +42,8 @@ from custom_esimd_kernels_vllm.ops import (  # noqa: F401
     esimd_kv4_attention,
     esimd_gemm_fp8_a8w8,
     esimd_gemm_fp8_a8w8_gelu_and_mul,
+    esimd_per_token_quant_int8,
+    esimd_fused_add_rms_norm_quant_int8,
+    esimd_gemm_int8_a8w8,
+    esimd_gemm_int8_a8w8_glu,
 )

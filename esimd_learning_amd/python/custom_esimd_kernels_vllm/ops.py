@@ -361,3 +361,50 @@ def esimd_gemm_fp8_a8w8_gelu_and_mul(
     """esimd_gemm_fp8_a8w8 over a merged [2d, K] gate/up weight, then
     gelu_and_mul, fused for M <= 16: output [M, d]."""
     _ops.esimd_gemm_fp8_a8w8_gelu_and_mul(a, a_scale, b, b_scale, output)
+
+
+# ---- the int8 path ---------------------------------------------------------
+
+def esimd_per_token_quant_int8(input: torch.Tensor, out_q: torch.Tensor, out_scale: torch.Tensor) -> None:
+    """int8 codes and one fp32 scale of each row of input [..., H] (fp16 or bf16).
+
+    out_scale[t] = max(amax_t / 127, 2^-126); out_q = input / out_scale[t] to the
+    nearest integer, ties to even.  Takes activations (a row per token) and, when a
+    model is loaded, an [N, K] weight (a row per output channel).  A row with a
+    value that is not finite gets scale NaN and codes 0: its products are NaN."""
+    _ops.esimd_per_token_quant_int8(input, out_q, out_scale)
+
+
+def esimd_fused_add_rms_norm_quant_int8(
+    hidden_states: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float,
+    out_q: torch.Tensor, out_scale: torch.Tensor,
+) -> None:
+    """residual += hidden_states (in place); int8 codes and scales of
+    rmsnorm(residual) * weight into out_q [T, H] and out_scale [T], as
+    esimd_per_token_quant_int8 of the normed rows before any rounding to 16
+    bits.  hidden_states is only read."""
+    _ops.esimd_fused_add_rms_norm_quant_int8(hidden_states, residual, weight, eps, out_q, out_scale)
+
+
+def esimd_gemm_int8_a8w8(
+    a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+    output: torch.Tensor,
+) -> torch.Tensor:
+    """output[m, n] = (sum_k a[m, k] * b[n, k]) * b_scale[n] * a_scale[m], the sum exact.
+
+    a [M, K], b [N, K] int8, scales fp32 [M] and [N], output [M, N] fp16 or bf16.
+    Any M (decode steps stream the weights, prompts run MFMA tiles) and N, K a
+    multiple of 16 up to 131071.  A row of the output does not depend on the others,
+    on M or on the kernel that served the call.  Returns ``output``."""
+    return _ops.esimd_gemm_int8_a8w8(a, a_scale, b, b_scale, output)
+
+
+def esimd_gemm_int8_a8w8_glu(
+    a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+    output: torch.Tensor, activation: str = "gelu_tanh",
+) -> None:
+    """The gated block in one launch: output[m, i] = act(g) * u, g and u the fp32
+    values that esimd_gemm_int8_a8w8 has for rows i and d + i of b [2d, K] (gate rows, then
+    up rows), not rounded before the product.  activation: "gelu_tanh" or
+    "silu"; output [M, d] fp16 or bf16."""
+    _ops.esimd_gemm_int8_a8w8_glu(a, a_scale, b, b_scale, output, activation)

@@ -63,7 +63,7 @@ setup(
     package_data={"custom_esimd_kernels_vllm": ["libcek.so"]},
     ext_modules=[
         ext("custom_esimd_kernels", ["esimd_kernel.cpp", "esimd_kernel_kv.cpp", "torch_extension.cpp"]),
-        ext("custom_esimd_kernels_gemm", ["esimd_kernel_gemm.cpp", "torch_extension_gemm.cpp"]),
+        ext("custom_esimd_kernels_gemm", ["esimd_kernel_gemm.cpp", "esimd_kernel_int8.cpp", "torch_extension_gemm.cpp"]),
     ],
     cmdclass={"build_ext": BuildWithCabi.with_options(use_ninja=True)},
 )

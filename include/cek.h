@@ -30,6 +30,8 @@ extern "C" {
 enum cek_dtype { CEK_F16 = 0, CEK_BF16 = 1, CEK_F32 = 2 };
 /* fp8 weight encodings (reference get_fp8_mode, csrc/xpu/esimd_kernel.sycl:14-16) */
 enum cek_fp8 { CEK_E4M3 = 0, CEK_E5M2 = 1 };
+/* the gate's activation in a gated block */
+enum cek_act { CEK_GELU_TANH = 0, CEK_SILU = 1 };
 
 enum cek_status {
   CEK_OK = 0,
@@ -441,6 +443,47 @@ int cek_kv4_attention(const void* q, const void* cache, const int32_t* block_tab
                       int64_t block_size, int64_t num_blocks, int64_t q_stride, int64_t out_stride, int64_t block_stride,
                       int64_t table_stride, int64_t max_blocks, float scale, int64_t max_q_len, int64_t max_kv_len,
                       int64_t window, int io_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The int8 path (NEW, all of it): activations and weights as int8 codes with one
+ * fp32 scale per row (per token; per output channel), the value code * scale.
+ *
+ * cek_per_token_quant_int8: scale[t] = max(amax_t / 127, 2^-126), q[t, i] =
+ * x[t, i] / scale[t] rounded to the nearest integer, ties to even (of the exact
+ * quotient).  A row with a value that is not finite has scale NaN and codes 0.
+ * Any rows and H (x and q 16-byte aligned and H % 8 == 0 are faster).  The rows of
+ * an [N, K] weight quantise the same way, a scale per output channel.
+ *
+ * cek_fused_add_rms_norm_quant_int8: residual = Out(hidden + residual) in place,
+ * then the codes and scales of residual * rsqrt(mean((hidden + residual)^2) + eps) *
+ * weight, which is not rounded to 16 bits before (cek_fused_add_rms_norm_quant_fp8
+ * rounds it).  hidden is only read.
+ *
+ * cek_gemm_int8_a8w8: y[m, n] = Out((f32(sum_k a[m, k] b[n, k]) * sb[n]) * sa[m]),
+ * the sum exact in int32.  a [M, K], b [N, K] int8 row-major, sa [M], sb [N], y [M, N]
+ * out_dtype (F16|BF16).  Any M and N, K a multiple of 16 up to 131071, a and b
+ * 16-byte aligned; the same values bit for bit whatever M, workspace or kernel.
+ *
+ * cek_gemm_int8_a8w8_glu: b [2d, K], gate rows, then up rows, sb [2d], y [M, d]:
+ *   y[m, i] = Out(act(g) * u), g, u = the fp32 values above of b's rows i and d + i
+ * (not rounded between), act CEK_GELU_TANH (0.5 g (1 + tanh(sqrt(2/pi) (g + 0.044715
+ * g^3)))) or CEK_SILU (g / (1 + exp(-g))).
+ *
+ * y shares no memory with the operands.  workspace: the bytes that the
+ * _workspace_size of the same sizes gives (0: none needed), 16-byte aligned, no
+ * initialisation; with less (or none) the call does not split K.  Calls that may
+ * overlap in time need their own.
+ */
+int cek_per_token_quant_int8(const void* x, int64_t rows, int64_t H, int io_dtype, int8_t* q, float* scale, void* stream);
+int cek_fused_add_rms_norm_quant_int8(const void* hidden, void* residual, const void* weight, int64_t rows, int64_t H,
+                                      float eps, int io_dtype, int8_t* q, float* scale, void* stream);
+int64_t cek_gemm_int8_a8w8_workspace_size(int64_t M, int64_t N, int64_t K);
+int cek_gemm_int8_a8w8(const int8_t* a, const float* sa, const int8_t* b, const float* sb, void* y, int64_t M, int64_t N,
+                       int64_t K, int out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t cek_gemm_int8_a8w8_glu_workspace_size(int64_t M, int64_t d, int64_t K);
+int cek_gemm_int8_a8w8_glu(const int8_t* a, const float* sa, const int8_t* b, const float* sb, void* y, int64_t M,
+                           int64_t d, int64_t K, int activation, int out_dtype, void* workspace, int64_t workspace_bytes,
+                           void* stream);
 
 /*
  * Measurement utility, no counterpart in the reference: reads `bytes` bytes
