@@ -90,6 +90,13 @@ __device__ inline float int8_glu(int ag, int au, float sa, float sg, float su) {
   return f32_round(int8_act<ACT>(int8_scaled(ag, sa, sg)) * int8_scaled(au, sa, su));
 }
 
+// Two values to 16 bits, each rounded once (the compiler's packed conversion where the
+// type has one).
+template <typename T>
+__device__ inline uint32_t int8_pack2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, typename T::pair));
+}
+
 template <typename T>
 __device__ inline float unit_f32(u4 v, int e) { return T::to_f32((uint16_t)((e & 1) ? v[e >> 1] >> 16 : v[e >> 1] & 0xFFFF)); }
 

@@ -2,47 +2,142 @@
 // output channel, and the gated block over a merged gate/up matrix, gfx950:
 //   y[m, n] = Out((f32(sum_k a[m, k] b[n, k]) sb[n]) sa[m])
 //   y[m, i] = Out(act(g) u), g and u such values of b's rows i and d + i, unrounded
-#include "cek_int8.h"
+#include "cek_int8_tile.h"
+#include "cek_segs.h"
 
 namespace cek {
 
-// One 16 x 16 block of outputs per wave, operands straight from memory: 64 rows of
-// a and 16 of b per workgroup.  Rows past the end repeat the last one, K values
-// past the row are zeros.
-template <typename T, int ACT>  // ACT < 0: the plain product
-__global__ __launch_bounds__(256) void int8_simple_kernel(const uint8_t* __restrict__ a, const float* __restrict__ sa,
-                                                          const uint8_t* __restrict__ b, const float* __restrict__ sb,
-                                                          uint16_t* __restrict__ y, int M, int N, int K) {
+// Split K: y from the parts' int32 sums [parts][M][NB] (NB = N, or 2 N for the gated
+// block), added as integers: what one part would have given, bit for bit.  Four
+// outputs of a row per thread.
+template <typename T, int ACT>
+__global__ __launch_bounds__(256) void int8_join_kernel(const int32_t* __restrict__ P, const float* __restrict__ sa,
+                                                        const float* __restrict__ sb, uint16_t* __restrict__ y, int M,
+                                                        int N, int parts) {
   constexpr bool GLU = ACT >= 0;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
-  const int n = blockIdx.x * 16 + r16, m0 = blockIdx.y * 64 + wave * 16;
-  const uint8_t* pa = a + (size_t)min(m0 + r16, M - 1) * K;
-  const uint8_t* pb = b + (size_t)min(n, N - 1) * K;
-  const uint8_t* pu = pb + (size_t)(GLU ? N : 0) * K;
-  i4 acc{0, 0, 0, 0}, acu{0, 0, 0, 0};
-  for (int k = 16 * g; k < ((K + 63) & ~63); k += 64) {
-    const bool in = k < K;
-    const u4 z{0, 0, 0, 0};
-    const u4 av = in ? load_u4(pa + k) : z, bv = in ? load_u4(pb + k) : z;
-    acc = mfma_i8(av, bv, acc);
-    if constexpr (GLU) acu = mfma_i8(av, in ? load_u4(pu + k) : z, acu);
-  }
-  if (n >= N) return;
-  const float s0 = sb[n], s1 = GLU ? sb[N + n] : 0.f;
+  const uint32_t quads = (uint32_t)(N + 3) / 4, q = blockIdx.x * 256 + threadIdx.x;
+  const int m = (int)(q / quads), n = (int)(q % quads) * 4;
+  if (m >= M) return;
+  const size_t NB = GLU ? 2 * (size_t)N : N, step = NB * M;
+  const int32_t* p = P + m * NB + n;
+  const float s0 = sa[m];
+  if ((N & 3) == 0 && (reinterpret_cast<uintptr_t>(y) & 7) == 0 && (reinterpret_cast<uintptr_t>(sb) & 15) == 0) {
+    i4 g{0, 0, 0, 0}, u{0, 0, 0, 0};
+    for (int k = 0; k < parts; ++k, p += step) {
+      g += *reinterpret_cast<const i4*>(p);
+      if constexpr (GLU) u += *reinterpret_cast<const i4*>(p + N);
+    }
+    const f4 sg = *reinterpret_cast<const f4*>(sb + n);
+    f4 su = sg;
+    if constexpr (GLU) su = *reinterpret_cast<const f4*>(sb + N + n);
+    float o[4];
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    const int m = m0 + 4 * g + v;
-    if (m >= M) continue;
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (GLU) o[e] = int8_glu<ACT>(g[e], u[e], s0, sg[e], su[e]);
+      else o[e] = int8_scaled(g[e], s0, sg[e]);
+    }
+    *reinterpret_cast<uint2*>(y + (size_t)m * N + n) = make_uint2(int8_pack2<T>(o[0], o[1]), int8_pack2<T>(o[2], o[3]));
+    return;
+  }
+  for (int e = 0; e < 4 && n + e < N; ++e) {
+    int g = 0, u = 0;
+    for (int k = 0; k < parts; ++k) {
+      g += p[k * step + e];
+      if constexpr (GLU) u += p[k * step + N + e];
+    }
     float o;
-    if constexpr (GLU) o = int8_glu<ACT>(acc[v], acu[v], sa[m], s0, s1);
-    else o = int8_scaled(acc[v], sa[m], s0);
-    y[(size_t)m * N + n] = T::from_f32(o);
+    if constexpr (GLU) o = int8_glu<ACT>(g, u, s0, sb[n + e], sb[(size_t)N + n + e]);
+    else o = int8_scaled(g, s0, sb[n + e]);
+    y[(size_t)m * N + n + e] = T::from_f32(o);
   }
 }
 
+// ---- which tile, how many parts of K -----------------------------------------
+// Time of a launch: rounds of 256 workgroups (one per CU), each a fixed part and a
+// time per 128 values of K; a last round of fewer workgroups runs between the times
+// of a nearly empty and a full chip.  Split K adds the join and its traffic.  Fitted
+// to 1100 launches over 35 shapes of 65 to 8192 rows (weights from HBM): 10% off on
+// average, and the pick 0.6% above the fastest of all tiles and splits (geometric
+// mean; 12% at worst).  Larger tiles move fewer operand bytes per product, smaller
+// ones fill the chip sooner.
+struct Int8Opt {
+  int bm, bn;
+  double fixed, step, fixed0, step0;  // us: a full round, and one with few workgroups
+};
+constexpr Int8Opt kInt8Opts[] = {
+    {256, 256, 5.19, 1.582, 8.66, 0.957}, {256, 192, 5.12, 1.316, 7.24, 0.751}, {256, 128, 5.78, 0.823, 4.75, 0.589},
+    {128, 256, 5.90, 0.821, 5.30, 0.560}, {128, 192, 5.24, 0.772, 5.19, 0.434}, {128, 128, 4.59, 0.613, 4.78, 0.308},
+    {64, 256, 4.31, 0.694, 4.64, 0.338},  {64, 128, 4.45, 0.384, 2.76, 0.291}};
+constexpr int kInt8Tiles = sizeof(kInt8Opts) / sizeof(kInt8Opts[0]);
+constexpr int kInt8Parts[] = {1, 2, 3, 4, 6, 8, 12};
+constexpr int64_t kInt8MaxWorkspace = int64_t(1) << 28;
+
+static double int8_us(const Int8Opt& o, int64_t M, int64_t NB, int64_t steps, int parts) {
+  const int64_t n = (M + o.bm - 1) / o.bm * ((NB + o.bn - 1) / o.bn) * parts, full = n / kCUs, rest = n % kCUs;
+  const double s = (double)((steps + parts - 1) / parts), f = (double)rest / kCUs;
+  constexpr double kStart = 2.07;  // of a round's fixed part, what only the first one takes
+  double t = kStart + (double)full * (o.fixed - kStart + s * o.step);
+  if (rest) t += o.fixed0 + (o.fixed - o.fixed0) * f - kStart + s * (o.step0 + (o.step - o.step0) * f);
+  if (parts > 1) t += 3.15 + 3.35e-7 * 4.0 * (double)parts * (double)M * (double)NB;
+  return t;
+}
+
+struct Int8Plan {
+  int cfg, parts;
+};
+// NB: rows of b.
+static int64_t int8_parts_bytes(int parts, int64_t M, int64_t NB) {
+  return parts > 1 ? ((int64_t)parts * M * NB * 4 + 15) / 16 * 16 : 0;
+}
+static Int8Plan int8_plan(int64_t M, int64_t NB, int64_t K, int64_t ws_bytes) {
+  Int8Plan best{0, 1};
+  double us = 0;
+  const int64_t steps = (K + 127) / 128;
+  for (int c = 0; c < kInt8Tiles; ++c)
+    for (int parts : kInt8Parts) {
+      if (parts > 1 && (steps < 4 * parts || (double)M * (double)NB * 4 * parts > (double)kInt8MaxWorkspace ||
+                        int8_parts_bytes(parts, M, NB) > ws_bytes))
+        break;
+      const double t = int8_us(kInt8Opts[c], M, NB, steps, parts);
+      if ((c == 0 && parts == 1) || t < us) {
+        us = t;
+        best = Int8Plan{c, parts};
+      }
+    }
+  return best;
+}
+
+static bool int8_sizes_ok(int64_t M, int64_t N, int64_t K, int64_t NB) {
+  return M >= 0 && N >= 0 && K > 0 && K % 16 == 0 && K <= kInt8MaxK && M <= (1 << 24) && N <= INT32_MAX && NB <= INT32_MAX;
+}
+static int64_t int8_workspace(int64_t M, int64_t N, int64_t K, bool glu) {
+  if (N > INT32_MAX || !int8_sizes_ok(M, N, K, glu ? 2 * N : N) || M == 0 || N == 0) return 0;
+  const int64_t NB = glu ? 2 * N : N;
+  return int8_parts_bytes(int8_plan(M, NB, K, INT64_MAX).parts, M, NB);
+}
+
+template <class C, class T, int ACT>
+static int launch_int8_tile(Int8Args& g, hipStream_t st) {
+  g.tiles_m = (g.M + C::BM - 1) / C::BM;
+  g.tiles_n = (g.N + C::BO - 1) / C::BO;
+  const int64_t n = (int64_t)g.tiles_m * g.tiles_n * g.parts;
+  if (n > INT32_MAX / C::NT) return CEK_ERR_UNSUPPORTED;
+  if (g.parts == 1) {
+    int8_tile_kernel<C, T, ACT, false><<<(unsigned)n, C::NT, 0, st>>>(g);
+    return check_launch();
+  }
+  int8_tile_kernel<C, T, ACT, true><<<(unsigned)n, C::NT, 0, st>>>(g);
+  const int rc = check_launch();
+  if (rc != CEK_OK) return rc;
+  // (a workspace of at most 2^28 bytes: M is below 2^26 / N / parts)
+  int8_join_kernel<T, ACT><<<(unsigned)(((int64_t)g.M * ((g.N + 3) / 4) + 255) / 256), 256, 0, st>>>(g.part, g.sa, g.sb, g.y,
+                                                                                                     g.M, g.N, g.parts);
+  return check_launch();
+}
+
 static int int8_args(const void* a, const void* sa, const void* b, const void* sb, const void* y, int64_t M, int64_t N,
-                     int64_t K, int64_t rows_b, int out_dtype, const void* ws, int64_t ws_bytes) {
-  if (M < 0 || N < 0 || K <= 0 || K % 16 != 0 || K > kInt8MaxK || M > (1 << 24) || rows_b > INT32_MAX) return CEK_ERR_INVALID;
+                     int64_t K, int64_t NB, int out_dtype, const void* ws, int64_t ws_bytes) {
+  if (!int8_sizes_ok(M, N, K, NB)) return CEK_ERR_INVALID;
   if (ws_bytes < 0 || (ws && !aligned(ws, 16))) return CEK_ERR_INVALID;
   if (out_dtype != CEK_F16 && out_dtype != CEK_BF16) return CEK_ERR_INVALID;
   if (M == 0 || N == 0) return CEK_OK;
@@ -52,29 +147,47 @@ static int int8_args(const void* a, const void* sa, const void* b, const void* s
   return CEK_OK;
 }
 
+template <class T, int ACT>
+static int launch_int8_t(Int8Args& g, int cfg, hipStream_t st) {
+  constexpr bool G = ACT >= 0;
+  switch (cfg) {
+    case 0: return launch_int8_tile<Int8Tile<256, 256, 2, 4, 4, 2, G>, T, ACT>(g, st);
+    case 1: return launch_int8_tile<Int8Tile<256, 192, 4, 2, 4, 2, G>, T, ACT>(g, st);
+    case 2: return launch_int8_tile<Int8Tile<256, 128, 4, 2, 4, 3, G>, T, ACT>(g, st);
+    case 3: return launch_int8_tile<Int8Tile<128, 256, 2, 4, 4, 3, G>, T, ACT>(g, st);
+    case 4: return launch_int8_tile<Int8Tile<128, 192, 4, 2, 4, 3, G>, T, ACT>(g, st);
+    case 5: return launch_int8_tile<Int8Tile<128, 128, 2, 4, 4, 4, G>, T, ACT>(g, st);
+    case 6: return launch_int8_tile<Int8Tile<64, 256, 2, 4, 4, 3, G>, T, ACT>(g, st);
+    case 7: return launch_int8_tile<Int8Tile<64, 128, 2, 4, 4, 5, G>, T, ACT>(g, st);
+    default: return CEK_ERR_UNSUPPORTED;
+  }
+}
+
 template <int ACT>
 static int launch_int8(const int8_t* a, const float* sa, const int8_t* b, const float* sb, void* y, int64_t M, int64_t N,
                        int64_t K, int out_dtype, void* ws, int64_t ws_bytes, hipStream_t st) {
-  const uint8_t* ap = reinterpret_cast<const uint8_t*>(a);
-  const uint8_t* bp = reinterpret_cast<const uint8_t*>(b);
-  uint16_t* yp = static_cast<uint16_t*>(y);
-  for (int64_t m = 0; m < M; m += 65535 * 64) {
-    const int rows = (int)(M - m < 65535 * 64 ? M - m : 65535 * 64);
-    const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((rows + 63) / 64));
-    if (out_dtype == CEK_F16)
-      int8_simple_kernel<F16, ACT><<<grid, 256, 0, st>>>(ap + m * K, sa + m, bp, sb, yp + m * N, rows, (int)N, (int)K);
-    else
-      int8_simple_kernel<BF16, ACT><<<grid, 256, 0, st>>>(ap + m * K, sa + m, bp, sb, yp + m * N, rows, (int)N, (int)K);
-  }
-  return check_launch();
+  const Int8Plan p = int8_plan(M, ACT >= 0 ? 2 * N : N, K, ws ? ws_bytes : 0);
+  Int8Args g{reinterpret_cast<const uint8_t*>(a), sa, reinterpret_cast<const uint8_t*>(b), sb, static_cast<uint16_t*>(y),
+             static_cast<int32_t*>(ws), (int)M, (int)N, (int)K, 0, 0, p.parts};
+  return out_dtype == CEK_F16 ? launch_int8_t<F16, ACT>(g, p.cfg, st) : launch_int8_t<BF16, ACT>(g, p.cfg, st);
 }
 
 }  // namespace cek
 
 using namespace cek;
 
-extern "C" int64_t cek_gemm_int8_a8w8_workspace_size(int64_t M, int64_t N, int64_t K) { return 0; }
-extern "C" int64_t cek_gemm_int8_a8w8_glu_workspace_size(int64_t M, int64_t d, int64_t K) { return 0; }
+extern "C" int64_t cek_gemm_int8_a8w8_workspace_size(int64_t M, int64_t N, int64_t K) {
+  return int8_workspace(M, N, K, false);
+}
+extern "C" int64_t cek_gemm_int8_a8w8_glu_workspace_size(int64_t M, int64_t d, int64_t K) {
+  return int8_workspace(M, d, K, true);
+}
+
+extern "C" int cek_gemm_int8_plan(int64_t M, int64_t rows_b, int64_t K, int64_t workspace_bytes) {
+  if (!int8_sizes_ok(M, rows_b, K, rows_b) || M == 0 || rows_b == 0) return -1;
+  const Int8Plan p = int8_plan(M, rows_b, K, workspace_bytes);
+  return 16 * p.cfg + p.parts;
+}
 
 extern "C" int cek_gemm_int8_a8w8(const int8_t* a, const float* sa, const int8_t* b, const float* sb, void* y, int64_t M,
                                   int64_t N, int64_t K, int out_dtype, void* workspace, int64_t workspace_bytes,
@@ -88,7 +201,7 @@ extern "C" int cek_gemm_int8_a8w8_glu(const int8_t* a, const float* sa, const in
                                       int64_t M, int64_t d, int64_t K, int activation, int out_dtype, void* workspace,
                                       int64_t workspace_bytes, void* stream) {
   if (activation != CEK_GELU_TANH && activation != CEK_SILU) return CEK_ERR_INVALID;
-  if (d > INT32_MAX / 2) return CEK_ERR_INVALID;
+  if (d > INT32_MAX) return CEK_ERR_INVALID;
   const int rc = int8_args(a, sa, b, sb, y, M, d, K, 2 * d, out_dtype, workspace, workspace_bytes);
   if (rc != CEK_OK || M == 0 || d == 0) return rc;
   return activation == CEK_SILU ? launch_int8<CEK_SILU>(a, sa, b, sb, y, M, d, K, out_dtype, workspace, workspace_bytes,

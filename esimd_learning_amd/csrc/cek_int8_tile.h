@@ -1,0 +1,278 @@
+// cek_int8_tile.h -- the tiled int8 product (and gated block), gfx950.
+#pragma once
+
+#include "cek_int8.h"
+
+namespace cek {
+
+typedef int i16v __attribute__((ext_vector_type(16)));
+
+template <int BM_, int BN_, int WM_, int WN_, int LW_, int RING_, bool GLU_>
+struct Int8Tile {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, RING = RING_, BK = 128;
+  static constexpr bool GLU = GLU_;
+  static constexpr int BO = GLU ? BN / 2 : BN;              // output columns
+  static constexpr int NW = WM * WN, NT = 64 * NW;
+  static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+  static constexpr int ASLOT = BM * BK, BSLOT = BN * BK, SLOT = ASLOT + BSLOT;
+  static constexpr int LW = LW_;                            // waves that load
+  static constexpr int AL = BM / 8 / LW, BL = BN / 8 / LW, L = AL + BL;  // 1 KB loads per such wave and step
+  static constexpr int L3 = RING == 2 ? L : (L + 3) / 4;    // of them, in the slice behind the barrier
+  static constexpr int RA = (BM + 63) / 64 * 64, RO = (BO + 63) / 64 * 64;  // scale regions
+  static constexpr int NSC = RA + (GLU ? 2 : 1) * RO;
+  static constexpr int OUT = BM * BO * 2;
+  static constexpr int MAIN = RING * SLOT > OUT ? RING * SLOT : OUT;
+  static constexpr int SMEM = MAIN + NSC * 4;
+  static constexpr int GROUPS = FM * FN;                     // MFMAs of a slice
+  static constexpr int RPG = (2 * (FM + FN) + GROUPS - 1) / GROUPS;  // fragments read beside a MFMA: all in the slice's first half
+  static constexpr int SW = (BO / 4) % 16 == 0 ? 15 : 7;     // swizzle of the staged output's 8-byte units
+  // first output column of accumulator quad q of block column j (lanes of h = 1 hold the next four)
+  static constexpr __device__ int col(int wn, int j, int q) {
+    return GLU ? wn * (TN / 2) + 16 * j + 8 * (q >> 1) : wn * TN + 32 * j + 8 * q;
+  }
+  static_assert(FM * 32 * WM == BM && FN * 32 * WN == BN && AL * 8 * LW == BM && BL * 8 * LW == BN, "tile");
+  static_assert(!GLU || LW % 2 == 0, "a wave loads gate rows or up rows");
+  static_assert((BO / 4) % 8 == 0 && SMEM <= 163840, "LDS");
+};
+
+__device__ inline i16v mfma32_i8(u4 a, u4 b, i16v c) {
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i4, a), __builtin_bit_cast(i4, b), c, 0, 0, 0);
+}
+
+template <int N>
+__device__ __forceinline__ void tile_barrier() {  // all but the N latest loads have landed, LDS reads are done
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+__device__ inline __amdgpu_buffer_rsrc_t int8_rsrc(const void* p, uint32_t n) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)n, 0x00020000);
+}
+
+constexpr uint32_t kOutOfRange = 0x80000000u;  // an offset beyond every resource here: the load gives zeros
+
+// Tile and part of workgroup b of n: runs of n / 8 consecutive ones per XCD (workgroup
+// b is on XCD b % 8), in groups of GM tile rows.
+template <int GM>
+__device__ inline void int8_tile_of(int b, int n, int tiles_m, int tiles_n, int& tm, int& tn, int& part) {
+  const int x = b & 7, lo = n >> 3, more = n & 7;
+  const int t = x * lo + min(x, more) + (b >> 3), per = tiles_m * tiles_n;
+  part = t / per;
+  const int q = t - part * per, per_group = GM * tiles_n, group = q / per_group;
+  const int first = group * GM, rows = min(tiles_m - first, GM), in = q - group * per_group;
+  tm = first + in % rows;
+  tn = in / rows;
+}
+
+struct Int8Args {
+  const uint8_t* a;
+  const float* sa;
+  const uint8_t* b;
+  const float* sb;
+  uint16_t* y;
+  int32_t* part;  // split K: int32 sums [parts][M][rows of b]
+  int M, N, K;    // N: output columns
+  int tiles_m, tiles_n, parts;
+};
+
+template <class C, class T, int ACT, bool SPLIT>
+__global__ __launch_bounds__(C::NT, 1) void int8_tile_kernel(Int8Args p) {
+  constexpr int FM = C::FM, FN = C::FN, L = C::L, RING = C::RING;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[C::SMEM];
+  float* const sc = reinterpret_cast<float*>(smem + C::MAIN);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int wm = wave / C::WN, wn = wave % C::WN;
+  int tm, tn, part;
+  int8_tile_of<4>(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, tm, tn, part);
+  const int K = p.K, m0 = tm * C::BM, n0 = tn * C::BO;
+  const int rows_m = min(C::BM, p.M - m0), rows_n = min(C::BO, p.N - n0);
+  const __amdgpu_buffer_rsrc_t rA = int8_rsrc(p.a + (size_t)m0 * K, (uint32_t)rows_m * (uint32_t)K);
+  // The gated block's tile holds eight gate rows of b, then the eight up rows of the same
+  // outputs, and so on: a loading wave takes the ones or the others, and a lane's
+  // accumulators hold both factors of its outputs.
+  const int up_rows = C::GLU && (wave & 1) ? p.N : 0;
+  const __amdgpu_buffer_rsrc_t rB = int8_rsrc(p.b + (size_t)(up_rows + n0) * K, (uint32_t)rows_n * (uint32_t)K);
+
+  // scales to LDS: BM row scales, BO gate (or plain) and BO up scales, in runs of 64
+#pragma unroll
+  for (int q = 0; q < C::NSC / 64; ++q) {
+    if (q % C::NW != wave) continue;
+    const bool isA = q < C::RA / 64;
+    const int base = isA ? q * 64 : (q * 64 - C::RA) % C::RO;
+    const bool up = C::GLU && q * 64 >= C::RA + C::RO;
+    const float* src = isA ? p.sa + m0 : p.sb + n0 + (up ? p.N : 0);
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(int8_rsrc(src, (uint32_t)(isA ? rows_m : rows_n) * 4u),
+                                             (lds_ptr_t)(sc + 64 * q), 4, (uint32_t)(base + lane) * 4u, 0, 0, 0);
+#endif
+  }
+
+  // load i of this wave: rows 8 (wave + NW i) .. + 7 of the slice, lane l row l >> 3 at
+  // position l & 7, which holds the row's 16-byte chunk (l & 7) ^ ((row >> 1) & 7)
+  const uint32_t cofs = (uint32_t)(((lane & 7) ^ ((lane >> 4) + 4 * (wave & 1))) * 16);
+  uint32_t va[C::AL], vb[C::BL];
+#pragma unroll
+  for (int i = 0; i < C::AL; ++i)
+    va[i] = (uint32_t)min(8 * (wave + C::LW * i) + (lane >> 3), rows_m - 1) * (uint32_t)K + cofs;
+#pragma unroll
+  for (int i = 0; i < C::BL; ++i) {
+    const int r = (C::GLU ? (wave + C::LW * i) >> 1 : wave + C::LW * i) * 8;
+    vb[i] = (uint32_t)min(r + (lane >> 3), rows_n - 1) * (uint32_t)K + cofs;
+  }
+  const int steps = (K + C::BK - 1) / C::BK;
+  const int k0 = SPLIT ? (int)((int64_t)steps * part / p.parts) : 0;
+  const int n = (SPLIT ? (int)((int64_t)steps * (part + 1) / p.parts) : steps) - k0;
+
+  auto load = [&](int i, int step, int slot) __attribute__((always_inline)) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    // past the part: nothing; past the row's end: zeros for a, what lies there for b
+    const uint32_t kb = step < n ? (uint32_t)(k0 + step) * C::BK : kOutOfRange;
+    if (i < C::BL) {
+      const int r = 8 * (wave + C::LW * i);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rB, (lds_ptr_t)(smem + slot * C::SLOT + C::ASLOT + r * C::BK), 16,
+                                               vb[i] + kb, 0, 0, 0);
+    } else {
+      const int j = i - C::BL;
+      const uint32_t ka = kb + cofs >= (uint32_t)K ? kOutOfRange : kb;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rA, (lds_ptr_t)(smem + slot * C::SLOT + 8 * (wave + C::LW * j) * C::BK), 16,
+                                               va[j] + ka, 0, 0, 0);
+    }
+#endif
+  };
+  // a step's loads are issued behind the barrier of its slot's last use, spread over
+  // that step's last slice and the next step's first ones
+  constexpr int L3 = C::L3;
+
+  const bool loader = wave < C::LW;
+  if (loader) {
+#pragma unroll
+    for (int s = 0; s < RING; ++s)
+#pragma unroll
+      for (int i = 0; i < (s + 1 < RING ? L : L3); ++i) load(i, s, s);
+  }
+
+  const int r32 = lane & 31, h = lane >> 5;
+  const uint32_t la = (uint32_t)((wm * C::TM + r32) * C::BK), lb = (uint32_t)(C::ASLOT + (wn * C::TN + r32) * C::BK);
+  const uint32_t sw = (uint32_t)((h ^ ((r32 >> 1) & 7)) * 16);
+  i16v acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
+  u4 fa[2][FM], fb[2][FN];
+  // fragment f (b's first) of slice s of a slot into set e
+  auto read = [&](int f, int slot, int s, int e) __attribute__((always_inline)) {
+    const uint8_t* at = smem + slot * C::SLOT + (sw ^ (32u * s));
+    if (f < FN) fb[e][f] = *reinterpret_cast<const u4*>(at + lb + f * 32 * C::BK);
+    else fa[e][f - FN] = *reinterpret_cast<const u4*>(at + la + (f - FN) * 32 * C::BK);
+  };
+
+  tile_barrier<(RING - 2) * L + L3>();
+#pragma unroll
+  for (int f = 0; f < FM + FN; ++f) read(f, 0, 0, 0);
+
+  int c = 0;
+  for (int kt = 0; kt < n; ++kt) {
+    const int cn = c + 1 == RING ? 0 : c + 1, cp = c == 0 ? RING - 1 : c - 1;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      if (s == 3) tile_barrier<(RING - 2) * L>();
+      constexpr int RL = L - L3;                     // loads left for slices 0 .. 2
+#pragma unroll
+      for (int g = 0; g < C::GROUPS; ++g) {
+        // (behind the last step the reads are of whatever the next slot holds)
+#pragma unroll
+        for (int f = g * C::RPG; f < (g + 1) * C::RPG && f < FM + FN; ++f) read(f, s == 3 ? cn : c, (s + 1) & 3, (s + 1) & 1);
+        const int i = g / FN, j = g % FN;
+        acc[i][j] = mfma32_i8(fb[s & 1][j], fa[s & 1][i], acc[i][j]);
+        if (!loader) {
+        } else if (s == 3) {
+#pragma unroll
+          for (int q = g * L3 / C::GROUPS; q < (g + 1) * L3 / C::GROUPS; ++q) load(q, kt + RING, c);
+        } else {
+#pragma unroll
+          for (int q = (s * C::GROUPS + g) * RL / (3 * C::GROUPS); q < (s * C::GROUPS + g + 1) * RL / (3 * C::GROUPS); ++q)
+            load(L3 + q, kt + RING - 1, cp);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    c = cn;
+  }
+  tile_barrier<0>();
+
+  // Lane l holds, of block (i, j), row m = l & 31 and columns 8 (v / 4) + 4 (l >> 5) + v % 4.
+  if constexpr (SPLIT) {
+    const int NB = C::GLU ? 2 * p.N : p.N;
+    int32_t* P = p.part + (size_t)part * p.M * NB;
+    const bool vec = (p.N & 3) == 0;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int m = m0 + wm * C::TM + i * 32 + r32;
+      if (m >= p.M) continue;
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const bool up = C::GLU && (q & 1);
+          const int nn = n0 + C::col(wn, j, q) + 4 * h;
+          int32_t* dst = P + (size_t)m * NB + (up ? p.N : 0) + nn;
+          const i4 v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+          if (vec && nn < p.N) *reinterpret_cast<i4*>(dst) = v;
+          else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (nn + e < p.N) dst[e] = v[e];
+        }
+    }
+    return;
+  }
+  uint8_t* const out = smem;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int m = wm * C::TM + i * 32 + r32;
+    const float s0 = sc[m];
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; q += C::GLU ? 2 : 1) {
+        const int nn = C::col(wn, j, q) + 4 * h;
+        const f4 sg = *reinterpret_cast<const f4*>(sc + C::RA + nn);
+        float o[4];
+        if constexpr (C::GLU) {
+          const f4 su = *reinterpret_cast<const f4*>(sc + C::RA + C::RO + nn);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int ag = acc[i][j][4 * q + e], au = acc[i][j][4 * q + 4 + e];
+            o[e] = int8_glu<ACT>(ag, au, s0, sg[e], su[e]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = int8_scaled(acc[i][j][4 * q + e], s0, sg[e]);
+        }
+        const uint2 w = make_uint2(int8_pack2<T>(o[0], o[1]), int8_pack2<T>(o[2], o[3]));
+        *reinterpret_cast<uint2*>(out + (size_t)m * (C::BO * 2) + ((nn >> 2) ^ (m & C::SW)) * 8) = w;
+      }
+  }
+  __syncthreads();
+  uint16_t* const Y = p.y + (size_t)m0 * p.N + n0;
+  if ((p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0) {
+    for (int q = threadIdx.x; q < C::BM * C::BO / 8; q += C::NT) {
+      const int r = q / (C::BO / 8), k = q % (C::BO / 8), s = r & C::SW;
+      if (r >= rows_m || 8 * k >= rows_n) continue;
+      u4 v = *reinterpret_cast<const u4*>(out + (size_t)r * (C::BO * 2) + (((2 * k) ^ s) & ~1) * 8);
+      if (s & 1) v = u4{v[2], v[3], v[0], v[1]};
+      __builtin_nontemporal_store(v, reinterpret_cast<u4*>(Y + (size_t)r * p.N + 8 * k));
+    }
+  } else {  // rows that start anywhere: consecutive lanes store consecutive values
+    for (int q = threadIdx.x; q < C::BM * C::BO; q += C::NT) {
+      const int r = q / C::BO, k = q % C::BO;
+      if (r < rows_m && k < rows_n)
+        Y[(size_t)r * p.N + k] =
+            *reinterpret_cast<const uint16_t*>(out + (size_t)r * (C::BO * 2) + ((k >> 2) ^ (r & C::SW)) * 8 + (k & 3) * 2);
+    }
+  }
+}
+
+}  // namespace cek
