@@ -41,7 +41,8 @@ HIP_FLAGS = [
 
 CABI_SOURCES = ["cek_api.cpp", "cek_gemv.hip", "cek_stream.hip", "cek_norm.hip", "cek_act.hip", "cek_gemm.hip", "cek_probe.hip",
                 "cek_kv4.hip", "cek_kv4_attn.hip", "cek_kv4_attn_rows.hip", "cek_kv_tables.hip",
-                "cek_int8_rows.hip", "cek_int8_gemm.hip"]
+                "cek_int8_rows.hip", "cek_int8_gemm.hip",
+                "cek_int8_stream.hip"]
 
 
 def _run(cmd):

@@ -3,6 +3,7 @@
 //   y[m, n] = Out((f32(sum_k a[m, k] b[n, k]) sb[n]) sa[m])
 //   y[m, i] = Out(act(g) u), g and u such values of b's rows i and d + i, unrounded
 #include "cek_int8_tile.h"
+#include "cek_int8_few.h"
 #include "cek_segs.h"
 
 namespace cek {
@@ -83,13 +84,13 @@ static double int8_us(const Int8Opt& o, int64_t M, int64_t NB, int64_t steps, in
 }
 
 struct Int8Plan {
-  int cfg, parts;
+  int cfg, parts;  // cfg < 0: the kernels for few rows
 };
 // NB: rows of b.
 static int64_t int8_parts_bytes(int parts, int64_t M, int64_t NB) {
   return parts > 1 ? ((int64_t)parts * M * NB * 4 + 15) / 16 * 16 : 0;
 }
-static Int8Plan int8_plan(int64_t M, int64_t NB, int64_t K, int64_t ws_bytes) {
+static Int8Plan int8_plan(int64_t M, int64_t NB, int64_t K, bool glu, int64_t ws_bytes) {
   Int8Plan best{0, 1};
   double us = 0;
   const int64_t steps = (K + 127) / 128;
@@ -104,6 +105,7 @@ static Int8Plan int8_plan(int64_t M, int64_t NB, int64_t K, int64_t ws_bytes) {
         best = Int8Plan{c, parts};
       }
     }
+  if (int8_few_takes(M, NB, K, glu, us)) return Int8Plan{-1, 1};
   return best;
 }
 
@@ -113,7 +115,7 @@ static bool int8_sizes_ok(int64_t M, int64_t N, int64_t K, int64_t NB) {
 static int64_t int8_workspace(int64_t M, int64_t N, int64_t K, bool glu) {
   if (N > INT32_MAX || !int8_sizes_ok(M, N, K, glu ? 2 * N : N) || M == 0 || N == 0) return 0;
   const int64_t NB = glu ? 2 * N : N;
-  return int8_parts_bytes(int8_plan(M, NB, K, INT64_MAX).parts, M, NB);
+  return int8_parts_bytes(int8_plan(M, NB, K, glu, INT64_MAX).parts, M, NB);
 }
 
 template <class C, class T, int ACT>
@@ -166,7 +168,11 @@ static int launch_int8_t(Int8Args& g, int cfg, hipStream_t st) {
 template <int ACT>
 static int launch_int8(const int8_t* a, const float* sa, const int8_t* b, const float* sb, void* y, int64_t M, int64_t N,
                        int64_t K, int out_dtype, void* ws, int64_t ws_bytes, hipStream_t st) {
-  const Int8Plan p = int8_plan(M, ACT >= 0 ? 2 * N : N, K, ws ? ws_bytes : 0);
+  const Int8Plan p = int8_plan(M, ACT >= 0 ? 2 * N : N, K, ACT >= 0, ws ? ws_bytes : 0);
+  if (p.cfg < 0)
+    return launch_int8_few(Int8Few{reinterpret_cast<const uint8_t*>(a), sa, reinterpret_cast<const uint8_t*>(b), sb,
+                                   static_cast<uint16_t*>(y), (int)M, (int)N, (int)K, out_dtype == CEK_BF16, ACT},
+                           st);
   Int8Args g{reinterpret_cast<const uint8_t*>(a), sa, reinterpret_cast<const uint8_t*>(b), sb, static_cast<uint16_t*>(y),
              static_cast<int32_t*>(ws), (int)M, (int)N, (int)K, 0, 0, p.parts};
   return out_dtype == CEK_F16 ? launch_int8_t<F16, ACT>(g, p.cfg, st) : launch_int8_t<BF16, ACT>(g, p.cfg, st);
@@ -183,10 +189,11 @@ extern "C" int64_t cek_gemm_int8_a8w8_glu_workspace_size(int64_t M, int64_t d, i
   return int8_workspace(M, d, K, true);
 }
 
-extern "C" int cek_gemm_int8_plan(int64_t M, int64_t rows_b, int64_t K, int64_t workspace_bytes) {
-  if (!int8_sizes_ok(M, rows_b, K, rows_b) || M == 0 || rows_b == 0) return -1;
-  const Int8Plan p = int8_plan(M, rows_b, K, workspace_bytes);
-  return 16 * p.cfg + p.parts;
+extern "C" int cek_gemm_int8_plan(int64_t M, int64_t N, int64_t K, int gated, int64_t workspace_bytes) {
+  const int64_t NB = gated ? 2 * N : N;
+  if (N > INT32_MAX || !int8_sizes_ok(M, N, K, NB) || M == 0 || N == 0) return -1;
+  const Int8Plan p = int8_plan(M, NB, K, gated != 0, workspace_bytes);
+  return p.cfg < 0 ? -1 : 16 * p.cfg + p.parts;
 }
 
 extern "C" int cek_gemm_int8_a8w8(const int8_t* a, const float* sa, const int8_t* b, const float* sb, void* y, int64_t M,

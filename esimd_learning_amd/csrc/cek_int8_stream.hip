@@ -1,0 +1,376 @@
+// cek_int8_stream.hip -- int8 products of a few rows of a (up to 64), gfx950: the weights
+// are read from HBM once, and that is what bounds them.
+#include <algorithm>
+#include <type_traits>
+
+#include "cek_int8_few.h"
+#include "cek_segs.h"
+
+namespace cek {
+
+// ---- one to four rows --------------------------------------------------------
+// v_dot4 on 16-byte units: thread u of a workgroup holds a's values of unit u of
+// every 4 KB of K, for all M rows, and multiplies them with the same unit of R
+// weight rows, so that a wave's load reads 1 KB of one row.  The sums meet in the
+// lanes of a wave, then of four waves in LDS.
+// TPR threads per weight row: 256, or fewer where K is shorter than 4 KB.
+template <int M, int R, int CH, int TPR, bool GLU>
+__global__ __launch_bounds__(256) void int8_dot_kernel(Int8Few p) {
+  constexpr int RT = GLU ? 2 * R : R;  // weight rows of a thread: R gate rows, then their up rows
+  constexpr int G = 256 / TPR, W = TPR / 64;
+  __shared__ int red[4][M * RT];
+  const int units = p.K / 16, tid = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+  const int n0 = (blockIdx.x * G + grp) * R;
+  int acc[RT][M];
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int m = 0; m < M; ++m) acc[r][m] = 0;
+  for (int u0 = 0; u0 < units; u0 += TPR * CH) {
+    u4 w[RT][CH], x[M][CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int u = min(u0 + TPR * c + tid, units - 1);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const size_t row = (size_t)min(n0 + r % R, p.N - 1) + (r >= R ? (size_t)p.N : 0);
+        w[r][c] = load_u4_stream(p.b + row * p.K + 16 * u);
+      }
+#pragma unroll
+      for (int m = 0; m < M; ++m) x[m][c] = load_u4(p.a + (size_t)m * p.K + 16 * u);
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const bool in = u0 + TPR * c + tid < units;
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const u4 xv = in ? x[m][c] : u4{0, 0, 0, 0};
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[r][m] = __builtin_amdgcn_sdot4((int)w[r][c][e], (int)xv[e], acc[r][m], false);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int m = 0; m < M; ++m) acc[r][m] = wave_isum(acc[r][m]);
+  if ((tid & 63) == 0) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int m = 0; m < M; ++m) red[threadIdx.x >> 6][r * M + m] = acc[r][m];
+  }
+  __syncthreads();
+  if (tid < M * R) {
+    const int r = tid / M, m = tid % M, n = n0 + r;
+    auto sum = [&](int i) {
+      int s = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) s += red[grp * W + w][i];
+      return s;
+    };
+    if (n < p.N) {
+      if constexpr (GLU) int8_store(p, m, n, sum(tid), sum(tid + M * R), p.sa[m], p.sb[n], p.sb[(size_t)p.N + n]);
+      else int8_store(p, m, n, sum(tid), 0, p.sa[m], p.sb[n], 0.f);
+    }
+  }
+}
+
+template <int M, int R, bool GLU>
+static int launch_dot_r(const Int8Few& p, hipStream_t st) {
+#define CEK_I8D(CH, TPR) \
+  int8_dot_kernel<M, R, CH, TPR, GLU><<<(unsigned)(((int64_t)p.N + R * (256 / TPR) - 1) / (R * (256 / TPR))), 256, 0, st>>>(p)
+  if (p.K <= 1024) CEK_I8D(1, 64);
+  else if (p.K <= 2048) CEK_I8D(1, 128);
+  else if (p.K <= 4096) CEK_I8D(1, 256);
+  else CEK_I8D(2, 256);
+#undef CEK_I8D
+  return check_launch();
+}
+// Weight rows of a thread, measured (us): N = 14336, K = 4096, one row 2 / 4 / 8 10.30 /
+// 10.46 / 10.75; N = 28672, K = 1024 7.12 / 6.56 / 6.78; N = 512, K = 16384 3.8 / 4.2 / 6.1.
+// The gated block's two outputs are four rows: one row of d = 14336 19.46 (four
+// outputs 19.46, one 21.0).
+template <int M>
+static int launch_dot_m(const Int8Few& p, hipStream_t st) {
+  if (p.act >= 0) return launch_dot_r<M, 2, true>(p, st);
+  return p.K <= 2048 && p.N >= 8192 ? launch_dot_r<M, 4, false>(p, st) : launch_dot_r<M, 2, false>(p, st);
+}
+
+static int launch_int8_dot(const Int8Few& p, hipStream_t st) {
+  switch (p.M) {
+    case 1: return launch_dot_m<1>(p, st);
+    case 2: return launch_dot_m<2>(p, st);
+    case 3: return launch_dot_m<3>(p, st);
+    case 4: return p.act >= 0 ? launch_dot_r<4, 2, true>(p, st) : CEK_ERR_UNSUPPORTED;
+    default: return CEK_ERR_UNSUPPORTED;
+  }
+}
+
+// ---- up to 64 rows -----------------------------------------------------------
+// Weights and activations stream through LDS rings that loader waves fill with
+// direct-to-LDS loads (1 KB: two rows x 512 bytes); eight consumer waves take 64 K
+// values of a stage's 512 each over all 16 x 16 blocks of the workgroup (AR rows of a
+// x RW of b) and meet in LDS at the end.  One barrier a stage.
+constexpr int kConsumers = 8;
+
+template <int AR_, int RW_, bool GLU_>
+struct Int8Stream {
+  static constexpr int AR = AR_, RW = RW_;
+  static constexpr bool GLU = GLU_;
+  static constexpr int KS = 512, MB = (AR + 15) / 16, NT = (RW + 15) / 16;
+  static constexpr int WL = 2, AL = AR >= 64 ? 4 : 2;
+  static constexpr int THREADS = 64 * (kConsumers + WL + AL);
+  static constexpr int LDSB = AR <= 16 && RW <= 24 ? 81920 : 163840;  // two workgroups per CU, or one
+  static constexpr int RING = LDSB - 512;
+  static constexpr int ASZ = AR * KS, WSZ = RW * KS, SLOT = ASZ + WSZ;
+  static constexpr int AM = ASZ / 1024 / AL, WM = WSZ / 1024 / WL;    // loads per loader wave and stage
+  static constexpr int PER = AM > WM ? AM : WM, R0 = RING / SLOT, R1 = R0 > 24 ? 24 : R0;
+  static constexpr int R = R1 > 62 / PER + 1 ? 62 / PER + 1 : R1;
+  static_assert(AM * AL * 1024 == ASZ && WM * WL * 1024 == WSZ, "loads");
+  static_assert(R >= 2 && (!GLU || RW % 8 == 0), "rings; four gate rows beside four up rows");
+};
+
+// A loader wave: MINE loads a stage, of the 1 KB pieces who + WAVES m, through a ring of
+// R slots SLOT bytes apart.  A slot holds rows of 512 bytes one after another, unit u
+// of row r at u ^ (r & 15).  Row offsets vo, this lane's byte offset of its unit within
+// the stage ku.  ZERO: units past the row are zeros, else whatever lies there.  The
+// wave takes part in the S stage barriers: before barrier i stage i has landed, after
+// it stage i - 1's slot is free.
+template <int MINE, int WAVES, int R, int SLOT, bool ZERO>
+__device__ __forceinline__ void int8_stream_load(uint8_t* slots, const uint32_t (&vo)[MINE], const uint32_t (&ku)[MINE],
+                                                 int K, int S, int k_first, __amdgpu_buffer_rsrc_t even,
+                                                 __amdgpu_buffer_rsrc_t odd, int who) {
+  auto issue = [&](int s, int slot) {
+    const uint32_t k0 = (uint32_t)(s + k_first >= S ? s + k_first - S : s + k_first) * 512;
+#pragma unroll
+    for (int m = 0; m < MINE; ++m) {
+      uint32_t off = vo[m] + k0 + ku[m];
+      if (ZERO && k0 + ku[m] >= (uint32_t)K) off = 0x80000000u;
+#if defined(__HIP_DEVICE_COMPILE__)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(m & 1 ? odd : even, (lds_ptr_t)(slots + slot * SLOT + 1024 * (who + WAVES * m)),
+                                               16, off, 0, 0, 0);
+#endif
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < R; ++s)
+    if (s < S) issue(s, s);
+  if (S >= R) {
+    wait_vmcnt<(R - 1) * MINE>();
+    bare_barrier();
+    int slot = 0;
+    for (int s = R; s < S; ++s) {
+      wait_vmcnt<(R - 2) * MINE>();
+      bare_barrier();
+      issue(s, slot);
+      slot = slot + 1 == R ? 0 : slot + 1;
+    }
+  }
+  auto drain = [&](auto self, auto rc) {
+    constexpr int r = decltype(rc)::value;
+    if (S >= R ? r < R - 1 : r < S) {
+      wait_vmcnt<r * MINE>();
+      bare_barrier();
+    }
+    if constexpr (r > 0) self(self, std::integral_constant<int, r - 1>{});
+  };
+  drain(drain, std::integral_constant<int, R - 1>{});
+}
+
+template <class C>
+__global__ __launch_bounds__(C::THREADS, (C::LDSB > 81920 ? 3 : 6)) void int8_stream_kernel(Int8Few p) {
+  constexpr int MB = C::MB, NT = C::NT, R = C::R;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[C::LDSB];
+  float* const sw = reinterpret_cast<float*>(smem + C::RING);  // [RW]
+  float* const sx = sw + 64;                                   // [M]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  constexpr int RO = C::GLU ? C::RW / 2 : C::RW;               // outputs of a workgroup
+  const int n0 = blockIdx.x * RO, K = p.K, S = (K + C::KS - 1) / C::KS;
+  const int rows = min(RO, p.N - n0);
+  const int k_first = p.N >= 8192 ? (int)((blockIdx.x >> 3) % (unsigned)S) : 0;
+  // weight row r of the workgroup: of the gated block four gate rows, their up rows, four more
+  // (the weights' loader waves take pairs of rows in turn: an even load is gate, an odd one up)
+  auto out_of = [](int r) { return C::GLU ? (r >> 3) * 4 + (r & 3) : r; };
+
+  i4 acc[MB][NT];
+#pragma unroll
+  for (int b = 0; b < MB; ++b)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[b][t] = i4{0, 0, 0, 0};
+
+  if (wave >= kConsumers + C::WL) {
+    const int who = wave - kConsumers - C::WL;
+    uint32_t vo[C::AM], ku[C::AM];
+#pragma unroll
+    for (int m = 0; m < C::AM; ++m) {
+      const int row = 2 * (who + C::AL * m) + (lane >> 5);
+      vo[m] = (uint32_t)min(row, p.M - 1) * (uint32_t)K;
+      ku[m] = 16u * (uint32_t)((lane & 31) ^ (row & 15));
+    }
+    const __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.a), 0, (int)((uint32_t)p.M * (uint32_t)K), 0x00020000);
+    int8_stream_load<C::AM, C::AL, R, C::SLOT, true>(smem, vo, ku, K, S, k_first, r, r, who);
+  } else if (wave >= kConsumers) {
+    const int who = wave - kConsumers;
+    uint32_t vo[C::WM], ku[C::WM];
+#pragma unroll
+    for (int m = 0; m < C::WM; ++m) {
+      const int row = 2 * (who + C::WL * m) + (lane >> 5);
+      vo[m] = (uint32_t)min(out_of(row), rows - 1) * (uint32_t)K;
+      ku[m] = 16u * (uint32_t)((lane & 31) ^ (row & 15));
+    }
+    auto rsrc = [&](size_t first) {
+      return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.b + first * K), 0, (int)((uint32_t)rows * (uint32_t)K), 0x00020000);
+    };
+    const __amdgpu_buffer_rsrc_t rg = rsrc(n0), ru = C::GLU ? rsrc((size_t)p.N + n0) : rg;
+    int8_stream_load<C::WM, C::WL, R, C::SLOT, false>(smem + C::ASZ, vo, ku, K, S, k_first, rg, ru, who);
+  } else {
+    if (wave == 0 && lane < C::RW) sw[lane] = p.sb[(C::GLU && (lane & 4) ? (size_t)p.N : 0) + min(n0 + out_of(lane), p.N - 1)];
+    if (wave == 1 && lane < p.M) sx[lane] = p.sa[lane];
+    const int r16 = lane & 15, g = lane >> 4, unit = 4 * wave + g;
+    int ao[MB], wo[NT];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+      const int row = min(16 * b + r16, C::AR - 1);
+      ao[b] = row * C::KS + 16 * (unit ^ (row & 15));
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int row = min(16 * t + r16, C::RW - 1);
+      wo[t] = C::ASZ + row * C::KS + 16 * (unit ^ (row & 15));
+    }
+    const uint8_t* at = smem;
+    int ks = k_first;
+    for (int i = 0; i < S; ++i) {
+      lds_barrier();  // stage i has landed; this wave's reads of stage i - 1 are done
+      if (ks * C::KS + wave * 64 < K) {
+        u4 av[MB], wv[NT];
+#pragma unroll
+        for (int b = 0; b < MB; ++b) av[b] = *reinterpret_cast<const u4*>(at + ao[b]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) wv[t] = *reinterpret_cast<const u4*>(at + wo[t]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int b = 0; b < MB; ++b) acc[b][t] = mfma_i8(av[b], wv[t], acc[b][t]);
+      }
+      ks = ks + 1 == S ? 0 : ks + 1;
+      at = at + C::SLOT == smem + R * C::SLOT ? smem : at + C::SLOT;
+    }
+  }
+
+  // The eight waves' sums meet in LDS, GB blocks at a time: D row 4 (lane >> 4) + v of a
+  // block is row m of a, column lane & 15 the weight row.
+  constexpr int BL = MB * NT, GB0 = C::RING / (kConsumers * 1024), GB = GB0 < BL ? GB0 : BL;
+  i4* const red = reinterpret_cast<i4*>(smem);  // [8][GB][64]
+#pragma unroll
+  for (int b0 = 0; b0 < BL; b0 += GB) {
+    lds_barrier();  // the slots, or the blocks before, are done with
+    if (wave < kConsumers) {
+#pragma unroll
+      for (int j = 0; j < GB; ++j)
+        if (b0 + j < BL) red[(wave * GB + j) * 64 + lane] = acc[(b0 + j) / NT][(b0 + j) % NT];
+    }
+    lds_barrier();
+    for (int q = threadIdx.x; q < GB * 64; q += C::THREADS) {
+      const int blk = b0 + q / 64, r = 16 * (blk % NT) + (q & 15), m0 = 16 * (blk / NT) + 4 * ((q & 63) >> 4);
+      const int n = n0 + out_of(r);
+      if (blk >= BL || r >= C::RW || n >= p.N || m0 >= p.M || (C::GLU && (q & 4))) continue;
+      i4 c = red[q], u{0, 0, 0, 0};
+      if constexpr (C::GLU) u = red[q + 4];
+#pragma unroll
+      for (int w = 1; w < kConsumers; ++w) {
+        c += red[w * GB * 64 + q];
+        if constexpr (C::GLU) u += red[w * GB * 64 + q + 4];
+      }
+      const float sg = sw[r], su = C::GLU ? sw[r + 4] : 0.f;
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        if (m0 + v < p.M) int8_store(p, m0 + v, n, c[v], u[v], sx[m0 + v], sg, su);
+    }
+  }
+}
+
+template <int AR, bool GLU>
+static int launch_stream_ar(const Int8Few& p, int rw, hipStream_t st) {
+  const unsigned grid = (unsigned)((p.N + (GLU ? rw / 2 : rw) - 1) / (GLU ? rw / 2 : rw));
+#define CEK_I8S(RW) int8_stream_kernel<Int8Stream<AR, RW, GLU>><<<grid, (Int8Stream<AR, RW, GLU>::THREADS), 0, st>>>(p)
+  switch (rw) {
+    case 8: CEK_I8S(8); break;
+    case 12:
+      if constexpr (!GLU) CEK_I8S(12);
+      else return CEK_ERR_UNSUPPORTED;
+      break;
+    case 16: CEK_I8S(16); break;
+    case 24: CEK_I8S(24); break;
+    case 32: CEK_I8S(32); break;
+    case 40: CEK_I8S(40); break;
+    case 48: CEK_I8S(48); break;
+    case 56: CEK_I8S(56); break;
+    case 64: CEK_I8S(64); break;
+    default: return CEK_ERR_UNSUPPORTED;
+  }
+#undef CEK_I8S
+  return check_launch();
+}
+
+template <bool GLU>
+static int launch_stream_g(const Int8Few& p, int rw, hipStream_t st) {
+  if (p.M <= 8) return launch_stream_ar<8, GLU>(p, rw, st);
+  if (p.M <= 16) return launch_stream_ar<16, GLU>(p, rw, st);
+  if (p.M <= 32) return launch_stream_ar<32, GLU>(p, rw, st);
+  if (p.M <= 48) return launch_stream_ar<48, GLU>(p, rw, st);
+  return launch_stream_ar<64, GLU>(p, rw, st);
+}
+
+// Weight rows per workgroup and the launch's time in us: a CU's workgroups cost their
+// weight and activation bytes, and each after the first its start and end, less where two
+// share a CU (the rings of one cover the other's); no launch takes less than its start and
+// the weights at the rate HBM gives.  Fitted to 540 launches over 62 shapes (weights from
+// HBM); the pick is 1.5% above the fastest count up to 16 rows, 1% above that.
+static int stream_plan(int64_t M, int64_t NB, int64_t K, bool glu, double* us) {
+  const bool few = M <= 16;
+  const double start = few ? 2.61 : 2.91, weight = few ? 0.0234e-3 : 0.0352e-3, act = few ? 0.0103e-3 : 0.0051e-3,
+               next = few ? 5.06 : 2.90;
+  const int rows[] = {8, 12, 16, 24, 32, 40, 48, 56, 64};
+  const int ar = M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : M <= 48 ? 48 : 64;
+  int best = 0;
+  for (int r : rows) {
+    if (glu && r == 12) continue;
+    const int64_t per_cu = ((NB + r - 1) / r + kCUs - 1) / kCUs;
+    const double t = start + (double)per_cu * (r * weight + ar * act) * (double)K +
+                     (double)(per_cu - 1) * (few && r <= 24 ? 0.77 : next);
+    if (!best || t < *us) {
+      *us = t;
+      best = r;
+    }
+  }
+  *us = std::max(*us, start + (double)NB * (double)K / 6.0e6);
+  return best;
+}
+
+// Up to three rows (four of the gated block) v_dot4, us at N = 14336, K = 4096: one row 10.3
+// against 12.1 of the rings, three 11.8 against 12.3, four 12.8 against 12.4; the block's
+// four 21.9 against 23.2.
+static bool int8_dot_takes(int64_t M, bool glu) { return M <= (glu ? 4 : 3); }
+
+bool int8_few_takes(int64_t M, int64_t NB, int64_t K, bool glu, double tile_us) {
+  if (M > 64) return false;
+  if (M <= 32) return true;  // (the tiles were 2 to 40% slower throughout)
+  double us;
+  stream_plan(M, NB, K, glu, &us);
+  return us <= tile_us;
+}
+
+int launch_int8_few(const Int8Few& p, hipStream_t st) {
+  const bool glu = p.act >= 0;
+  if (int8_dot_takes(p.M, glu)) return launch_int8_dot(p, st);
+  double us;
+  const int rw = stream_plan(p.M, glu ? 2 * (int64_t)p.N : p.N, p.K, glu, &us);
+  return glu ? launch_stream_g<true>(p, rw, st) : launch_stream_g<false>(p, rw, st);
+}
+
+}  // namespace cek

@@ -480,13 +480,16 @@ int cek_fused_add_rms_norm_quant_int8(const void* hidden, void* residual, const 
 int64_t cek_gemm_int8_a8w8_workspace_size(int64_t M, int64_t N, int64_t K);
 int cek_gemm_int8_a8w8(const int8_t* a, const float* sa, const int8_t* b, const float* sb, void* y, int64_t M, int64_t N,
                        int64_t K, int out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
-/* NEW, for tests and tuning: the tiled launch of a product with rows_b rows of b and that much
- * workspace, 16 * tile + parts of K; -1 where other kernels serve it. */
-int cek_gemm_int8_plan(int64_t M, int64_t rows_b, int64_t K, int64_t workspace_bytes);
 int64_t cek_gemm_int8_a8w8_glu_workspace_size(int64_t M, int64_t d, int64_t K);
 int cek_gemm_int8_a8w8_glu(const int8_t* a, const float* sa, const int8_t* b, const float* sb, void* y, int64_t M,
                            int64_t d, int64_t K, int activation, int out_dtype, void* workspace, int64_t workspace_bytes,
                            void* stream);
+/*
+ * NEW, for tests and tuning: the tiled launch that a product [M, N] (gated != 0: a gated
+ * block with N outputs) with that much workspace takes, 16 * tile + parts of K; -1 where
+ * the kernels for up to 64 rows serve it.
+ */
+int cek_gemm_int8_plan(int64_t M, int64_t N, int64_t K, int gated, int64_t workspace_bytes);
 
 /*
  * Measurement utility, no counterpart in the reference: reads `bytes` bytes
