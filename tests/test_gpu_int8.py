@@ -35,7 +35,8 @@ def _rows(t, h, seed, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("t,h", [(1, 1), (3, 7), (1, 8), (5, 64), (2, 129), (9, 136), (4, 512), (1, 1000), (3, 2048), (2, 2056),
                                  (7, 4096), (2, 5120), (1, 14336), (600, 520), (513, 4104), (2, 16384), (2, 16392), (1, 33001),
-                                 (2, 40960)])
+                                 (2, 40960), (5, 9), (3, 15), (1025, 1001), (1030, 4099), (2, 8195), (1024, 8190), (1, 65536), (1, 65537),
+                                 (1, 70000)])
 def test_quant(ops, dev, t, h, dtype):
     x = _rows(t, h, t * 1000 + h, dtype)
     q = torch.full((t, h), 77, dtype=torch.int8, device=dev)
@@ -92,7 +93,8 @@ def test_quant_ends_of_the_range(ops, dev, h, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("t,h", [(1, 1), (3, 7), (4, 64), (2, 136), (5, 1000), (4, 5120), (1, 4096), (513, 2048), (3, 8192), (2, 16384),
-                                 (2, 16400), (2, 4099)])
+                                 (2, 16400), (2, 4099), (5, 9), (3, 15), (1030, 1001), (1025, 4099), (1024, 5121), (1027, 8190), (2, 8195), (3, 30001),
+                                 (1, 32768), (1, 32769)])
 def test_norm_quant(ops, dev, t, h, dtype):
     """The residual and the scale are the oracle's (the scale within fp32's roundings), codes at most one off and
     only next to a border."""
@@ -113,6 +115,27 @@ def test_norm_quant(ops, dev, t, h, dtype):
     off = q.cpu().double() - exact
     assert (off.abs() <= 0.5 + 127 * 2 * rel).all()
     assert (q.cpu() != want_q).double().mean() <= 4 * 127 * rel + 1.0 / (t * h)
+
+
+@pytest.mark.parametrize("h", [4096, 4093, 520, 77])
+def test_rows_that_start_anywhere(ops, dev, h):
+    """Tensors whose storage is not aligned: the same codes, and nothing outside them written."""
+    t = 3
+    x, res, w = _rows(t, h, 1, torch.float16), _rows(t, h, 2, torch.float16), synthetic.norm_weight(h, 3)
+    want_q, want_s = oint8.quant(x)
+    for off in (1, 3, 8):
+        put = lambda v: torch.cat([torch.zeros(off, dtype=v.dtype), v.reshape(-1)]).to(dev)[off:].view(v.shape)  # noqa: E731
+        buf = torch.full((off + t * h + 16,), 99, dtype=torch.int8, device=dev)
+        q, s = buf[off:off + t * h].view(t, h), torch.empty(t, device=dev)
+        ops.esimd_per_token_quant_int8(put(x), q, s)
+        assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
+        a, b = torch.empty(t, h, dtype=torch.int8, device=dev), torch.empty(t, device=dev)
+        r, r0 = put(res), res.to(dev)
+        ops.esimd_fused_add_rms_norm_quant_int8(put(x), r, put(w), 1e-6, q, s)
+        ops.esimd_fused_add_rms_norm_quant_int8(x.to(dev), r0, w.to(dev), 1e-6, a, b)
+        assert torch.equal(r, r0)
+        assert (q - a).abs().max() <= 1 and ((s - b).abs() <= b * 2.0 ** -20).all()
+        assert (buf[:off] == 99).all() and (buf[off + t * h:] == 99).all()
 
 
 def test_norm_quant_not_finite(ops, dev):
