@@ -61,6 +61,23 @@ alone, prompt chunks beside them, the join of keys shared by workgroups).  Rows 
 request that got no room, where its rows stay)
 are padding: nothing is stored for them and their outputs mean nothing.
 
+Int8 weights (Wqkv, Wo, Wgu and Wd all int8, their scales fp32; ``synthetic.gemma_layer(fmt=torch.int8)``, or
+esimd_per_token_quant_int8 of an [N, K] weight) make it a W8A8 layer, for any number of rows: each
+product takes int8 codes and a scale per token,
+
+    q8, r1 = quant(add_rmsnorm(hidden, residual, w_in))    esimd_fused_add_rms_norm_quant_int8
+    qkv    = q8 @ Wqkv^T                                   esimd_gemm_int8_a8w8
+    q, k, attention as above
+    o      = quant(a) @ Wo^T                               esimd_per_token_quant_int8, esimd_gemm_int8_a8w8
+    q8, r2 = quant(add_rmsnorm(o, r1, w_post))             esimd_fused_add_rms_norm_quant_int8
+    g      = act(q8 @ Wg^T) * (q8 @ Wu^T)                  esimd_gemm_int8_a8w8_glu
+    out    = quant(g) @ Wd^T                               esimd_per_token_quant_int8, esimd_gemm_int8_a8w8
+
+with act = params["activation"], "gelu_tanh" (the default) or "silu".  hidden is only
+read; ``fuse_glu=False`` runs gate/up as one product into [M, 2d] and esimd_gelu_and_mul (gelu_tanh
+only), which rounds both halves in between; the other ``fuse_`` options and
+``defer_norm`` have no int8 form and are off.
+
 The intermediate buffers and counters are allocated once in the
 constructor, so at decode sizes a step enqueues only kernels: it can be
 captured in a HIP graph (``capture``) and replayed, which removes host launch
@@ -69,7 +86,7 @@ exception: with ``act_fp8`` at M = 64 the a8w8 op splits K where K exceeds
 5120 or N 16384 (a wide gate/up matrix) and takes its fp32 workspace from
 PyTorch's caching allocator on every call -- inside a captured graph, from the
 graph's memory pool.  The attention's workspace, where keys are split, is taken
-the same way.)
+the same way, and so is that of an int8 product above 32 rows that splits K.)
 """
 
 import torch
@@ -105,7 +122,23 @@ class GemmaDecodeLayer:
         self.r_mid = mk(self.hidden)            # r1 between the two fused norms
         self.fuse_tails = fuse_tails and not act_fp8 and not self.fuse_norm
         self.cnt_rope = self.ops.gemv_tail_counters(self.nq, self.nk, device)
-        e4m3 = all(w.dtype == torch.float8_e4m3fn for w in (self.Wqkv, self.Wo, self.Wgu, self.Wd))
+        weights = (self.Wqkv, self.Wo, self.Wgu, self.Wd)
+        self.int8 = any(w.dtype == torch.int8 for w in weights)
+        self.activation = p.get("activation", "gelu_tanh")
+        if self.int8:
+            if any(w.dtype != torch.int8 for w in weights) or any(s.dtype != torch.float32 for s in (self.sqkv, self.so, self.sgu, self.sd)):
+                raise ValueError("an int8 layer needs int8 codes and fp32 scales of all four weights")
+            if act_fp8:
+                raise ValueError("act_fp8 needs e4m3 weights")
+            if not fuse_glu and self.activation != "gelu_tanh":
+                raise ValueError("fuse_glu=False has gelu_tanh alone")
+            self.fuse_norm = self.fuse_tails = False
+            codes = lambda n: torch.empty(M, n, dtype=torch.int8, device=device)  # noqa: E731
+            self.q8, self.a8, self.d8 = codes(self.hidden), codes(self.nq * self.hd), codes(self.mlp)
+            self.s8 = torch.empty(M, dtype=torch.float32, device=device)   # of the product at hand
+        elif self.activation != "gelu_tanh":
+            raise ValueError("fp8 layers have gelu_tanh alone")
+        e4m3 = all(w.dtype == torch.float8_e4m3fn for w in weights)
         # the shapes the deferred-norm kernels take (else the unfused step)
         kib = lambda k: k % 1024 == 0 and k // 1024 in (2, 3, 4, 5, 14, 24)  # noqa: E731
         # (hidden: the QKV and gate/up K the consumers take, and at most 256
@@ -161,6 +194,10 @@ class GemmaDecodeLayer:
         ``next_norm`` (the next layer's (w_in, shift_in)) the down projection
         produces that for the next layer and ss_d."""
         o, hd, nq, nk = self.ops, self.hd, self.nq, self.nk
+        if self.int8:
+            if ss_in is not None or next_norm is not None:
+                raise ValueError("ss_in / next_norm need defer_norm")
+            return self._step_int8(hidden, residual, positions, kv)
         if self.fuse_norm:
             return self._step_fused(hidden, residual, positions, kv)
         if self.defer_norm:
@@ -199,6 +236,25 @@ class GemmaDecodeLayer:
         if not self.fuse_glu:
             o.esimd_gelu_and_mul(self.act, self.gu)
         o.esimd_gemv_fp8_pern(self.act, self.Wd, self.sd, self.out, self.hidden, self.mlp)
+        return self.out
+
+    def _step_int8(self, hidden, residual, positions, kv):
+        o, hd, nq, nk, s8 = self.ops, self.hd, self.nq, self.nk, self.s8
+        o.esimd_fused_add_rms_norm_quant_int8(hidden, residual, self.w_in, self.eps, self.q8, s8)
+        o.esimd_gemm_int8_a8w8(self.q8, s8, self.Wqkv, self.sqkv, self.qkv)
+        o.esimd_qk_norm_rope(self.qkv[:, : nq * hd], self.qkv[:, nq * hd:(nq + nk) * hd], self.qw, self.kw, positions,
+                             self.eps, self.theta, True)
+        self._attend(kv)
+        o.esimd_per_token_quant_int8(self.attn, self.a8, s8)
+        o.esimd_gemm_int8_a8w8(self.a8, s8, self.Wo, self.so, self.o)
+        o.esimd_fused_add_rms_norm_quant_int8(self.o, residual, self.w_post, self.eps, self.q8, s8)
+        if self.fuse_glu:
+            o.esimd_gemm_int8_a8w8_glu(self.q8, s8, self.Wgu, self.sgu, self.act, self.activation)
+        else:
+            o.esimd_gemm_int8_a8w8(self.q8, s8, self.Wgu, self.sgu, self.gu)
+            o.esimd_gelu_and_mul(self.act, self.gu)
+        o.esimd_per_token_quant_int8(self.act, self.d8, s8)
+        o.esimd_gemm_int8_a8w8(self.d8, s8, self.Wd, self.sd, self.out)
         return self.out
 
     def _step_fused(self, hidden, residual, positions, kv):

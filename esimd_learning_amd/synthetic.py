@@ -7,6 +7,7 @@ callers move them to the GPU.
 Weight recipe (per output row n):
     W ~ N(0, 0.02) fp32;  s[n] = amax_k |W[n, k]| / 448 (fp32);
     W8 = e4m3(clamp(W / s[:, None], -448, 448))        (RNE)
+    int8: s[n] = amax / 127, W8 = W / s[:, None] to the nearest integer
 Activations are fp16 N(0, 1); RMSNorm weights 1 + N(0, 0.1) in fp16 (already
 in the Gemma w + 1 convention); eps 1e-6; RoPE theta 10000 and positions drawn
 from [0, 8192).
@@ -23,7 +24,10 @@ def gen(seed):
 
 
 def quantize_rows(W, fmt=torch.float8_e4m3fn):
-    """Per-row fp8 quantisation of an fp32 [N, K] matrix -> (W8, s fp32 [N])."""
+    """Per-row fp8 (or int8) quantisation of an fp32 [N, K] matrix -> (W8, s fp32 [N])."""
+    if fmt == torch.int8:
+        s = W.abs().amax(dim=1) / 127
+        return (W / s[:, None]).round().to(torch.int8), s.float()
     fmax = E5M2_MAX if fmt == torch.float8_e5m2 else E4M3_MAX
     s = W.abs().amax(dim=1) / fmax
     W8 = (W / s[:, None]).clamp(-fmax, fmax).to(fmt)
@@ -49,7 +53,7 @@ def positions(T, seed=3, max_pos=8192):
 
 def gemma_layer(seed=10, hidden=3072, n_q=16, n_kv=16, head_dim=256, mlp=24576,
                 fmt=torch.float8_e4m3fn):
-    """Random-init fp8 weights of one Gemma-style decoder layer (config 5)."""
+    """Random-init fp8 (fmt=torch.int8: int8) weights of one Gemma-style decoder layer (config 5)."""
     qkv_n = (n_q + 2 * n_kv) * head_dim
     p = {"hidden": hidden, "n_q": n_q, "n_kv": n_kv, "head_dim": head_dim, "mlp": mlp,
          "eps": 1e-6, "theta": 10000.0}
