@@ -270,3 +270,52 @@ def test_no_rows_and_refusals(ops, dev):
             call()
             print("not refused:", i)
     assert (y == 1).all()
+
+
+# Sizes of no tile: each tile's own, then tiles that split K, in two to eight parts.
+TILED = [(769, 12311, 464), (520, 13273, 464), (408, 12613, 464), (324, 16348, 464), (261, 13159, 464), (580, 6402, 464),
+         (132, 11154, 464), (65, 68, 464)]
+SPLIT = [(500, 4090, 14320), (3000, 700, 12000), (66, 5442, 4944), (68, 5910, 4272), (685, 133, 2576), (65, 66, 1968),
+         (71, 65, 3056), (65, 70, 4032), (1030, 1030, 16384)]
+
+
+def test_every_tile_is_tested():
+    from esimd_learning_amd import cabi
+    plan = cabi.load().cek_gemm_int8_plan
+    for gated in (0, 1):
+        plans = [plan(m, n // (1 + gated), k, gated, 1 << 40) for m, n, k in TILED]
+        assert sorted(p // 16 for p in plans) == list(range(8)) and all(p % 16 == 1 for p in plans)
+        plans = [plan(m, n // (1 + gated), k, gated, 1 << 40) for m, n, k in SPLIT]
+        assert all(p % 16 > 1 for p in plans) and {p // 16 for p in plans} >= {2, 3, 5, 7}
+
+
+@pytest.mark.parametrize("m,n,k", TILED + SPLIT)
+def test_tiles(ops, dev, m, n, k):
+    """Both forms of every tile, whole and split, and without the workspace that the split takes."""
+    from esimd_learning_amd import cabi
+    lib = cabi.load()
+    n -= n % 2
+    g = torch.Generator(device=dev).manual_seed(m + n + k)
+    a, b = (torch.randint(-128, 128, (rows, k), generator=g, dtype=torch.int8, device=dev) for rows in (m, n))
+    sa, sb = torch.rand(m, generator=g, device=dev) * 0.01, torch.rand(n, generator=g, device=dev) * 0.01
+    acc = a.double() @ b.double().t()                 # integers below 2^53: exact in any order
+    want = (acc.float() * sb * sa[:, None]).bfloat16()
+    y = torch.full((m, n), math.nan, dtype=torch.bfloat16, device=dev)
+    ops.esimd_gemm_int8_a8w8(a, sa, b, sb, y)
+    assert torch.equal(y, want)
+    y.fill_(math.nan)
+    cabi.check(lib.cek_gemm_int8_a8w8(cabi.ptr(a), cabi.ptr(sa), cabi.ptr(b), cabi.ptr(sb), cabi.ptr(y), m, n, k, cabi.CEK_BF16,
+                                      None, 0, cabi.stream_ptr()))
+    assert torch.equal(y, want)
+    sb /= 127 * math.sqrt(k)                          # gates of some units
+    z, z0 = (torch.full((m, n // 2), math.nan, dtype=torch.float16, device=dev) for _ in range(2))
+    ops.esimd_gemm_int8_a8w8_glu(a, sa, b, sb, z, "silu")
+    cabi.check(lib.cek_gemm_int8_a8w8_glu(cabi.ptr(a), cabi.ptr(sa), cabi.ptr(b), cabi.ptr(sb), cabi.ptr(z0), m, n // 2, k,
+                                          cabi.CEK_SILU, cabi.CEK_F16, None, 0, cabi.stream_ptr()))
+    assert torch.equal(z, z0)
+    gu = acc * sb.double() * sa.double()[:, None]
+    gate, up = gu[:, : n // 2], gu[:, n // 2:]
+    f = gate * torch.sigmoid(gate) * up
+    rel = (16 + 16 * gate.abs() * torch.sigmoid(-gate)) * 2.0 ** -24      # the bound of oracle.int8.gated
+    limit = f.abs() * (rel + 2.0 ** -11) + gate.abs() * up.abs() * 2.0 ** -126 + 2.0 ** -25
+    assert ((z.double() - f).abs() <= limit).all()
