@@ -5,39 +5,31 @@
 
 namespace cek {
 
-typedef int i16v __attribute__((ext_vector_type(16)));
-
 template <int BM_, int BN_, int WM_, int WN_, int LW_, int RING_, bool GLU_>
 struct Int8Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, RING = RING_, BK = 128;
   static constexpr bool GLU = GLU_;
   static constexpr int BO = GLU ? BN / 2 : BN;              // output columns
   static constexpr int NW = WM * WN, NT = 64 * NW;
-  static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+  static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
   static constexpr int ASLOT = BM * BK, BSLOT = BN * BK, SLOT = ASLOT + BSLOT;
   static constexpr int LW = LW_;                            // waves that load
   static constexpr int AL = BM / 8 / LW, BL = BN / 8 / LW, L = AL + BL;  // 1 KB loads per such wave and step
-  static constexpr int L3 = RING == 2 ? L : (L + 3) / 4;    // of them, in the slice behind the barrier
+  static constexpr int GROUPS = 2 * FM;                     // of FN MFMAs, in a step
+  static constexpr int PB = GROUPS - 3;                     // the group behind the step's barrier
+  static constexpr int LB = RING == 2 ? L : (3 * L + GROUPS - 1) / GROUPS;  // loads in the groups behind it
   static constexpr int RA = (BM + 63) / 64 * 64, RO = (BO + 63) / 64 * 64;  // scale regions
   static constexpr int NSC = RA + (GLU ? 2 : 1) * RO;
   static constexpr int OUT = BM * BO * 2;
   static constexpr int MAIN = RING * SLOT > OUT ? RING * SLOT : OUT;
   static constexpr int SMEM = MAIN + NSC * 4;
-  static constexpr int GROUPS = FM * FN;                     // MFMAs of a slice
-  static constexpr int RPG = (2 * (FM + FN) + GROUPS - 1) / GROUPS;  // fragments read beside a MFMA: all in the slice's first half
   static constexpr int SW = (BO / 4) % 16 == 0 ? 15 : 7;     // swizzle of the staged output's 8-byte units
-  // first output column of accumulator quad q of block column j (lanes of h = 1 hold the next four)
-  static constexpr __device__ int col(int wn, int j, int q) {
-    return GLU ? wn * (TN / 2) + 16 * j + 8 * (q >> 1) : wn * TN + 32 * j + 8 * q;
-  }
-  static_assert(FM * 32 * WM == BM && FN * 32 * WN == BN && AL * 8 * LW == BM && BL * 8 * LW == BN, "tile");
-  static_assert(!GLU || LW % 2 == 0, "a wave loads gate rows or up rows");
+  // first output column of block column j (lane group g = lane >> 4 holds four from 4 g on)
+  static constexpr __device__ int col(int wn, int j) { return GLU ? wn * (TN / 2) + 8 * j : wn * TN + 16 * j; }
+  static_assert(FM * 16 * WM == BM && FN * 16 * WN == BN && AL * 8 * LW == BM && BL * 8 * LW == BN, "tile");
+  static_assert(FM % 2 == 0 && (!GLU || (LW == 4 && FN % 2 == 0)), "A fragments in a ring of four; gate and up in one wave");
   static_assert((BO / 4) % 8 == 0 && SMEM <= 163840, "LDS");
 };
-
-__device__ inline i16v mfma32_i8(u4 a, u4 b, i16v c) {
-  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i4, a), __builtin_bit_cast(i4, b), c, 0, 0, 0);
-}
 
 template <int N>
 __device__ __forceinline__ void tile_barrier() {  // all but the N latest loads have landed, LDS reads are done
@@ -86,10 +78,10 @@ __global__ __launch_bounds__(C::NT, 1) void int8_tile_kernel(Int8Args p) {
   const int K = p.K, m0 = tm * C::BM, n0 = tn * C::BO;
   const int rows_m = min(C::BM, p.M - m0), rows_n = min(C::BO, p.N - n0);
   const __amdgpu_buffer_rsrc_t rA = int8_rsrc(p.a + (size_t)m0 * K, (uint32_t)rows_m * (uint32_t)K);
-  // The gated block's tile holds eight gate rows of b, then the eight up rows of the same
-  // outputs, and so on: a loading wave takes the ones or the others, and a lane's
-  // accumulators hold both factors of its outputs.
-  const int up_rows = C::GLU && (wave & 1) ? p.N : 0;
+  // The gated block's tile holds sixteen gate rows of b, then the sixteen up rows of the same
+  // outputs, and so on: loading waves 0 and 1 take the ones, 2 and 3 the others, and a
+  // lane's accumulators hold both factors of its outputs.
+  const int up_rows = C::GLU && (wave & 2) ? p.N : 0;
   const __amdgpu_buffer_rsrc_t rB = int8_rsrc(p.b + (size_t)(up_rows + n0) * K, (uint32_t)rows_n * (uint32_t)K);
 
   // scales to LDS: BM row scales, BO gate (or plain) and BO up scales, in runs of 64
@@ -115,7 +107,7 @@ __global__ __launch_bounds__(C::NT, 1) void int8_tile_kernel(Int8Args p) {
     va[i] = (uint32_t)min(8 * (wave + C::LW * i) + (lane >> 3), rows_m - 1) * (uint32_t)K + cofs;
 #pragma unroll
   for (int i = 0; i < C::BL; ++i) {
-    const int r = (C::GLU ? (wave + C::LW * i) >> 1 : wave + C::LW * i) * 8;
+    const int q = wave + C::LW * i, r = 8 * (C::GLU ? (q >> 2) * 2 + (q & 1) : q);
     vb[i] = (uint32_t)min(r + (lane >> 3), rows_n - 1) * (uint32_t)K + cofs;
   }
   const int steps = (K + C::BK - 1) / C::BK;
@@ -138,122 +130,125 @@ __global__ __launch_bounds__(C::NT, 1) void int8_tile_kernel(Int8Args p) {
     }
 #endif
   };
-  // a step's loads are issued behind the barrier of its slot's last use, spread over
-  // that step's last slice and the next step's first ones
-  constexpr int L3 = C::L3;
-
   const bool loader = wave < C::LW;
   if (loader) {
 #pragma unroll
     for (int s = 0; s < RING; ++s)
 #pragma unroll
-      for (int i = 0; i < (s + 1 < RING ? L : L3); ++i) load(i, s, s);
+      for (int i = 0; i < (s + 1 < RING ? L : C::LB); ++i) load(i, s, s);
   }
 
-  const int r32 = lane & 31, h = lane >> 5;
-  const uint32_t la = (uint32_t)((wm * C::TM + r32) * C::BK), lb = (uint32_t)(C::ASLOT + (wn * C::TN + r32) * C::BK);
-  const uint32_t sw = (uint32_t)((h ^ ((r32 >> 1) & 7)) * 16);
-  i16v acc[FM][FN];
+  const int r16 = lane & 15, g = lane >> 4;
+  const uint32_t la = (uint32_t)((wm * C::TM + r16) * C::BK), lb = (uint32_t)(C::ASLOT + (wn * C::TN + r16) * C::BK);
+  const uint32_t sw = (uint32_t)((g ^ ((r16 >> 1) & 7)) * 16);
+  i4 acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
-  u4 fa[2][FM], fb[2][FN];
-  // fragment f (b's first) of slice s of a slot into set e
-  auto read = [&](int f, int slot, int s, int e) __attribute__((always_inline)) {
-    const uint8_t* at = smem + slot * C::SLOT + (sw ^ (32u * s));
-    if (f < FN) fb[e][f] = *reinterpret_cast<const u4*>(at + lb + f * 32 * C::BK);
-    else fa[e][f - FN] = *reinterpret_cast<const u4*>(at + la + (f - FN) * 32 * C::BK);
+    for (int j = 0; j < FN; ++j) acc[i][j] = i4{0, 0, 0, 0};
+  // A step is two halves of 64 K values, FM groups each: A fragment i of the half against
+  // its FN B fragments.  A fragments pass through a ring of four, read three groups
+  // ahead; B fragments are held in two sets.
+  u4 fa[4], fb[2][FN];
+  auto read_a = [&](int q, int slot) __attribute__((always_inline)) {  // of group q
+    fa[q & 3] = *reinterpret_cast<const u4*>(smem + slot * C::SLOT + (sw ^ (q < FM ? 0u : 64u)) + la + (q % FM) * 16 * C::BK);
+  };
+  auto read_b = [&](int j, int slot, int half) __attribute__((always_inline)) {
+    fb[half][j] = *reinterpret_cast<const u4*>(smem + slot * C::SLOT + (sw ^ (64u * half)) + lb + j * 16 * C::BK);
   };
 
-  tile_barrier<(RING - 2) * L + L3>();
+  tile_barrier<(RING - 2) * L + C::LB>();
 #pragma unroll
-  for (int f = 0; f < FM + FN; ++f) read(f, 0, 0, 0);
+  for (int j = 0; j < FN; ++j) read_b(j, 0, 0);
+#pragma unroll
+  for (int q = 0; q < 3; ++q) read_a(q, 0);
 
   int c = 0;
   for (int kt = 0; kt < n; ++kt) {
     const int cn = c + 1 == RING ? 0 : c + 1, cp = c == 0 ? RING - 1 : c - 1;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      if (s == 3) tile_barrier<(RING - 2) * L>();
-      constexpr int RL = L - L3;                     // loads left for slices 0 .. 2
+    for (int q = 0; q < C::GROUPS; ++q) {
+      // The barrier: the next step's slot has landed, this step's is fully read.  Behind the
+      // last step the reads are of whatever the next slot holds, and unused.
+      if (q == C::PB) tile_barrier<(RING - 2) * L>();
+      if (q < C::PB) {
+        constexpr int QB = FM < C::PB ? FM : C::PB;  // the second half's B fragments: in the first groups
 #pragma unroll
-      for (int g = 0; g < C::GROUPS; ++g) {
-        // (behind the last step the reads are of whatever the next slot holds)
+        for (int j = q * FN / QB; j < (q + 1) * FN / QB && j < FN; ++j) read_b(j, c, 1);
+        read_a(q + 3, c);
+      } else {
+        constexpr int Q0 = C::PB > FM ? C::PB : FM, NQ = C::GROUPS - Q0;  // (the first half's are free from group FM on)
+        if (q >= Q0) {
 #pragma unroll
-        for (int f = g * C::RPG; f < (g + 1) * C::RPG && f < FM + FN; ++f) read(f, s == 3 ? cn : c, (s + 1) & 3, (s + 1) & 1);
-        const int i = g / FN, j = g % FN;
-        acc[i][j] = mfma32_i8(fb[s & 1][j], fa[s & 1][i], acc[i][j]);
-        if (!loader) {
-        } else if (s == 3) {
-#pragma unroll
-          for (int q = g * L3 / C::GROUPS; q < (g + 1) * L3 / C::GROUPS; ++q) load(q, kt + RING, c);
-        } else {
-#pragma unroll
-          for (int q = (s * C::GROUPS + g) * RL / (3 * C::GROUPS); q < (s * C::GROUPS + g + 1) * RL / (3 * C::GROUPS); ++q)
-            load(L3 + q, kt + RING - 1, cp);
+          for (int j = (q - Q0) * FN / NQ; j < (q - Q0 + 1) * FN / NQ; ++j) read_b(j, cn, 0);
         }
-        __builtin_amdgcn_sched_barrier(0);
+        read_a(q - C::PB, cn);
       }
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        acc[q % FM][j] = mfma_i8(fb[q / FM][j], fa[q & 3], acc[q % FM][j]);
+        // the loads of step kt + RING into the slot just read, then the rest of the step before's
+        if (loader && j + 1 == FN) {
+          if (q >= C::PB) {
+#pragma unroll
+            for (int i = (q - C::PB) * C::LB / 3; i < (q - C::PB + 1) * C::LB / 3; ++i) load(i, kt + RING, c);
+          } else {
+#pragma unroll
+            for (int i = C::LB + q * (L - C::LB) / C::PB; i < C::LB + (q + 1) * (L - C::LB) / C::PB; ++i)
+              load(i, kt + RING - 1, cp);
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     c = cn;
   }
   tile_barrier<0>();
 
-  // Lane l holds, of block (i, j), row m = l & 31 and columns 8 (v / 4) + 4 (l >> 5) + v % 4.
+  // Lane l holds, of block (i, j), row m = l & 15 and columns 4 (l >> 4) + v.
   if constexpr (SPLIT) {
     const int NB = C::GLU ? 2 * p.N : p.N;
     int32_t* P = p.part + (size_t)part * p.M * NB;
     const bool vec = (p.N & 3) == 0;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-      const int m = m0 + wm * C::TM + i * 32 + r32;
+      const int m = m0 + wm * C::TM + i * 16 + r16;
       if (m >= p.M) continue;
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
+      for (int j = 0; j < FN; ++j) {
+        const bool up = C::GLU && (j & 1);
+        const int nn = n0 + C::col(wn, up ? j - 1 : j) + 4 * g;
+        int32_t* dst = P + (size_t)m * NB + (up ? p.N : 0) + nn;
+        if (vec && nn < p.N) *reinterpret_cast<i4*>(dst) = acc[i][j];
+        else
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const bool up = C::GLU && (q & 1);
-          const int nn = n0 + C::col(wn, j, q) + 4 * h;
-          int32_t* dst = P + (size_t)m * NB + (up ? p.N : 0) + nn;
-          const i4 v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-          if (vec && nn < p.N) *reinterpret_cast<i4*>(dst) = v;
-          else
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (nn + e < p.N) dst[e] = v[e];
-        }
+          for (int e = 0; e < 4; ++e)
+            if (nn + e < p.N) dst[e] = acc[i][j][e];
+      }
     }
     return;
   }
   uint8_t* const out = smem;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
-    const int m = wm * C::TM + i * 32 + r32;
+    const int m = wm * C::TM + i * 16 + r16;
     const float s0 = sc[m];
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
+    for (int j = 0; j < FN; j += C::GLU ? 2 : 1) {
+      const int nn = C::col(wn, j) + 4 * g;
+      const f4 sg = *reinterpret_cast<const f4*>(sc + C::RA + nn);
+      float o[4];
+      if constexpr (C::GLU) {
+        const f4 su = *reinterpret_cast<const f4*>(sc + C::RA + C::RO + nn);
 #pragma unroll
-      for (int q = 0; q < 4; q += C::GLU ? 2 : 1) {
-        const int nn = C::col(wn, j, q) + 4 * h;
-        const f4 sg = *reinterpret_cast<const f4*>(sc + C::RA + nn);
-        float o[4];
-        if constexpr (C::GLU) {
-          const f4 su = *reinterpret_cast<const f4*>(sc + C::RA + C::RO + nn);
+        for (int e = 0; e < 4; ++e) o[e] = int8_glu<ACT>(acc[i][j][e], acc[i][j + 1][e], s0, sg[e], su[e]);
+      } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int ag = acc[i][j][4 * q + e], au = acc[i][j][4 * q + 4 + e];
-            o[e] = int8_glu<ACT>(ag, au, s0, sg[e], su[e]);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = int8_scaled(acc[i][j][4 * q + e], s0, sg[e]);
-        }
-        const uint2 w = make_uint2(int8_pack2<T>(o[0], o[1]), int8_pack2<T>(o[2], o[3]));
-        *reinterpret_cast<uint2*>(out + (size_t)m * (C::BO * 2) + ((nn >> 2) ^ (m & C::SW)) * 8) = w;
+        for (int e = 0; e < 4; ++e) o[e] = int8_scaled(acc[i][j][e], s0, sg[e]);
       }
+      *reinterpret_cast<uint2*>(out + (size_t)m * (C::BO * 2) + ((nn >> 2) ^ (m & C::SW)) * 8) =
+          make_uint2(int8_pack2<T>(o[0], o[1]), int8_pack2<T>(o[2], o[3]));
+    }
   }
   __syncthreads();
   uint16_t* const Y = p.y + (size_t)m0 * p.N + n0;
