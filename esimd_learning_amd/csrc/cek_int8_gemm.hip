@@ -153,14 +153,14 @@ template <class T, int ACT>
 static int launch_int8_t(Int8Args& g, int cfg, hipStream_t st) {
   constexpr bool G = ACT >= 0;
   switch (cfg) {
-    case 0: return launch_int8_tile<Int8Tile<256, 256, 2, 4, 4, 2, G>, T, ACT>(g, st);
-    case 1: return launch_int8_tile<Int8Tile<256, 192, 4, 2, 4, 2, G>, T, ACT>(g, st);
-    case 2: return launch_int8_tile<Int8Tile<256, 128, 4, 2, 4, 3, G>, T, ACT>(g, st);
-    case 3: return launch_int8_tile<Int8Tile<128, 256, 2, 4, 4, 3, G>, T, ACT>(g, st);
-    case 4: return launch_int8_tile<Int8Tile<128, 192, 4, 2, 4, 3, G>, T, ACT>(g, st);
-    case 5: return launch_int8_tile<Int8Tile<128, 128, 2, 4, 4, 4, G>, T, ACT>(g, st);
-    case 6: return launch_int8_tile<Int8Tile<64, 256, 2, 4, 4, 3, G>, T, ACT>(g, st);
-    case 7: return launch_int8_tile<Int8Tile<64, 128, 2, 4, 4, 5, G>, T, ACT>(g, st);
+    case 0: return launch_int8_tile<Int8Tile<256, 256, 2, 4, 2, 2, G>, T, ACT>(g, st);
+    case 1: return launch_int8_tile<Int8Tile<256, 192, 4, 2, 2, 3, G>, T, ACT>(g, st);
+    case 2: return launch_int8_tile<Int8Tile<256, 128, 4, 2, 3, 3, G>, T, ACT>(g, st);
+    case 3: return launch_int8_tile<Int8Tile<128, 256, 2, 4, 3, 3, G>, T, ACT>(g, st);
+    case 4: return launch_int8_tile<Int8Tile<128, 192, 4, 2, 3, 4, G>, T, ACT>(g, st);
+    case 5: return launch_int8_tile<Int8Tile<128, 128, 2, 4, 4, 5, G>, T, ACT>(g, st);
+    case 6: return launch_int8_tile<Int8Tile<64, 256, 2, 4, 3, 4, G>, T, ACT>(g, st);
+    case 7: return launch_int8_tile<Int8Tile<64, 128, 2, 4, 5, 6, G>, T, ACT>(g, st);
     default: return CEK_ERR_UNSUPPORTED;
   }
 }

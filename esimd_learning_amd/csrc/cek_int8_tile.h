@@ -5,29 +5,33 @@
 
 namespace cek {
 
-template <int BM_, int BN_, int WM_, int WN_, int LW_, int RING_, bool GLU_>
+// RA slots of A, RB of B: a step's loads go out RA steps ahead, B's RB.
+template <int BM_, int BN_, int WM_, int WN_, int RA_, int RB_, bool GLU_>
 struct Int8Tile {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, RING = RING_, BK = 128;
+  static constexpr int BM = BM_, BN = BN_, BK = 128, WM = WM_, WN = WN_, RA = RA_, RB = RB_;
   static constexpr bool GLU = GLU_;
   static constexpr int BO = GLU ? BN / 2 : BN;              // output columns
   static constexpr int NW = WM * WN, NT = 64 * NW;
   static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-  static constexpr int ASLOT = BM * BK, BSLOT = BN * BK, SLOT = ASLOT + BSLOT;
-  static constexpr int LW = LW_;                            // waves that load
+  static constexpr int ASLOT = BM * BK, BSLOT = BN * BK;
+  static constexpr int LW = 4;                              // waves that load
   static constexpr int AL = BM / 8 / LW, BL = BN / 8 / LW, L = AL + BL;  // 1 KB loads per such wave and step
   static constexpr int GROUPS = 2 * FM;                     // of FN MFMAs, in a step
   static constexpr int PB = GROUPS - 3;                     // the group behind the step's barrier
-  static constexpr int LB = RING == 2 ? L : (3 * L + GROUPS - 1) / GROUPS;  // loads in the groups behind it
-  static constexpr int RA = (BM + 63) / 64 * 64, RO = (BO + 63) / 64 * 64;  // scale regions
-  static constexpr int NSC = RA + (GLU ? 2 : 1) * RO;
+  static constexpr int LB = RA == 2 ? L : (3 * L + GROUPS - 1) / GROUPS;  // loads in the groups behind it
+  // in flight at the barrier: what was issued behind the A rows of the next step
+  static constexpr int FLY = (RA - 2) * L + (RB > RA ? BL : 0);
+  static constexpr int SA = (BM + 63) / 64 * 64, SO = (BO + 63) / 64 * 64;  // scale regions
+  static constexpr int NSC = SA + (GLU ? 2 : 1) * SO;
   static constexpr int OUT = BM * BO * 2;
-  static constexpr int MAIN = RING * SLOT > OUT ? RING * SLOT : OUT;
+  static constexpr int RINGS = RA * ASLOT + RB * BSLOT, MAIN = RINGS > OUT ? RINGS : OUT;
   static constexpr int SMEM = MAIN + NSC * 4;
   static constexpr int SW = (BO / 4) % 16 == 0 ? 15 : 7;     // swizzle of the staged output's 8-byte units
   // first output column of block column j (lane group g = lane >> 4 holds four from 4 g on)
   static constexpr __device__ int col(int wn, int j) { return GLU ? wn * (TN / 2) + 8 * j : wn * TN + 16 * j; }
   static_assert(FM * 16 * WM == BM && FN * 16 * WN == BN && AL * 8 * LW == BM && BL * 8 * LW == BN, "tile");
-  static_assert(FM % 2 == 0 && (!GLU || (LW == 4 && FN % 2 == 0)), "A fragments in a ring of four; gate and up in one wave");
+  static_assert(GROUPS % 4 == 0 && (!GLU || FN % 2 == 0), "A fragments in a ring of four; gate and up in one wave");
+  static_assert(RA >= 2 && (RB == RA || RB == RA + 1) && FLY + LB <= 63, "rings");
   static_assert((BO / 4) % 8 == 0 && SMEM <= 163840, "LDS");
 };
 
@@ -68,7 +72,7 @@ struct Int8Args {
 
 template <class C, class T, int ACT, bool SPLIT>
 __global__ __launch_bounds__(C::NT, 1) void int8_tile_kernel(Int8Args p) {
-  constexpr int FM = C::FM, FN = C::FN, L = C::L, RING = C::RING;
+  constexpr int FM = C::FM, FN = C::FN, L = C::L, RA = C::RA, RB = C::RB;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[C::SMEM];
   float* const sc = reinterpret_cast<float*>(smem + C::MAIN);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -88,9 +92,9 @@ __global__ __launch_bounds__(C::NT, 1) void int8_tile_kernel(Int8Args p) {
 #pragma unroll
   for (int q = 0; q < C::NSC / 64; ++q) {
     if (q % C::NW != wave) continue;
-    const bool isA = q < C::RA / 64;
-    const int base = isA ? q * 64 : (q * 64 - C::RA) % C::RO;
-    const bool up = C::GLU && q * 64 >= C::RA + C::RO;
+    const bool isA = q < C::SA / 64;
+    const int base = isA ? q * 64 : (q * 64 - C::SA) % C::SO;
+    const bool up = C::GLU && q * 64 >= C::SA + C::SO;
     const float* src = isA ? p.sa + m0 : p.sb + n0 + (up ? p.N : 0);
 #if defined(__HIP_DEVICE_COMPILE__)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(int8_rsrc(src, (uint32_t)(isA ? rows_m : rows_n) * 4u),
@@ -98,49 +102,60 @@ __global__ __launch_bounds__(C::NT, 1) void int8_tile_kernel(Int8Args p) {
 #endif
   }
 
-  // load i of this wave: rows 8 (wave + NW i) .. + 7 of the slice, lane l row l >> 3 at
-  // position l & 7, which holds the row's 16-byte chunk (l & 7) ^ ((row >> 1) & 7)
-  const uint32_t cofs = (uint32_t)(((lane & 7) ^ ((lane >> 4) + 4 * (wave & 1))) * 16);
+  // Load i of this wave: rows 8 (wave + LW i) on of the slice, lane l row l >> 3 at position
+  // l & 7.  A row's 16-byte chunk k lies at k ^ swz(row): the sixteen rows of a fragment
+  // read then fall in all 64 banks.
+  auto swz = [](int row) { return (row >> 1) & 7; };
+  const int lrow = lane >> 3;
+  const uint32_t cofs = (uint32_t)(((lane & 7) ^ swz(8 * (wave & 1) + lrow)) * 16);
   uint32_t va[C::AL], vb[C::BL];
 #pragma unroll
-  for (int i = 0; i < C::AL; ++i)
-    va[i] = (uint32_t)min(8 * (wave + C::LW * i) + (lane >> 3), rows_m - 1) * (uint32_t)K + cofs;
+  for (int i = 0; i < C::AL; ++i) va[i] = (uint32_t)min(8 * (wave + C::LW * i) + lrow, rows_m - 1) * (uint32_t)K + cofs;
 #pragma unroll
   for (int i = 0; i < C::BL; ++i) {
-    const int q = wave + C::LW * i, r = 8 * (C::GLU ? (q >> 2) * 2 + (q & 1) : q);
-    vb[i] = (uint32_t)min(r + (lane >> 3), rows_n - 1) * (uint32_t)K + cofs;
+    const int r = 8 * (wave + C::LW * i);
+    vb[i] = (uint32_t)min((C::GLU ? (r >> 5) * 16 + (r & 15) : r) + lrow, rows_n - 1) * (uint32_t)K + cofs;
   }
   const int steps = (K + C::BK - 1) / C::BK;
   const int k0 = SPLIT ? (int)((int64_t)steps * part / p.parts) : 0;
-  const int n = (SPLIT ? (int)((int64_t)steps * (part + 1) / p.parts) : steps) - k0;
+  const int n = (SPLIT ? (int)((int64_t)steps * (part + 1) / p.parts) : steps) - k0;  // steps of this part
 
-  auto load = [&](int i, int step, int slot) __attribute__((always_inline)) {
+  uint8_t* const sB = smem + RA * C::ASLOT;
+  auto load_a = [&](int i, int step, int slot) __attribute__((always_inline)) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    // past the part: nothing; past the row's end: zeros for a, what lies there for b
-    const uint32_t kb = step < n ? (uint32_t)(k0 + step) * C::BK : kOutOfRange;
-    if (i < C::BL) {
-      const int r = 8 * (wave + C::LW * i);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rB, (lds_ptr_t)(smem + slot * C::SLOT + C::ASLOT + r * C::BK), 16,
-                                               vb[i] + kb, 0, 0, 0);
-    } else {
-      const int j = i - C::BL;
-      const uint32_t ka = kb + cofs >= (uint32_t)K ? kOutOfRange : kb;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rA, (lds_ptr_t)(smem + slot * C::SLOT + 8 * (wave + C::LW * j) * C::BK), 16,
-                                               va[j] + ka, 0, 0, 0);
-    }
+    // past the part: nothing (zeros); past the row's end: zeros, whatever b has there
+    const uint32_t kb = step < n ? (uint32_t)(k0 + step) * C::BK : kOutOfRange, ka = kb + cofs >= (uint32_t)K ? kOutOfRange : kb;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rA, (lds_ptr_t)(smem + slot * C::ASLOT + 1024 * (wave + C::LW * i)), 16, va[i] + ka,
+                                             0, 0, 0);
 #endif
+  };
+  auto load_b = [&](int i, int step, int slot) __attribute__((always_inline)) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const uint32_t kb = step < n ? (uint32_t)(k0 + step) * C::BK : kOutOfRange;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rB, (lds_ptr_t)(sB + slot * C::BSLOT + 1024 * (wave + C::LW * i)), 16, vb[i] + kb,
+                                             0, 0, 0);
+#endif
+  };
+  // Load i of the group that step k's barrier lets go: A of step k + RA, then B of step k + RB.
+  auto load = [&](int i, int k, int ca, int cb) __attribute__((always_inline)) {
+    if (i < C::AL) load_a(i, k + RA, ca);
+    else load_b(i - C::AL, k + RB, cb);
   };
   const bool loader = wave < C::LW;
   if (loader) {
 #pragma unroll
-    for (int s = 0; s < RING; ++s)
+    for (int s = 0; s < RB - RA; ++s)
 #pragma unroll
-      for (int i = 0; i < (s + 1 < RING ? L : C::LB); ++i) load(i, s, s);
+      for (int i = 0; i < C::BL; ++i) load_b(i, s, s);
+#pragma unroll
+    for (int s = 0; s < RA; ++s)
+#pragma unroll
+      for (int i = 0; i < (s + 1 < RA ? L : C::LB); ++i) load(i, s - RA, s, s + RB - RA);
   }
 
   const int r16 = lane & 15, g = lane >> 4;
-  const uint32_t la = (uint32_t)((wm * C::TM + r16) * C::BK), lb = (uint32_t)(C::ASLOT + (wn * C::TN + r16) * C::BK);
-  const uint32_t sw = (uint32_t)((g ^ ((r16 >> 1) & 7)) * 16);
+  const uint32_t la = (uint32_t)((wm * C::TM + r16) * C::BK), lb = (uint32_t)((wn * C::TN + r16) * C::BK);
+  const uint32_t sw = (uint32_t)((g ^ swz(r16)) * 16);
   i4 acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -148,60 +163,60 @@ __global__ __launch_bounds__(C::NT, 1) void int8_tile_kernel(Int8Args p) {
     for (int j = 0; j < FN; ++j) acc[i][j] = i4{0, 0, 0, 0};
   // A step is two halves of 64 K values, FM groups each: A fragment i of the half against
   // its FN B fragments.  A fragments pass through a ring of four, read three groups
-  // ahead; B fragments are held in two sets.
+  // ahead; B fragments are held in two sets, the halves'.
   u4 fa[4], fb[2][FN];
   auto read_a = [&](int q, int slot) __attribute__((always_inline)) {  // of group q
-    fa[q & 3] = *reinterpret_cast<const u4*>(smem + slot * C::SLOT + (sw ^ (q < FM ? 0u : 64u)) + la + (q % FM) * 16 * C::BK);
+    fa[q & 3] = *reinterpret_cast<const u4*>(smem + slot * C::ASLOT + (sw ^ (q < FM ? 0u : 64u)) + la + (q % FM) * 16 * C::BK);
   };
   auto read_b = [&](int j, int slot, int half) __attribute__((always_inline)) {
-    fb[half][j] = *reinterpret_cast<const u4*>(smem + slot * C::SLOT + (sw ^ (64u * half)) + lb + j * 16 * C::BK);
+    fb[half][j] = *reinterpret_cast<const u4*>(sB + slot * C::BSLOT + (sw ^ (64u * half)) + lb + j * 16 * C::BK);
   };
 
-  tile_barrier<(RING - 2) * L + C::LB>();
+  tile_barrier<C::FLY + C::LB>();
 #pragma unroll
   for (int j = 0; j < FN; ++j) read_b(j, 0, 0);
 #pragma unroll
   for (int q = 0; q < 3; ++q) read_a(q, 0);
 
-  int c = 0;
+  int ca = 0, cb = 0;
   for (int kt = 0; kt < n; ++kt) {
-    const int cn = c + 1 == RING ? 0 : c + 1, cp = c == 0 ? RING - 1 : c - 1;
+    const int na = ca + 1 == RA ? 0 : ca + 1, nb = cb + 1 == RB ? 0 : cb + 1;
+    const int pa = ca == 0 ? RA - 1 : ca - 1, pb = cb == 0 ? RB - 1 : cb - 1;
 #pragma unroll
     for (int q = 0; q < C::GROUPS; ++q) {
-      // The barrier: the next step's slot has landed, this step's is fully read.  Behind the
-      // last step the reads are of whatever the next slot holds, and unused.
-      if (q == C::PB) tile_barrier<(RING - 2) * L>();
+      // The barrier: the next step's slots have landed, this step's are fully read.  Behind
+      // the last step the reads are of whatever the next slots hold, and unused.
+      if (q == C::PB) tile_barrier<C::FLY>();
       if (q < C::PB) {
         constexpr int QB = FM < C::PB ? FM : C::PB;  // the second half's B fragments: in the first groups
 #pragma unroll
-        for (int j = q * FN / QB; j < (q + 1) * FN / QB && j < FN; ++j) read_b(j, c, 1);
-        read_a(q + 3, c);
+        for (int j = q * FN / QB; j < (q + 1) * FN / QB && j < FN; ++j) read_b(j, cb, 1);
+        read_a(q + 3, ca);
       } else {
         constexpr int Q0 = C::PB > FM ? C::PB : FM, NQ = C::GROUPS - Q0;  // (the first half's are free from group FM on)
         if (q >= Q0) {
 #pragma unroll
-          for (int j = (q - Q0) * FN / NQ; j < (q - Q0 + 1) * FN / NQ; ++j) read_b(j, cn, 0);
+          for (int j = (q - Q0) * FN / NQ; j < (q - Q0 + 1) * FN / NQ; ++j) read_b(j, nb, 0);
         }
-        read_a(q - C::PB, cn);
+        read_a(q - C::PB, na);
       }
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        acc[q % FM][j] = mfma_i8(fb[q / FM][j], fa[q & 3], acc[q % FM][j]);
-        // the loads of step kt + RING into the slot just read, then the rest of the step before's
-        if (loader && j + 1 == FN) {
-          if (q >= C::PB) {
+      for (int j = 0; j < FN; ++j) acc[q % FM][j] = mfma_i8(fb[q / FM][j], fa[q & 3], acc[q % FM][j]);
+      // the group of loads that this barrier lets go, then the rest of the one before's
+      if (loader) {
+        if (q >= C::PB) {
 #pragma unroll
-            for (int i = (q - C::PB) * C::LB / 3; i < (q - C::PB + 1) * C::LB / 3; ++i) load(i, kt + RING, c);
-          } else {
+          for (int i = (q - C::PB) * C::LB / 3; i < (q - C::PB + 1) * C::LB / 3; ++i) load(i, kt, ca, cb);
+        } else {
 #pragma unroll
-            for (int i = C::LB + q * (L - C::LB) / C::PB; i < C::LB + (q + 1) * (L - C::LB) / C::PB; ++i)
-              load(i, kt + RING - 1, cp);
-          }
+          for (int i = C::LB + q * (L - C::LB) / C::PB; i < C::LB + (q + 1) * (L - C::LB) / C::PB; ++i)
+            load(i, kt - 1, pa, pb);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    c = cn;
+    ca = na;
+    cb = nb;
   }
   tile_barrier<0>();
 
@@ -236,10 +251,10 @@ __global__ __launch_bounds__(C::NT, 1) void int8_tile_kernel(Int8Args p) {
 #pragma unroll
     for (int j = 0; j < FN; j += C::GLU ? 2 : 1) {
       const int nn = C::col(wn, j) + 4 * g;
-      const f4 sg = *reinterpret_cast<const f4*>(sc + C::RA + nn);
+      const f4 sg = *reinterpret_cast<const f4*>(sc + C::SA + nn);
       float o[4];
       if constexpr (C::GLU) {
-        const f4 su = *reinterpret_cast<const f4*>(sc + C::RA + C::RO + nn);
+        const f4 su = *reinterpret_cast<const f4*>(sc + C::SA + C::SO + nn);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = int8_glu<ACT>(acc[i][j][e], acc[i][j + 1][e], s0, sg[e], su[e]);
       } else {
