@@ -17,8 +17,8 @@ struct Int8Tile {
   static constexpr int LW = 4;                              // waves that load
   static constexpr int AL = BM / 8 / LW, BL = BN / 8 / LW, L = AL + BL;  // 1 KB loads per such wave and step
   static constexpr int GROUPS = 2 * FM;                     // of FN MFMAs, in a step
-  static constexpr int PB = GROUPS - 3;                     // the group behind the step's barrier
-  static constexpr int LB = RA == 2 ? L : (3 * L + GROUPS - 1) / GROUPS;  // loads in the groups behind it
+  static constexpr int PB = GROUPS > 4 ? GROUPS - 4 : 1, NB = GROUPS - PB;  // the group before the step's barrier
+  static constexpr int LB = RA == 2 ? L : (NB * L + GROUPS - 1) / GROUPS;  // loads in the groups from there on
   // in flight at the barrier: what was issued behind the A rows of the next step
   static constexpr int FLY = (RA - 2) * L + (RB > RA ? BL : 0);
   static constexpr int SA = (BM + 63) / 64 * 64, SO = (BO + 63) / 64 * 64;  // scale regions
@@ -162,8 +162,9 @@ __global__ __launch_bounds__(C::NT, 1) void int8_tile_kernel(Int8Args p) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = i4{0, 0, 0, 0};
   // A step is two halves of 64 K values, FM groups each: A fragment i of the half against
-  // its FN B fragments.  A fragments pass through a ring of four, read three groups
-  // ahead; B fragments are held in two sets, the halves'.
+  // its FN B fragments.  A fragments pass through a ring of four: group q's place takes
+  // group q + 4's, read as soon as group q's MFMAs are out.  B fragments are held in two
+  // sets, the halves'.
   u4 fa[4], fb[2][FN];
   auto read_a = [&](int q, int slot) __attribute__((always_inline)) {  // of group q
     fa[q & 3] = *reinterpret_cast<const u4*>(smem + slot * C::ASLOT + (sw ^ (q < FM ? 0u : 64u)) + la + (q % FM) * 16 * C::BK);
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(C::NT, 1) void int8_tile_kernel(Int8Args p) {
 #pragma unroll
   for (int j = 0; j < FN; ++j) read_b(j, 0, 0);
 #pragma unroll
-  for (int q = 0; q < 3; ++q) read_a(q, 0);
+  for (int q = 0; q < 4; ++q) read_a(q, 0);
 
   int ca = 0, cb = 0;
   for (int kt = 0; kt < n; ++kt) {
@@ -184,29 +185,33 @@ __global__ __launch_bounds__(C::NT, 1) void int8_tile_kernel(Int8Args p) {
     const int pa = ca == 0 ? RA - 1 : ca - 1, pb = cb == 0 ? RB - 1 : cb - 1;
 #pragma unroll
     for (int q = 0; q < C::GROUPS; ++q) {
-      // The barrier: the next step's slots have landed, this step's are fully read.  Behind
-      // the last step the reads are of whatever the next slots hold, and unused.
-      if (q == C::PB) tile_barrier<C::FLY>();
-      if (q < C::PB) {
-        constexpr int QB = FM < C::PB ? FM : C::PB;  // the second half's B fragments: in the first groups
-#pragma unroll
-        for (int j = q * FN / QB; j < (q + 1) * FN / QB && j < FN; ++j) read_b(j, cb, 1);
-        read_a(q + 3, ca);
-      } else {
-        constexpr int Q0 = C::PB > FM ? C::PB : FM, NQ = C::GROUPS - Q0;  // (the first half's are free from group FM on)
-        if (q >= Q0) {
-#pragma unroll
-          for (int j = (q - Q0) * FN / NQ; j < (q - Q0 + 1) * FN / NQ; ++j) read_b(j, nb, 0);
-        }
-        read_a(q - C::PB, na);
-      }
 #pragma unroll
       for (int j = 0; j < FN; ++j) acc[q % FM][j] = mfma_i8(fb[q / FM][j], fa[q & 3], acc[q % FM][j]);
+      // The barrier, a group or more behind the last read of this step's slots: the next
+      // step's have landed, this step's are fully read.  Behind the last step the reads
+      // are of whatever the next slots hold, and unused.
+      if (q == C::PB) tile_barrier<C::FLY>();
+      constexpr int QB = FM - 1;                                 // the second half's B fragments: behind groups 0 ..
+      if (q < QB) {
+#pragma unroll
+        for (int j = q * FN / QB; j < (q + 1) * FN / QB; ++j) read_b(j, cb, 1);
+      }
+      constexpr int Q0 = C::PB > QB ? C::PB : QB, NQ = C::GROUPS - 1 - Q0;  // the next first half's, once its set is free
+      if (q >= Q0 && q < Q0 + NQ) {
+#pragma unroll
+        for (int j = (q - Q0) * FN / NQ; j < (q - Q0 + 1) * FN / NQ; ++j) read_b(j, nb, 0);
+      }
+      if (q + 4 < C::GROUPS) read_a(q + 4, ca);
+      else if (q > C::PB) read_a(q + 4 - C::GROUPS, na);
+      else if (q == C::PB) {
+#pragma unroll
+        for (int i = 0; i <= C::PB + 4 - C::GROUPS; ++i) read_a(i, na);
+      }
       // the group of loads that this barrier lets go, then the rest of the one before's
       if (loader) {
         if (q >= C::PB) {
 #pragma unroll
-          for (int i = (q - C::PB) * C::LB / 3; i < (q - C::PB + 1) * C::LB / 3; ++i) load(i, kt, ca, cb);
+          for (int i = (q - C::PB) * C::LB / C::NB; i < (q - C::PB + 1) * C::LB / C::NB; ++i) load(i, kt, ca, cb);
         } else {
 #pragma unroll
           for (int i = C::LB + q * (L - C::LB) / C::PB; i < C::LB + (q + 1) * (L - C::LB) / C::PB; ++i)
