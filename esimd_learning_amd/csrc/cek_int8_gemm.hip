@@ -57,18 +57,18 @@ __global__ __launch_bounds__(256) void int8_join_kernel(const int32_t* __restric
 // Time of a launch: rounds of 256 workgroups (one per CU), each a fixed part and a
 // time per 128 values of K; a last round of fewer workgroups runs between the times
 // of a nearly empty and a full chip.  Split K adds the join and its traffic.  Fitted
-// to 1100 launches over 35 shapes of 65 to 8192 rows (weights from HBM): 10% off on
-// average, and the pick 0.6% above the fastest of all tiles and splits (geometric
-// mean; 12% at worst).  Larger tiles move fewer operand bytes per product, smaller
+// to 730 launches over 41 shapes of 72 to 8192 rows (weights from HBM): 9% off on
+// average, and the pick 0.2% above the fastest of all tiles and splits (geometric
+// mean; 3% at worst).  Larger tiles move fewer operand bytes per product, smaller
 // ones fill the chip sooner.
 struct Int8Opt {
   int bm, bn;
   double fixed, step, fixed0, step0;  // us: a full round, and one with few workgroups
 };
 constexpr Int8Opt kInt8Opts[] = {
-    {256, 256, 5.19, 1.582, 8.66, 0.957}, {256, 192, 5.12, 1.316, 7.24, 0.751}, {256, 128, 5.78, 0.823, 4.75, 0.589},
-    {128, 256, 5.90, 0.821, 5.30, 0.560}, {128, 192, 5.24, 0.772, 5.19, 0.434}, {128, 128, 4.59, 0.613, 4.78, 0.308},
-    {64, 256, 4.31, 0.694, 4.64, 0.338},  {64, 128, 4.45, 0.384, 2.76, 0.291}};
+    {256, 256, 7.11, 1.441, 7.24, 1.075}, {256, 192, 7.22, 1.125, 7.36, 0.768}, {256, 128, 6.22, 0.851, 5.12, 0.582},
+    {128, 256, 6.15, 0.874, 5.26, 0.648}, {128, 192, 6.22, 0.722, 4.07, 0.547}, {128, 128, 5.52, 0.559, 3.55, 0.404},
+    {64, 128, 4.27, 0.399, 3.25, 0.280}};
 constexpr int kInt8Tiles = sizeof(kInt8Opts) / sizeof(kInt8Opts[0]);
 constexpr int kInt8Parts[] = {1, 2, 3, 4, 6, 8, 12};
 constexpr int64_t kInt8MaxWorkspace = int64_t(1) << 28;
@@ -76,10 +76,10 @@ constexpr int64_t kInt8MaxWorkspace = int64_t(1) << 28;
 static double int8_us(const Int8Opt& o, int64_t M, int64_t NB, int64_t steps, int parts) {
   const int64_t n = (M + o.bm - 1) / o.bm * ((NB + o.bn - 1) / o.bn) * parts, full = n / kCUs, rest = n % kCUs;
   const double s = (double)((steps + parts - 1) / parts), f = (double)rest / kCUs;
-  constexpr double kStart = 2.07;  // of a round's fixed part, what only the first one takes
+  constexpr double kStart = 2.51;  // of a round's fixed part, what only the first one takes
   double t = kStart + (double)full * (o.fixed - kStart + s * o.step);
   if (rest) t += o.fixed0 + (o.fixed - o.fixed0) * f - kStart + s * (o.step0 + (o.step - o.step0) * f);
-  if (parts > 1) t += 3.15 + 3.35e-7 * 4.0 * (double)parts * (double)M * (double)NB;
+  if (parts > 1) t += 3.97 + 3.07e-7 * 4.0 * (double)parts * (double)M * (double)NB;
   return t;
 }
 
@@ -159,8 +159,7 @@ static int launch_int8_t(Int8Args& g, int cfg, hipStream_t st) {
     case 3: return launch_int8_tile<Int8Tile<128, 256, 2, 4, 3, 3, G>, T, ACT>(g, st);
     case 4: return launch_int8_tile<Int8Tile<128, 192, 4, 2, 3, 4, G>, T, ACT>(g, st);
     case 5: return launch_int8_tile<Int8Tile<128, 128, 2, 4, 4, 5, G>, T, ACT>(g, st);
-    case 6: return launch_int8_tile<Int8Tile<64, 256, 2, 4, 3, 4, G>, T, ACT>(g, st);
-    case 7: return launch_int8_tile<Int8Tile<64, 128, 2, 4, 5, 6, G>, T, ACT>(g, st);
+    case 6: return launch_int8_tile<Int8Tile<64, 128, 2, 4, 5, 6, G>, T, ACT>(g, st);
     default: return CEK_ERR_UNSUPPORTED;
   }
 }
