@@ -109,8 +109,9 @@ static Int8Plan int8_plan(int64_t M, int64_t NB, int64_t K, bool glu, int64_t ws
   return best;
 }
 
+// (a grid counts its threads in 32 bits)
 static bool int8_sizes_ok(int64_t M, int64_t N, int64_t K, int64_t NB) {
-  return M >= 0 && N >= 0 && K > 0 && K % 16 == 0 && K <= kInt8MaxK && M <= (1 << 24) && N <= INT32_MAX && NB <= INT32_MAX;
+  return M >= 0 && N >= 0 && K > 0 && K % 16 == 0 && K <= kInt8MaxK && M <= (1 << 24) && NB <= (1 << 24);
 }
 static int64_t int8_workspace(int64_t M, int64_t N, int64_t K, bool glu) {
   if (N > INT32_MAX || !int8_sizes_ok(M, N, K, glu ? 2 * N : N) || M == 0 || N == 0) return 0;
@@ -189,8 +190,9 @@ extern "C" int64_t cek_gemm_int8_a8w8_glu_workspace_size(int64_t M, int64_t d, i
 }
 
 extern "C" int cek_gemm_int8_plan(int64_t M, int64_t N, int64_t K, int gated, int64_t workspace_bytes) {
+  if (N > INT32_MAX) return -1;
   const int64_t NB = gated ? 2 * N : N;
-  if (N > INT32_MAX || !int8_sizes_ok(M, N, K, NB) || M == 0 || N == 0) return -1;
+  if (!int8_sizes_ok(M, N, K, NB) || M == 0 || N == 0) return -1;
   const Int8Plan p = int8_plan(M, NB, K, gated != 0, workspace_bytes);
   return p.cfg < 0 ? -1 : 16 * p.cfg + p.parts;
 }

@@ -291,14 +291,24 @@ static int launch_norm(const uint16_t* h, uint16_t* r, const uint16_t* w, int ro
   return check_launch();
 }
 
+// A launch takes up to 2^20 rows: a grid counts its threads in 32 bits.
 template <typename T>
-static int launch_rows(const void* x, void* residual, const void* weight, int rows, int H, float eps, int8_t* q,
+static int launch_rows(const void* x, void* residual, const void* weight, int64_t rows, int H, float eps, int8_t* q,
                        float* scale, hipStream_t st) {
   const uint16_t *xp = static_cast<const uint16_t*>(x), *w = static_cast<const uint16_t*>(weight);
   uint16_t* r = static_cast<uint16_t*>(residual);
   const bool odd = H % 8 != 0 || !aligned(x, 16) || !aligned(q, 8) || (r && (!aligned(r, 16) || !aligned(w, 16)));
-  if (r) return odd ? launch_norm<T, true>(xp, r, w, rows, H, eps, q, scale, st) : launch_norm<T, false>(xp, r, w, rows, H, eps, q, scale, st);
-  return odd ? launch_quant<T, true>(xp, rows, H, q, scale, st) : launch_quant<T, false>(xp, rows, H, q, scale, st);
+  constexpr int64_t kMost = 1 << 20;
+  for (int64_t t = 0; t < rows; t += kMost) {
+    const int n = (int)(rows - t < kMost ? rows - t : kMost);
+    const size_t at = (size_t)t * (size_t)H;
+    const int rc = r     ? odd ? launch_norm<T, true>(xp + at, r + at, w, n, H, eps, q + at, scale + t, st)
+                               : launch_norm<T, false>(xp + at, r + at, w, n, H, eps, q + at, scale + t, st)
+                   : odd ? launch_quant<T, true>(xp + at, n, H, q + at, scale + t, st)
+                         : launch_quant<T, false>(xp + at, n, H, q + at, scale + t, st);
+    if (rc != CEK_OK) return rc;
+  }
+  return CEK_OK;
 }
 
 }  // namespace cek
@@ -307,23 +317,23 @@ using namespace cek;
 
 extern "C" int cek_per_token_quant_int8(const void* x, int64_t rows, int64_t H, int io_dtype, int8_t* q, float* scale,
                                         void* stream) {
-  if (rows < 0 || H <= 0 || rows > INT32_MAX / 1024 || H > INT32_MAX / 2) return CEK_ERR_INVALID;
+  if (rows < 0 || H <= 0 || rows > INT32_MAX || H > INT32_MAX / 2) return CEK_ERR_INVALID;
   if (io_dtype != CEK_F16 && io_dtype != CEK_BF16) return CEK_ERR_INVALID;
   if (rows == 0) return CEK_OK;
   if (!x || !q || !scale) return CEK_ERR_INVALID;
   hipStream_t st = (hipStream_t)stream;
-  return io_dtype == CEK_F16 ? launch_rows<F16>(x, nullptr, nullptr, (int)rows, (int)H, 0.f, q, scale, st)
-                             : launch_rows<BF16>(x, nullptr, nullptr, (int)rows, (int)H, 0.f, q, scale, st);
+  return io_dtype == CEK_F16 ? launch_rows<F16>(x, nullptr, nullptr, rows, (int)H, 0.f, q, scale, st)
+                             : launch_rows<BF16>(x, nullptr, nullptr, rows, (int)H, 0.f, q, scale, st);
 }
 
 extern "C" int cek_fused_add_rms_norm_quant_int8(const void* hidden, void* residual, const void* weight, int64_t rows,
                                                  int64_t H, float eps, int io_dtype, int8_t* q, float* scale,
                                                  void* stream) {
-  if (rows < 0 || H <= 0 || rows > INT32_MAX / 1024 || H > INT32_MAX / 2) return CEK_ERR_INVALID;
+  if (rows < 0 || H <= 0 || rows > INT32_MAX || H > INT32_MAX / 2) return CEK_ERR_INVALID;
   if (io_dtype != CEK_F16 && io_dtype != CEK_BF16) return CEK_ERR_INVALID;
   if (rows == 0) return CEK_OK;
   if (!hidden || !residual || !weight || !q || !scale) return CEK_ERR_INVALID;
   hipStream_t st = (hipStream_t)stream;
-  return io_dtype == CEK_F16 ? launch_rows<F16>(hidden, residual, weight, (int)rows, (int)H, eps, q, scale, st)
-                             : launch_rows<BF16>(hidden, residual, weight, (int)rows, (int)H, eps, q, scale, st);
+  return io_dtype == CEK_F16 ? launch_rows<F16>(hidden, residual, weight, rows, (int)H, eps, q, scale, st)
+                             : launch_rows<BF16>(hidden, residual, weight, rows, (int)H, eps, q, scale, st);
 }

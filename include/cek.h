@@ -451,8 +451,8 @@ int cek_kv4_attention(const void* q, const void* cache, const int32_t* block_tab
  * cek_per_token_quant_int8: scale[t] = max(amax_t / 127, 2^-126), q[t, i] =
  * x[t, i] / scale[t] rounded to the nearest integer, ties to even (of the exact
  * quotient).  A row with a value that is not finite has scale NaN and codes 0.
- * Any rows and H (x and q 16-byte aligned and H % 8 == 0 are faster).  The rows of
- * an [N, K] weight quantise the same way, a scale per output channel.
+ * Fewer than 2^31 rows, H < 2^30 (fastest: H % 8 == 0, x 16-byte and q 8-byte
+ * aligned).  The rows of an [N, K] weight quantise the same way, a scale per channel.
  *
  * cek_fused_add_rms_norm_quant_int8: residual = Out(hidden + residual) in place,
  * then the codes and scales of residual * rsqrt(mean((hidden + residual)^2) + eps) *
@@ -461,8 +461,9 @@ int cek_kv4_attention(const void* q, const void* cache, const int32_t* block_tab
  *
  * cek_gemm_int8_a8w8: y[m, n] = Out((f32(sum_k a[m, k] b[n, k]) * sb[n]) * sa[m]),
  * the sum exact in int32.  a [M, K], b [N, K] int8 row-major, sa [M], sb [N], y [M, N]
- * out_dtype (F16|BF16).  Any M and N, K a multiple of 16 up to 131071, a and b
- * 16-byte aligned; the same values bit for bit whatever M, workspace or kernel.
+ * out_dtype (F16|BF16).  M and the rows of b up to 2^24, K a multiple of 16 up to
+ * 131071, a and b 16-byte aligned; the same values bit for bit whatever M, workspace
+ * or kernel.
  *
  * cek_gemm_int8_a8w8_glu: b [2d, K], gate rows, then up rows, sb [2d], y [M, d]:
  *   y[m, i] = Out(act(g) * u), g, u = the fp32 values above of b's rows i and d + i

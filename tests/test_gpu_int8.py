@@ -319,3 +319,84 @@ def test_tiles(ops, dev, m, n, k):
     rel = (16 + 16 * gate.abs() * torch.sigmoid(-gate)) * 2.0 ** -24      # the bound of oracle.int8.gated
     limit = f.abs() * (rel + 2.0 ** -11) + gate.abs() * up.abs() * 2.0 ** -126 + 2.0 ** -25
     assert ((z.double() - f).abs() <= limit).all()
+
+
+# ---- offsets beyond 32 bits ----------------------------------------------------------
+
+@pytest.mark.parametrize("h", [16, 9])
+def test_more_rows_than_a_launch_takes(ops, dev, h):
+    t = (1 << 21) + 5
+    x = torch.randn(t, h, generator=torch.Generator(device=dev).manual_seed(h), device=dev).half()
+    q, s = torch.full((t, h), 77, dtype=torch.int8, device=dev), torch.full((t,), math.nan, device=dev)
+    ops.esimd_per_token_quant_int8(x, q, s)
+    r = torch.zeros_like(x)
+    qn, sn = torch.full_like(q, 77), torch.full_like(s, math.nan)
+    ops.esimd_fused_add_rms_norm_quant_int8(x, r, torch.ones(h, dtype=torch.float16, device=dev), 1e-6, qn, sn)
+    assert torch.equal(r, x)
+    for lo in (0, (1 << 20) - 300, (1 << 21) - 300):                 # 600 rows about each launch's end
+        part = x[lo:lo + 600]
+        want_q, want_s = oint8.quant(part.cpu())
+        assert torch.equal(s[lo:lo + 600].cpu(), want_s) and torch.equal(q[lo:lo + 600].cpu(), want_q)
+        pq, ps, pr = torch.empty_like(q[:len(part)]), torch.empty(len(part), device=dev), torch.zeros_like(part)
+        ops.esimd_fused_add_rms_norm_quant_int8(part, pr, torch.ones(h, dtype=torch.float16, device=dev), 1e-6, pq, ps)
+        assert torch.equal(qn[lo:lo + 600], pq) and torch.equal(sn[lo:lo + 600], ps)
+    assert not torch.isnan(s).any() and not torch.isnan(sn).any()
+
+
+@pytest.mark.parametrize("t,h", [(40001, 131072), (80001, 65536)])
+def test_more_values_than_32_bits_count(ops, dev, t, h):
+    x = torch.zeros(t, h, dtype=torch.float16, device=dev)
+    ends = [0, 2 ** 31 // h, 2 ** 32 // h, 2 ** 32 // h + 1, t - 1]
+    rows = torch.randn(len(ends), h, generator=synthetic.gen(1)).half()
+    x[ends] = rows.to(dev)
+    q, s = torch.full((t, h), 77, dtype=torch.int8, device=dev), torch.empty(t, device=dev)
+    ops.esimd_per_token_quant_int8(x, q, s)
+    want_q, want_s = oint8.quant(rows)
+    assert torch.equal(q[ends].cpu(), want_q) and torch.equal(s[ends].cpu(), want_s)
+    assert s.numel() - (s == 2.0 ** -126).sum().item() == len(ends)  # the rest are rows of zeros
+    assert sum(int(part.count_nonzero()) for part in q.split(4000)) == int(want_q.count_nonzero())
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m", [1, 16, 64, 300])
+def test_weights_beyond_32_bits(ops, dev, m, gated):
+    """b of 4.6 GB: every kernel reaches its last rows."""
+    n, k = 140000, 32768
+    b = torch.empty(n, k, dtype=torch.int8, device=dev)
+    for i in range(0, n, 20000):
+        b[i:i + 20000] = torch.randint(-128, 128, (20000, k), generator=torch.Generator(device=dev).manual_seed(i), dtype=torch.int8,
+                                       device=dev)
+    a, sa = _codes(m, k, 5)
+    a, sa, sb = a.to(dev), sa.to(dev), torch.rand(n, device=dev) * 0.01
+    cols = torch.tensor([0, 1, 65535, 65536, 65537, 69999, 70000, 131071, 131072, 131073, n - 2, n - 1], device=dev)
+
+    def sums(c):
+        return a.double() @ b[c].double().t()                        # integers below 2^53: exact in any order
+    if gated:
+        cols = cols[cols < n // 2]
+        y = torch.full((m, n // 2), math.nan, dtype=torch.bfloat16, device=dev)
+        ops.esimd_gemm_int8_a8w8_glu(a, sa, b, sb, y)
+        few = torch.cat([cols, cols + n // 2])                       # the same rows alone give the same bits
+        want = torch.empty(m, len(cols), dtype=torch.bfloat16, device=dev)
+        ops.esimd_gemm_int8_a8w8_glu(a, sa, b[few].contiguous(), sb[few].contiguous(), want)
+    else:
+        y = torch.full((m, n), math.nan, dtype=torch.bfloat16, device=dev)
+        ops.esimd_gemm_int8_a8w8(a, sa, b, sb, y)
+        want = (sums(cols).float() * sb[cols] * sa[:, None]).bfloat16()
+    assert torch.equal(y[:, cols], want) and not torch.isnan(y).any()
+
+
+@pytest.mark.parametrize("m,n,k", [(20001, 120002, 32), (140000, 130, 32768)])
+def test_outputs_and_activations_beyond_32_bits(ops, dev, m, n, k):
+    g = torch.Generator(device=dev).manual_seed(m)
+    a, b = (torch.empty(rows, k, dtype=torch.int8, device=dev) for rows in (m, n))
+    for t in (a, b):
+        for part in t.split(20000):
+            part.copy_(torch.randint(-128, 128, part.shape, generator=g, dtype=torch.int8, device=dev))
+    sa, sb = torch.rand(m, device=dev) * 0.01, torch.rand(n, device=dev) * 0.01
+    y = torch.full((m, n), math.nan, dtype=torch.bfloat16, device=dev)
+    ops.esimd_gemm_int8_a8w8(a, sa, b, sb, y)
+    rows = torch.tensor([0, 8947, 8948, 17895, 17896, 65535, 65536, 131071, 131072, m - 2, m - 1], device=dev)
+    rows = rows[rows < m]
+    want = ((a[rows].double() @ b.double().t()).float() * sb * sa[rows, None]).bfloat16()
+    assert torch.equal(y[rows], want) and not any(torch.isnan(part).any() for part in y.split(4000))

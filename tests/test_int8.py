@@ -80,7 +80,7 @@ def _call(fn, base, change):
 
 GEMM = dict(a=P, sa=P, b=P, sb=P, y=P, M=4, N=8, K=64, out=0, ws=N, ws_bytes=0, stream=N)
 BAD = [*[({n: N}, INVALID) for n in ("a", "sa", "b", "sb", "y")], (dict(a=ODD), INVALID), (dict(b=ODD), INVALID),
-       (dict(M=-1), INVALID), (dict(M=2 ** 31), INVALID), (dict(N=-1), INVALID), (dict(N=2 ** 31), INVALID),
+       (dict(M=-1), INVALID), (dict(M=2 ** 31), INVALID), (dict(M=2 ** 24 + 1), INVALID), (dict(N=2 ** 24 + 1), INVALID), (dict(N=-1), INVALID), (dict(N=2 ** 31), INVALID),
        (dict(K=0), INVALID), (dict(K=-16), INVALID), (dict(K=72), INVALID), (dict(K=131072), INVALID),
        (dict(out=2), INVALID), (dict(out=-1), INVALID), (dict(ws=ODD, ws_bytes=64), INVALID), (dict(ws_bytes=-1), INVALID),
        (dict(M=0, a=N, y=N), OK), (dict(N=0, b=N), OK)]
