@@ -24,9 +24,21 @@ __global__ __launch_bounds__(256) void int8_join_kernel(const int32_t* __restric
   const float s0 = sa[m];
   if ((N & 3) == 0 && (reinterpret_cast<uintptr_t>(y) & 7) == 0 && (reinterpret_cast<uintptr_t>(sb) & 15) == 0) {
     i4 g{0, 0, 0, 0}, u{0, 0, 0, 0};
-    for (int k = 0; k < parts; ++k, p += step) {
-      g += *reinterpret_cast<const i4*>(p);
-      if constexpr (GLU) u += *reinterpret_cast<const i4*>(p + N);
+    // four parts at a time: their loads are out together, past the last they repeat it
+    for (int k = 0; k < parts; k += 4) {
+      i4 pg[4], pu[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int32_t* q = p + (size_t)min(k + j, parts - 1) * step;
+        pg[j] = *reinterpret_cast<const i4*>(q);
+        if constexpr (GLU) pu[j] = *reinterpret_cast<const i4*>(q + N);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (k + j < parts) {
+          g += pg[j];
+          if constexpr (GLU) u += pu[j];
+        }
     }
     const f4 sg = *reinterpret_cast<const f4*>(sb + n);
     f4 su = sg;
