@@ -82,6 +82,7 @@ static void check_product(const at::Tensor& a, const at::Tensor& sa, const at::T
   check_contig(y, op, "output");
   TORCH_CHECK(a.size(1) > 0 && a.size(1) % 16 == 0, op, ": K must be a positive multiple of 16");
   TORCH_CHECK(a.size(1) <= 131071, op, ": K must be at most 131071 (the sums are held in 32 bits)");
+  TORCH_CHECK(a.size(0) <= (1 << 24) && b.size(0) <= (1 << 24), op, ": a and b must have at most 2^24 rows");
   TORCH_CHECK(sa.numel() == a.size(0) && sb.numel() == b.size(0), op, ": a_scale [M] and b_scale [rows of b] required");
   TORCH_CHECK(y.numel() == a.size(0) * N, op, ": output must be [M, ", N, "]");
   for (auto* t : {&a, &sa, &b, &sb})

@@ -130,6 +130,8 @@ class GemmaDecodeLayer:
                 raise ValueError("an int8 layer needs int8 codes and fp32 scales of all four weights")
             if act_fp8:
                 raise ValueError("act_fp8 needs e4m3 weights")
+            if self.activation not in ("gelu_tanh", "silu"):
+                raise ValueError("activation must be gelu_tanh or silu")
             if not fuse_glu and self.activation != "gelu_tanh":
                 raise ValueError("fuse_glu=False has gelu_tanh alone")
             self.fuse_norm = self.fuse_tails = False

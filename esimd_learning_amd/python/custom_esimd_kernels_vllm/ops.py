@@ -393,7 +393,7 @@ def esimd_gemm_int8_a8w8(
     """output[m, n] = (sum_k a[m, k] * b[n, k]) * b_scale[n] * a_scale[m], the sum exact.
 
     a [M, K], b [N, K] int8, scales fp32 [M] and [N], output [M, N] fp16 or bf16.
-    Any M (decode steps stream the weights, prompts run MFMA tiles) and N, K a
+    M and N up to 2^24 (decode steps stream the weights, prompts run MFMA tiles), K a
     multiple of 16 up to 131071.  A row of the output does not depend on the others,
     on M or on the kernel that served the call.  Returns ``output``."""
     return _ops.esimd_gemm_int8_a8w8(a, a_scale, b, b_scale, output)

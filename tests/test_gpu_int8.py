@@ -400,3 +400,21 @@ def test_outputs_and_activations_beyond_32_bits(ops, dev, m, n, k):
     rows = rows[rows < m]
     want = ((a[rows].double() @ b.double().t()).float() * sb * sa[rows, None]).bfloat16()
     assert torch.equal(y[rows], want) and not any(torch.isnan(part).any() for part in y.split(4000))
+
+
+def test_more_rows_than_a_grid_takes(ops, dev):
+    long, one = torch.zeros((1 << 24) + 1, 16, dtype=torch.int8, device=dev), torch.zeros(2, 16, dtype=torch.int8, device=dev)
+    s, y = torch.ones(len(long), device=dev), torch.empty(2 * len(long), dtype=torch.float16, device=dev)
+    for a, b in ((long, one), (one, long)):
+        with pytest.raises(RuntimeError, match="2\\^24 rows"):
+            ops.esimd_gemm_int8_a8w8(a, s[:len(a)], b, s[:len(b)], y.view(len(a), len(b)))
+    with pytest.raises(RuntimeError, match="2\\^24 rows"):
+        ops.esimd_gemm_int8_a8w8_glu(long, s, one, s[:2], y[:len(long)].view(-1, 1))
+    a, b = long[:-1], one                                            # the most that it takes
+    a[-3:] = 7
+    b += 1
+    ops.esimd_gemm_int8_a8w8(a, s[:-1], b, s[:2], y[:2 * len(a)].view(-1, 2))
+    assert (y[:2 * len(a)].view(-1, 2)[-4:].cpu() == torch.tensor([[0.], [112.], [112.], [112.]])).all()
+    y.zero_()
+    ops.esimd_gemm_int8_a8w8(b, s[:2], a, s[:-1], y[:2 * len(a)].view(2, -1))
+    assert (y[:2 * len(a)].view(2, -1)[:, -4:].cpu() == torch.tensor([0., 112., 112., 112.])).all()

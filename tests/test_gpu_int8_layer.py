@@ -167,7 +167,7 @@ def test_refusals(dev):
     p = synthetic.gemma_layer(seed=10, fmt=torch.int8, **SMALL)
     mixed = dict(p, Wd=synthetic.gemma_layer(seed=10, **SMALL)["Wd"])
     for bad, kw in ((mixed, {}), (p, dict(act_fp8=True)), (dict(p, so=p["so"].half()), {}),
-                    (dict(p, activation="silu"), dict(fuse_glu=False))):
+                    (dict(p, activation="silu"), dict(fuse_glu=False)), (dict(p, activation="relu"), {})):
         with pytest.raises(ValueError):
             GemmaDecodeLayer(bad, 2, dev, **kw)
     with pytest.raises(ValueError):
