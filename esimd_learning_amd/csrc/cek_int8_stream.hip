@@ -333,11 +333,14 @@ static int launch_stream_g(const Int8Few& p, int rw, hipStream_t st) {
 // weight and activation bytes, and each after the first its start and end, less where two
 // share a CU (the rings of one cover the other's); no launch takes less than its start and
 // the weights at the rate HBM gives.  Fitted to 540 launches over 62 shapes (weights from
-// HBM); the pick is 1.5% above the fastest count up to 16 rows, 1% above that.
+// HBM): the pick is 1.5% above the fastest count up to 16 rows.  Above 16 the constants are
+// fitted to 66 shapes of 34 to 64 rows, 9% off, for the choice between these kernels and the
+// tiles: 0.8% above the faster of the two on average, 34% at worst (34 x 14336 x 8192: 30.6
+// us, 22.8 here).
 static int stream_plan(int64_t M, int64_t NB, int64_t K, bool glu, double* us) {
   const bool few = M <= 16;
-  const double start = few ? 2.61 : 2.91, weight = few ? 0.0234e-3 : 0.0352e-3, act = few ? 0.0103e-3 : 0.0051e-3,
-               next = few ? 5.06 : 2.90;
+  const double start = few ? 2.61 : 2.97, weight = few ? 0.0234e-3 : 0.0416e-3, act = few ? 0.0103e-3 : 0.0084e-3,
+               next = few ? 5.06 : 3.48;
   const int rows[] = {8, 12, 16, 24, 32, 40, 48, 56, 64};
   const int ar = M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : M <= 48 ? 48 : 64;
   int best = 0;
