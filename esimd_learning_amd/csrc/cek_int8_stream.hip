@@ -365,7 +365,12 @@ static bool int8_dot_takes(int64_t M, bool glu) { return M <= (glu ? 4 : 3); }
 
 bool int8_few_takes(int64_t M, int64_t NB, int64_t K, bool glu, double tile_us) {
   if (M > 64) return false;
-  if (M <= 32) return true;  // (the tiles were 2 to 40% slower throughout)
+  // Up to 32 rows only wide matrices of short rows go to the tiles: there a workgroup of the
+  // rings is mostly start and end, and a CU has several.  Rings / tiles, us: 28672 x 512 with
+  // 16 rows 7.4 / 6.2, 28672 x 1024 10.3 / 9.0 but 43008 x 1024 14.0 / 15.5; with 32 rows
+  // 21504 x 2048 13.7 / 11.8, 131072 x 2048 61 / 54, 43008 x 2048 23.4 / 23.9, 28672 x 4096
+  // 25.2 / 26.9; 16384 x 512 4.7 / 5.4.
+  if (M <= 32) return int8_dot_takes(M, glu) || NB <= 16384 || K > (M > 16 ? 2048 : 512);
   double us;
   stream_plan(M, NB, K, glu, &us);
   return us <= tile_us;

@@ -277,6 +277,8 @@ TILED = [(771, 12299, 464), (513, 13092, 464), (386, 11726, 464), (513, 9821, 46
          (66, 68, 464)]
 SPLIT = [(500, 4090, 14320), (3000, 700, 12000), (66, 5442, 4944), (71, 65, 3056), (65, 70, 4032), (1030, 1030, 16384),
          (68, 5414, 4832), (384, 5122, 13824), (1030, 4098, 14336)]
+# Few rows of a wide matrix with short rows, which the tiles take too.
+WIDE = [(4, 16390, 496), (16, 21506, 512), (17, 16390, 2032), (32, 28674, 1040), (33, 16402, 240)]
 
 
 def test_every_tile_is_tested():
@@ -287,9 +289,10 @@ def test_every_tile_is_tested():
         assert sorted(p // 16 for p in plans) == list(range(7)) and all(p % 16 == 1 for p in plans)
         plans = [plan(m, n // (1 + gated), k, gated, 1 << 40) for m, n, k in SPLIT]
         assert all(p % 16 > 1 for p in plans) and {p // 16 for p in plans} >= {0, 2, 5, 6}
+        assert all(plan(m, n // (1 + gated), k, gated, 1 << 40) % 16 == 1 for m, n, k in WIDE if not (gated and m == 4))
 
 
-@pytest.mark.parametrize("m,n,k", TILED + SPLIT)
+@pytest.mark.parametrize("m,n,k", TILED + SPLIT + WIDE)
 def test_tiles(ops, dev, m, n, k):
     """Both forms of every tile, whole and split, and without the workspace that the split takes."""
     from esimd_learning_amd import cabi
