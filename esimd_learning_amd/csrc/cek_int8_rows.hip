@@ -7,6 +7,8 @@
 // 4096 11.9 us, 4.9 TB/s; one row of 14336 2.4 us).  The maximum is taken of the values' bits
 // without their sign, which order as the values do and NaN above infinity, so that one
 // reduction also tells whether the row is finite.
+#include <type_traits>
+
 #include "cek_int8.h"
 #include "cek_rowops.h"
 
@@ -120,6 +122,15 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void int8_quant_kernel(c
   }
 }
 
+// A bf16 row's sum of squares passes fp32 where its root is 2^64 or more, far below the type's
+// largest values (fp16 rows never get there).  Such a sum is taken again of the values times
+// 2^-80, whose squares are at most 2^96 and the largest at least 2^-62, and 1 / rms is 2^-80
+// times the scaled row's.  Ordinary rows pay a comparison (within 1.5% either way, 12 shapes).
+constexpr float kFar = 0x1p-80f;
+template <typename T>
+__device__ inline bool sum_passes(float sum) { return std::is_same<T, BF16>::value && __float_as_uint(sum) == 0x7F800000u; }
+__device__ inline float far_inv(float scaled, int H, float eps) { return kFar * rsqrtf(scaled / (float)H + eps * kFar * kFar); }
+
 // Residual add + RMS norm + codes, likewise.  A value that two units hold counts once in the
 // sum of squares, and the new residual is stored behind the sum's barrier, when every
 // thread has read the old one.
@@ -131,7 +142,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void int8_norm_kernel(co
                                                                               float* __restrict__ scale) {
   constexpr int TPR = 64 * WPR;
   __shared__ uint32_t sh[WPR];
-  __shared__ float shf[WPR];
+  __shared__ float shf[WPR], shg[WPR];
   const int row = WPR == 1 ? (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6) : (int)blockIdx.x;
   if (WPR == 1 && row >= rows) return;
   const int tid = WPR == 1 ? threadIdx.x & 63 : threadIdx.x, units = (H + 7) >> 3;
@@ -162,17 +173,28 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void int8_norm_kernel(co
         rv[j] = u4{int8_pack2<T>(a[0], a[1]), int8_pack2<T>(a[2], a[3]), int8_pack2<T>(a[4], a[5]), int8_pack2<T>(a[6], a[7])};
       } else {
         rv[j] = addnorm_pass1<T>(hv[j], rv[j], ss);
-        store_unit<false>(rr + u * 8, rv[j]);
       }
     }
   }
-  const float inv = rsqrtf(block_fsum<WPR>(ss, shf) / (float)H + eps);
-  if constexpr (ODD) {
+  const float sum = block_fsum<WPR>(ss, shf);
+  float inv = rsqrtf(sum / (float)H + eps);
+  if (sum_passes<T>(sum)) {  // (the same in all of the row's threads; its values are read again)
+    float far = 0.f;
+    for (int u = tid; u < units; u += TPR) {
+      const int at = unit_at<ODD>(u, H), twice = 8 * u - at;
+      const u4 h = load_unit<ODD>(hr + at), r = load_unit<ODD>(rr + at);
 #pragma unroll
-    for (int j = 0; j < UPT; ++j) {
-      const int u = tid + j * TPR;
-      if (u < units) store_unit<true>(rr + unit_at<true>(u, H), rv[j]);
+      for (int e = 0; e < 8; ++e) {
+        const float a = (unit_f32<T>(h, e) + unit_f32<T>(r, e)) * kFar;
+        far = e < twice ? far : fmaf(a, a, far);
+      }
     }
+    inv = far_inv(block_fsum<WPR>(far, shg), H, eps);
+  }
+#pragma unroll
+  for (int j = 0; j < UPT; ++j) {
+    const int u = tid + j * TPR;
+    if (u < units) store_unit<ODD>(rr + unit_at<ODD>(u, H), rv[j]);
   }
   // the normed values are computed twice, for the maximum and for the codes: cheaper than
   // the registers that would hold them (eight a unit)
@@ -221,16 +243,19 @@ __global__ __launch_bounds__(kRowThreads) void int8_norm_any_kernel(const uint16
                                                                     uint16_t* residual,
                                                                     const uint16_t* __restrict__ weight, int H, float eps,
                                                                     int8_t* __restrict__ q, float* __restrict__ scale) {
-  __shared__ float shf[kRowThreads / 64];
+  __shared__ float shf[kRowThreads / 64], shg[kRowThreads / 64];
   __shared__ uint32_t sh[kRowThreads / 64];
   const size_t at = (size_t)blockIdx.x * H;
-  float ss = 0.f;
+  float ss = 0.f, far = 0.f;
   for (int i = threadIdx.x; i < H; i += kRowThreads) {
     const float t = T::to_f32(hidden[at + i]) + T::to_f32(residual[at + i]);
     ss = fmaf(t, t, ss);
+    far = fmaf(t * kFar, t * kFar, far);
     residual[at + i] = T::from_f32(t);  // read again below by this same thread only
   }
-  const float inv = rsqrtf(block_fsum<kRowThreads / 64>(ss, shf) / (float)H + eps);
+  const float sum = block_fsum<kRowThreads / 64>(ss, shf);
+  float inv = rsqrtf(sum / (float)H + eps);
+  if (sum_passes<T>(sum)) inv = far_inv(block_fsum<kRowThreads / 64>(far, shg), H, eps);
   auto normed = [&](int i) { return T::to_f32(residual[at + i]) * inv * T::to_f32(weight[i]); };
   uint32_t amax = 0;
   for (int i = threadIdx.x; i < H; i += kRowThreads) amax = max(amax, __float_as_uint(normed(i)) & 0x7FFFFFFF);
