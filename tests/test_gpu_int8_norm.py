@@ -72,3 +72,24 @@ def test_rows_whose_squares_pass_fp32(ops, dev, t, h):
     if t == 12:
         alone = _run(ops, dev, hid[8:9], res[8:9], w, 1e-6)
         assert all(torch.equal(x[8:9], y) for x, y in zip(got, alone))
+
+
+FORMS = [(4, 1), (4, 7), (5, 8), (5, 9), (6, 15), (7, 64), (4, 136), (9, 505), (5, 520), (6, 1000), (5, 1031), (4, 2048), (3, 2056), (4, 4093),
+         (5, 4096), (4, 4099), (3, 5120), (4, 8192), (3, 8195), (4, 16384), (3, 16390), (4, 30001), (3, 32768), (3, 32769), (3, 40000),
+         (1025, 1001), (1026, 4096), (1025, 4099), (1027, 5121), (1024, 6144), (1025, 8185)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("t,h", FORMS)
+def test_within_the_reduction(ops, dev, t, h, dtype):
+    """Ordinary rows; one whose sums all round down, so that a mean of the rounded residual is off; one whose last eight
+    values, the last unit of an odd length, outweigh the rest, so that a value counted twice shows."""
+    g = synthetic.gen(t + h)
+    hid, res = torch.randn(t, h, generator=g), torch.randn(t, h, generator=g)
+    hid[:, 3 % h::17] *= 20
+    step, sign = torch.finfo(dtype).eps, torch.randint(0, 2, (h,), generator=g) * 2.0 - 1
+    res[1 % t] = sign * (1 + step * torch.randint(0, int(1 / step), (h,), generator=g))
+    hid[1 % t] = sign * step * 0.375
+    hid[2 % t, -8:] *= 30
+    hid, res, w = hid.to(dtype), res.to(dtype), synthetic.norm_weight(h, 3, dtype)
+    _check(_run(ops, dev, hid, res, w, 1e-6), hid, res, w, 1e-6, _rel(h))
