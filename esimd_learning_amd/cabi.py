@@ -69,6 +69,7 @@ SIGNATURES = {
     "cek_fused_add_rms_norm_quant_int8": (_i, [_p, _p, _p, _i64, _i64, _f, _i, _p, _p, _p]),
     "cek_gemm_int8_a8w8_workspace_size": (_i64, [_i64, _i64, _i64]),
     "cek_gemm_int8_plan": (_i, [_i64, _i64, _i64, _i, _i64]),
+    "cek_gemm_int8_few_plan": (_i, [_i64, _i64, _i64, _i, _i64]),
     "cek_gemm_int8_a8w8": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p, _i64, _p]),
     "cek_gemm_int8_a8w8_glu_workspace_size": (_i64, [_i64, _i64, _i64]),
     "cek_gemm_int8_a8w8_glu": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _i, _p, _i64, _p]),

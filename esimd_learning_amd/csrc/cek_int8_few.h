@@ -36,6 +36,8 @@ __device__ inline int wave_isum(int v) {
 // Up to 64 rows: whether these kernels serve the product rather than tiles that would take
 // tile_us (NB: rows of b), and their launch.
 bool int8_few_takes(int64_t M, int64_t NB, int64_t K, bool glu, double tile_us);
+// Which of them serves N outputs (the codes of cek_gemm_int8_few_plan).
+int int8_few_form(int64_t M, int64_t N, int64_t K, bool glu);
 int launch_int8_few(const Int8Few& p, hipStream_t st);
 
 }  // namespace cek

@@ -209,6 +209,13 @@ extern "C" int cek_gemm_int8_plan(int64_t M, int64_t N, int64_t K, int gated, in
   return p.cfg < 0 ? -1 : 16 * p.cfg + p.parts;
 }
 
+extern "C" int cek_gemm_int8_few_plan(int64_t M, int64_t N, int64_t K, int gated, int64_t workspace_bytes) {
+  if (N > INT32_MAX) return -1;
+  const int64_t NB = gated ? 2 * N : N;
+  if (!int8_sizes_ok(M, N, K, NB) || M == 0 || N == 0) return -1;
+  return int8_plan(M, NB, K, gated != 0, workspace_bytes).cfg < 0 ? int8_few_form(M, N, K, gated != 0) : 0;
+}
+
 extern "C" int cek_gemm_int8_a8w8(const int8_t* a, const float* sa, const int8_t* b, const float* sb, void* y, int64_t M,
                                   int64_t N, int64_t K, int out_dtype, void* workspace, int64_t workspace_bytes,
                                   void* stream) {

@@ -94,10 +94,11 @@ static int launch_dot_r(const Int8Few& p, hipStream_t st) {
 // 10.46 / 10.75; N = 28672, K = 1024 7.12 / 6.56 / 6.78; N = 512, K = 16384 3.8 / 4.2 / 6.1.
 // The gated block's two outputs are four rows: one row of d = 14336 19.46 (four
 // outputs 19.46, one 21.0).
+static int dot_rows(int64_t N, int64_t K, bool glu) { return !glu && K <= 2048 && N >= 8192 ? 4 : 2; }
 template <int M>
 static int launch_dot_m(const Int8Few& p, hipStream_t st) {
   if (p.act >= 0) return launch_dot_r<M, 2, true>(p, st);
-  return p.K <= 2048 && p.N >= 8192 ? launch_dot_r<M, 4, false>(p, st) : launch_dot_r<M, 2, false>(p, st);
+  return dot_rows(p.N, p.K, false) == 4 ? launch_dot_r<M, 4, false>(p, st) : launch_dot_r<M, 2, false>(p, st);
 }
 
 static int launch_int8_dot(const Int8Few& p, hipStream_t st) {
@@ -320,13 +321,18 @@ static int launch_stream_ar(const Int8Few& p, int rw, hipStream_t st) {
   return check_launch();
 }
 
+// Rows of a that a workgroup holds.
+static int stream_rows(int64_t M) { return M <= 8 ? 8 : (int)((M + 15) / 16 * 16); }
 template <bool GLU>
 static int launch_stream_g(const Int8Few& p, int rw, hipStream_t st) {
-  if (p.M <= 8) return launch_stream_ar<8, GLU>(p, rw, st);
-  if (p.M <= 16) return launch_stream_ar<16, GLU>(p, rw, st);
-  if (p.M <= 32) return launch_stream_ar<32, GLU>(p, rw, st);
-  if (p.M <= 48) return launch_stream_ar<48, GLU>(p, rw, st);
-  return launch_stream_ar<64, GLU>(p, rw, st);
+  switch (stream_rows(p.M)) {
+    case 8: return launch_stream_ar<8, GLU>(p, rw, st);
+    case 16: return launch_stream_ar<16, GLU>(p, rw, st);
+    case 32: return launch_stream_ar<32, GLU>(p, rw, st);
+    case 48: return launch_stream_ar<48, GLU>(p, rw, st);
+    case 64: return launch_stream_ar<64, GLU>(p, rw, st);
+    default: return CEK_ERR_UNSUPPORTED;
+  }
 }
 
 // Weight rows per workgroup and the launch's time in us: a CU's workgroups cost their
@@ -342,7 +348,7 @@ static int stream_plan(int64_t M, int64_t NB, int64_t K, bool glu, double* us) {
   const double start = few ? 2.61 : 2.97, weight = few ? 0.0234e-3 : 0.0416e-3, act = few ? 0.0103e-3 : 0.0084e-3,
                next = few ? 5.06 : 3.48;
   const int rows[] = {8, 12, 16, 24, 32, 40, 48, 56, 64};
-  const int ar = M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : M <= 48 ? 48 : 64;
+  const int ar = stream_rows(M);
   int best = 0;
   for (int r : rows) {
     if (glu && r == 12) continue;
@@ -374,6 +380,12 @@ bool int8_few_takes(int64_t M, int64_t NB, int64_t K, bool glu, double tile_us) 
   double us;
   stream_plan(M, NB, K, glu, &us);
   return us <= tile_us;
+}
+
+int int8_few_form(int64_t M, int64_t N, int64_t K, bool glu) {
+  if (int8_dot_takes(M, glu)) return 16 * (int)M + dot_rows(N, K, glu);
+  double us;
+  return 256 * stream_rows(M) + stream_plan(M, glu ? 2 * N : N, K, glu, &us);
 }
 
 int launch_int8_few(const Int8Few& p, hipStream_t st) {

@@ -491,6 +491,12 @@ int cek_gemm_int8_a8w8_glu(const int8_t* a, const float* sa, const int8_t* b, co
  * the kernels for up to 64 rows serve it.
  */
 int cek_gemm_int8_plan(int64_t M, int64_t N, int64_t K, int gated, int64_t workspace_bytes);
+/*
+ * NEW, likewise: which of the kernels for up to 64 rows serves the product, 256 * rows of a +
+ * rows of b of a workgroup for the rings, 16 * M + rows of b of a thread for v_dot4 (one to
+ * four rows); 0 where tiles do, -1 for sizes that the product refuses or that are empty.
+ */
+int cek_gemm_int8_few_plan(int64_t M, int64_t N, int64_t K, int gated, int64_t workspace_bytes);
 
 /*
  * Measurement utility, no counterpart in the reference: reads `bytes` bytes
