@@ -266,35 +266,32 @@ __global__ __launch_bounds__(C::THREADS, (C::LDSB > 81920 ? 3 : 6)) void int8_st
     }
   }
 
-  // The eight waves' sums meet in LDS, GB blocks at a time: D row 4 (lane >> 4) + v of a
-  // block is row m of a, column lane & 15 the weight row.
-  constexpr int BL = MB * NT, GB0 = C::RING / (kConsumers * 1024), GB = GB0 < BL ? GB0 : BL;
-  i4* const red = reinterpret_cast<i4*>(smem);  // [8][GB][64]
+  // The eight waves' sums meet in LDS: D row 4 (lane >> 4) + v of a block is row m of a,
+  // column lane & 15 the weight row.
+  constexpr int BL = MB * NT;
+  static_assert(kConsumers * BL * 1024 <= C::RING, "the sums take the slots' place");
+  i4* const red = reinterpret_cast<i4*>(smem);  // [8][BL][64]
+  lds_barrier();  // the slots are done with
+  if (wave < kConsumers) {
 #pragma unroll
-  for (int b0 = 0; b0 < BL; b0 += GB) {
-    lds_barrier();  // the slots, or the blocks before, are done with
-    if (wave < kConsumers) {
+    for (int j = 0; j < BL; ++j) red[(wave * BL + j) * 64 + lane] = acc[j / NT][j % NT];
+  }
+  lds_barrier();
+  for (int q = threadIdx.x; q < BL * 64; q += C::THREADS) {
+    const int blk = q / 64, r = 16 * (blk % NT) + (q & 15), m0 = 16 * (blk / NT) + 4 * ((q & 63) >> 4);
+    const int n = n0 + out_of(r);
+    if (r >= C::RW || n >= p.N || m0 >= p.M || (C::GLU && (q & 4))) continue;
+    i4 c = red[q], u{0, 0, 0, 0};
+    if constexpr (C::GLU) u = red[q + 4];
 #pragma unroll
-      for (int j = 0; j < GB; ++j)
-        if (b0 + j < BL) red[(wave * GB + j) * 64 + lane] = acc[(b0 + j) / NT][(b0 + j) % NT];
+    for (int w = 1; w < kConsumers; ++w) {
+      c += red[w * BL * 64 + q];
+      if constexpr (C::GLU) u += red[w * BL * 64 + q + 4];
     }
-    lds_barrier();
-    for (int q = threadIdx.x; q < GB * 64; q += C::THREADS) {
-      const int blk = b0 + q / 64, r = 16 * (blk % NT) + (q & 15), m0 = 16 * (blk / NT) + 4 * ((q & 63) >> 4);
-      const int n = n0 + out_of(r);
-      if (blk >= BL || r >= C::RW || n >= p.N || m0 >= p.M || (C::GLU && (q & 4))) continue;
-      i4 c = red[q], u{0, 0, 0, 0};
-      if constexpr (C::GLU) u = red[q + 4];
+    const float sg = sw[r], su = C::GLU ? sw[r + 4] : 0.f;
 #pragma unroll
-      for (int w = 1; w < kConsumers; ++w) {
-        c += red[w * GB * 64 + q];
-        if constexpr (C::GLU) u += red[w * GB * 64 + q + 4];
-      }
-      const float sg = sw[r], su = C::GLU ? sw[r + 4] : 0.f;
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-        if (m0 + v < p.M) int8_store(p, m0 + v, n, c[v], u[v], sx[m0 + v], sg, su);
-    }
+    for (int v = 0; v < 4; ++v)
+      if (m0 + v < p.M) int8_store(p, m0 + v, n, c[v], u[v], sx[m0 + v], sg, su);
   }
 }
 
