@@ -107,3 +107,48 @@ def test_dot(ops, dev, gated, m, rows, n, k):
 def test_split_tiles(ops, dev, tile, parts, gated):
     m, n, k = SPLIT[tile, parts]
     _check(ops, dev, m, n // (1 + gated), k, "silu" if gated else None, torch.bfloat16 if parts % 2 else torch.float16)
+
+
+# A workspace for fewer parts than the planner would take: (rows, rows of b, K, its parts)
+SHORT = [(66, 5442, 4944, 4), (65, 70, 8208, 12), (500, 4090, 14320, 4)]
+
+
+def _rooms(m, n, k, gated):
+    """Bytes to give, and the parts that they hold at most."""
+    lib = cabi.load()
+    size = lib.cek_gemm_int8_a8w8_glu_workspace_size if gated else lib.cek_gemm_int8_a8w8_workspace_size
+    full, one = size(m, n // (1 + gated), k), 4 * m * n
+    return full, [(b, b // one) for b in (full, full - 16, full * 3 // 4, full // 2, 2 * one + 15, 2 * one - 16, 0)]
+
+
+@pytest.mark.parametrize("gated", [0, 1])
+@pytest.mark.parametrize("m,n,k,most", SHORT)
+def test_parts_fit_their_workspace(m, n, k, most, gated):
+    full, rooms = _rooms(m, n, k, gated)
+    parts = [cabi.load().cek_gemm_int8_plan(m, n // (1 + gated), k, gated, b) % 16 for b, _ in rooms]
+    assert parts[0] == most and parts[-1] == 1 and all(p <= max(1, room) for p, (_, room) in zip(parts, rooms))
+    assert any(1 < p < most for p in parts)            # less room, still a split
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [0, 1])
+@pytest.mark.parametrize("m,n,k,most", SHORT)
+def test_workspaces_that_are_too_small(dev, m, n, k, most, gated):
+    """The same bits from any workspace, and nothing written behind its end."""
+    lib = cabi.load()
+    g = torch.Generator(device=dev).manual_seed(m)
+    a, b = (torch.randint(-128, 128, (r, k), generator=g, dtype=torch.int8, device=dev) for r in (m, n))
+    sa, sb = torch.rand(m, generator=g, device=dev) * 0.01, torch.rand(n, generator=g, device=dev) * 1e-4
+    want = None
+    full, rooms = _rooms(m, n, k, gated)
+    for room, _ in reversed(rooms):
+        ws = torch.full((full + 4096,), 0x5A, dtype=torch.uint8, device=dev)
+        y = torch.full((m, n // (1 + gated)), math.nan, dtype=torch.bfloat16, device=dev)
+        ptrs = [cabi.ptr(t) for t in (a, sa, b, sb, y)]
+        if gated:
+            rc = lib.cek_gemm_int8_a8w8_glu(*ptrs, m, n // 2, k, cabi.CEK_SILU, cabi.CEK_BF16, cabi.ptr(ws), room, cabi.stream_ptr())
+        else:
+            rc = lib.cek_gemm_int8_a8w8(*ptrs, m, n, k, cabi.CEK_BF16, cabi.ptr(ws), room, cabi.stream_ptr())
+        cabi.check(rc)
+        want = y if want is None else want               # none: one part
+        assert not torch.isnan(y).any() and torch.equal(y, want) and (ws[room:] == 0x5A).all(), room
