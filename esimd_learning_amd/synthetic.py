@@ -7,7 +7,7 @@ callers move them to the GPU.
 Weight recipe (per output row n):
     W ~ N(0, 0.02) fp32;  s[n] = amax_k |W[n, k]| / 448 (fp32);
     W8 = e4m3(clamp(W / s[:, None], -448, 448))        (RNE)
-    int8: s[n] = amax / 127, W8 = W / s[:, None] to the nearest integer
+    int8: s[n] = max(amax / 127, 2^-126), W8 = W / s[:, None] to the nearest integer, ties to even
 Activations are fp16 N(0, 1); RMSNorm weights 1 + N(0, 0.1) in fp16 (already
 in the Gemma w + 1 convention); eps 1e-6; RoPE theta 10000 and positions drawn
 from [0, 8192).
@@ -25,9 +25,11 @@ def gen(seed):
 
 def quantize_rows(W, fmt=torch.float8_e4m3fn):
     """Per-row fp8 (or int8) quantisation of an fp32 [N, K] matrix -> (W8, s fp32 [N])."""
-    if fmt == torch.int8:
-        s = W.abs().amax(dim=1) / 127
-        return (W / s[:, None]).round().to(torch.int8), s.float()
+    if fmt == torch.int8:                   # as esimd_per_token_quant_int8: quotients in 64 bits, ties to even
+        s = (W.float().abs().amax(dim=1) / 127).clamp_min(2.0 ** -126)
+        bad = ~torch.isfinite(W).all(dim=1)
+        q = (W.double() / s.double()[:, None]).round()
+        return q.masked_fill(bad[:, None], 0).to(torch.int8), s.masked_fill(bad, float("nan"))
     fmax = E5M2_MAX if fmt == torch.float8_e5m2 else E4M3_MAX
     s = W.abs().amax(dim=1) / fmax
     W8 = (W / s[:, None]).clamp(-fmax, fmax).to(fmt)
