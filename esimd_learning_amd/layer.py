@@ -113,17 +113,18 @@ class GemmaDecodeLayer:
         self.qkv = mk(nqkv)
         self.attn = mk(self.nq * self.hd).zero_()   # padding rows of an attention keep this
         self.o = mk(self.hidden)
-        self.gu = mk(2 * self.mlp)
         self.act = mk(self.mlp)
         self.out = mk(self.hidden)
         self.act_fp8 = act_fp8
         self.fuse_glu = fuse_glu
         self.fuse_norm = fuse_norm and M <= 4   # the fused launch covers up to four rows
-        self.r_mid = mk(self.hidden)            # r1 between the two fused norms
         self.fuse_tails = fuse_tails and not act_fp8 and not self.fuse_norm
         self.cnt_rope = self.ops.gemv_tail_counters(self.nq, self.nk, device)
         weights = (self.Wqkv, self.Wo, self.Wgu, self.Wd)
         self.int8 = any(w.dtype == torch.int8 for w in weights)
+        # int8 layers may have many rows: no buffer that their step does not touch
+        self.gu = None if self.int8 and fuse_glu else mk(2 * self.mlp)   # both halves, unfused
+        self.r_mid = None if self.int8 else mk(self.hidden)              # r1 between the two fused norms
         self.activation = p.get("activation", "gelu_tanh")
         if self.int8:
             if any(w.dtype != torch.int8 for w in weights) or any(s.dtype != torch.float32 for s in (self.sqkv, self.so, self.sgu, self.sd)):
