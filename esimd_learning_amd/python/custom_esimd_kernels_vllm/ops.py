@@ -382,7 +382,10 @@ def esimd_fused_add_rms_norm_quant_int8(
     """residual += hidden_states (in place); int8 codes and scales of
     rmsnorm(residual) * weight into out_q [T, H] and out_scale [T], as
     esimd_per_token_quant_int8 of the normed rows before any rounding to 16
-    bits.  hidden_states is only read."""
+    bits.  hidden_states is only read.
+
+    The normed values are fp32: a code whose exact quotient lies next to a half may be
+    one off (some ten of a million; the same every time for the same call)."""
     _ops.esimd_fused_add_rms_norm_quant_int8(hidden_states, residual, weight, eps, out_q, out_scale)
 
 
@@ -403,7 +406,7 @@ def esimd_gemm_int8_a8w8_glu(
     a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
     output: torch.Tensor, activation: str = "gelu_tanh",
 ) -> None:
-    """The gated block in one launch: output[m, i] = act(g) * u, g and u the fp32
+    """The gated block in one call: output[m, i] = act(g) * u, g and u the fp32
     values that esimd_gemm_int8_a8w8 has for rows i and d + i of b [2d, K] (gate rows, then
     up rows), not rounded before the product.  activation: "gelu_tanh" or
     "silu"; output [M, d] fp16 or bf16."""

@@ -457,7 +457,16 @@ int cek_kv4_attention(const void* q, const void* cache, const int32_t* block_tab
  * cek_fused_add_rms_norm_quant_int8: residual = Out(hidden + residual) in place,
  * then the codes and scales of residual * rsqrt(mean((hidden + residual)^2) + eps) *
  * weight, which is not rounded to 16 bits before (cek_fused_add_rms_norm_quant_fp8
- * rounds it).  hidden is only read.
+ * rounds it).  hidden is only read.  The normed values are fp32, within a few units of
+ * the last place (the more the longer the row): a code whose exact quotient lies that
+ * near to a half may be the other neighbour, so implementations that sum in another
+ * order, the forms for other lengths and alignments here among them, may differ by one
+ * in some ten codes of a million; each gives the same bits every time.  Any finite
+ * values; eps at least 2^-100 for rows whose squares vanish in fp32 (bf16 values below
+ * 2^-63).
+ *
+ * Of both, outputs (residual among them) share no memory with the other arguments or
+ * each other.
  *
  * cek_gemm_int8_a8w8: y[m, n] = Out((f32(sum_k a[m, k] b[n, k]) * sb[n]) * sa[m]),
  * the sum exact in int32.  a [M, K], b [N, K] int8 row-major, sa [M], sb [N], y [M, N]
