@@ -71,8 +71,8 @@ __global__ __launch_bounds__(256) void int8_join_kernel(const int32_t* __restric
 // of a nearly empty and a full chip.  Split K adds the join and its traffic.  Fitted
 // to 730 launches over 41 shapes of 72 to 8192 rows (weights from HBM): 9% off on
 // average, and the pick 0.2% above the fastest of all tiles and splits (geometric
-// mean; 3% at worst).  Larger tiles move fewer operand bytes per product, smaller
-// ones fill the chip sooner.
+// mean; 3% at worst).  They are plain products; the gated block goes by the same constants.
+// Larger tiles move fewer operand bytes per product, smaller ones fill the chip sooner.
 struct Int8Opt {
   int bm, bn;
   double fixed, step, fixed0, step0;  // us: a full round, and one with few workgroups

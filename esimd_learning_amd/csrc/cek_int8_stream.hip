@@ -116,8 +116,9 @@ static int launch_int8_dot(const Int8Few& p, hipStream_t st) {
 // direct-to-LDS loads (1 KB: two rows x 512 bytes); eight consumer waves take 64 K
 // values of a stage's 512 each over all 16 x 16 blocks of the workgroup (AR rows of a
 // x RW of b) and meet in LDS at the end.  One barrier a stage.  Weights from HBM: 16 x 4096 x
-// 14336 13.1 us (4.5 TB/s; a read alone 9.7), 37 x 10750 x 2576 10.1, 64 x 14336 x 4096 16.7.
-// Activations straight to the consumers' registers (16 rows x 64 bytes a load) take 15.7
+// 14336 13.0 us (4.5 TB/s; a read alone 9.8), 37 x 10750 x 2576 10.0 (a read 5.6), 48 x 4096 x
+// 4096 8.1.  Beside the read it is the bytes of a that bound them: a CU loads AR rows of a
+// beside its RW rows of b.  Activations straight to the consumers' registers (16 rows x 64 bytes a load) take 15.7
 // in the place of 13.1 and 11.1 in the place of 8.3 (48 x 4096 x 4096).
 constexpr int kConsumers = 8;
 
@@ -338,8 +339,10 @@ static int launch_stream_g(const Int8Few& p, int rw, hipStream_t st) {
 // the weights at the rate HBM gives.  Fitted to 540 launches over 62 shapes (weights from
 // HBM): the pick is 1.5% above the fastest count up to 16 rows.  Above 16 the constants are
 // fitted to 66 shapes of 34 to 64 rows, 9% off, for the choice between these kernels and the
-// tiles: 0.8% above the faster of the two on average, 34% at worst (34 x 14336 x 8192: 30.6
-// us, 22.8 here).
+// tiles: 0.8% above the faster of the two on average, 40% at worst (34 x 14336 x 8192 by
+// tiles 31 to 32 us, by rings 22.4; 64 x 14336 x 4096 19.8 and 16.7).  These are plain
+// products; the gated block goes by the same constants (64 x 14336 x 4096 by tiles 29.8, by
+// rings 34.4; 40 rows 27.3 and 27.9).
 static int stream_plan(int64_t M, int64_t NB, int64_t K, bool glu, double* us) {
   const bool few = M <= 16;
   const double start = few ? 2.61 : 2.97, weight = few ? 0.0234e-3 : 0.0416e-3, act = few ? 0.0103e-3 : 0.0084e-3,
@@ -372,7 +375,9 @@ bool int8_few_takes(int64_t M, int64_t NB, int64_t K, bool glu, double tile_us) 
   // rings is mostly start and end, and a CU has several.  Rings / tiles, us: 28672 x 512 with
   // 16 rows 7.4 / 6.2, 28672 x 1024 10.3 / 9.0 but 43008 x 1024 14.0 / 15.5; with 32 rows
   // 21504 x 2048 13.7 / 11.8, 131072 x 2048 61 / 54, 43008 x 2048 23.4 / 23.9, 28672 x 4096
-  // 25.2 / 26.9; 16384 x 512 4.7 / 5.4.
+  // 25.2 / 26.9; 16384 x 512 4.7 / 5.4.  No limit in K alone is right for all of these: up to
+  // 16 rows this one gives K = 1024 to the rings, which costs 28672 and 131072 wide matrices
+  // 5 to 14%, and from 17 rows K = 2048 to the tiles, which costs 43008 wide ones 2 to 7%.
   if (M <= 32) return int8_dot_takes(M, glu) || NB <= 16384 || K > (M > 16 ? 2048 : 512);
   double us;
   stream_plan(M, NB, K, glu, &us);

@@ -12,8 +12,8 @@
 // from its L2, but in 38 to 45 where the lines come from HBM, whatever their depth, row
 // pitch or sharing (touching them ahead of the loads made every shape 5 to 10% slower).
 // A launch's fixed part is 7 to 15 us: its first slots 2.4, the epilogue 4 to 6, the burst
-// of all CUs' outputs.  4096 x 28672 x 4096 369 us, 2610 TOPS; 2048 x 6144 x 4096 43 to 46
-// us, 2300; 512 x 4096 x 14336 41 us (split, with its join 7).
+// of all CUs' outputs.  4096 x 28672 x 4096 369 to 380 us, 2530 to 2610 TOPS; 2048 x 6144 x
+// 4096 43 to 46 us, 2300; 512 x 4096 x 14336 41 us (split, with its join 7).
 #pragma once
 
 #include "cek_int8.h"
