@@ -4,9 +4,9 @@
 // A row is read once and stays in registers between its maximum (or its sum of
 // squares and its maximum) and its codes.  What bounds the kernels: for many rows HBM,
 // for few the chain load, reduction, store (28672 x 4096 59 us, 6.0 TB/s; norm of 2048 x
-// 4096 from HBM 13.9 us, 4.2 TB/s; one row of 14336 2.4 us).  The maximum is taken of the values' bits
-// without their sign, which order as the values do and NaN above infinity, so that one
-// reduction also tells whether the row is finite.
+// 4096 from HBM 13.9 us, 4.2 TB/s; one row of 14336 2.4 us).  The maximum is taken of the
+// values' bits without their sign, which order as the values do and NaN above infinity, so
+// that one reduction also tells whether the row is finite.
 #include <type_traits>
 
 #include "cek_int8.h"

@@ -118,8 +118,8 @@ static int launch_int8_dot(const Int8Few& p, hipStream_t st) {
 // x RW of b) and meet in LDS at the end.  One barrier a stage.  Weights from HBM: 16 x 4096 x
 // 14336 13.0 us (4.5 TB/s; a read alone 9.8), 37 x 10750 x 2576 10.0 (a read 5.6), 48 x 4096 x
 // 4096 8.1.  Beside the read it is the bytes of a that bound them: a CU loads AR rows of a
-// beside its RW rows of b.  Activations straight to the consumers' registers (16 rows x 64 bytes a load) take 15.7
-// in the place of 13.1 and 11.1 in the place of 8.3 (48 x 4096 x 4096).
+// beside its RW rows of b.  Activations straight to the consumers' registers (16 rows x 64
+// bytes a load) take 15.7 in the place of 13.1 and 11.1 in the place of 8.3.
 constexpr int kConsumers = 8;
 
 template <int AR_, int RW_, bool GLU_>

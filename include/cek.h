@@ -461,8 +461,8 @@ int cek_kv4_attention(const void* q, const void* cache, const int32_t* block_tab
  * the last place (the more the longer the row): a code whose exact quotient lies that
  * near to a half may be the other neighbour, so implementations that sum in another
  * order, the forms for other lengths and alignments here among them, may differ by one
- * in some ten codes of a million; each gives the same bits every time.  Any finite
- * values; eps at least 2^-100 for rows whose squares vanish in fp32 (bf16 values below
+ * in some ten codes of a million; each gives the same bits every time.  Any values
+ * whose sums are finite in the type; eps at least 2^-100 for rows whose squares vanish in fp32 (bf16 values below
  * 2^-63).
  *
  * Of both, outputs (residual among them) share no memory with the other arguments or
