@@ -75,9 +75,9 @@ product takes int8 codes and a scale per token,
 
 with act = params["activation"], "gelu_tanh" (the default) or "silu"; layers of fp8 weights have gelu_tanh
 alone and refuse params that name another.  torch.int8 means these codes: e4m3 bytes are held as
-torch.float8_e4m3fn (or uint8).  hidden is only read; ``fuse_glu=False`` runs gate/up as one product into [M, 2d] and esimd_gelu_and_mul (gelu_tanh
-only), which rounds both halves in between; the other ``fuse_`` options and
-``defer_norm`` have no int8 form and are off.
+torch.float8_e4m3fn (or uint8).  hidden is only read; ``fuse_glu=False`` runs gate/up as one product into
+[M, 2d] and esimd_gelu_and_mul (gelu_tanh only), which rounds both halves in between; the other ``fuse_``
+options and ``defer_norm`` have no int8 form and are off.
 
 The intermediate buffers and counters are allocated once in the
 constructor, so at decode sizes a step enqueues only kernels: it can be

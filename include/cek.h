@@ -462,8 +462,8 @@ int cek_kv4_attention(const void* q, const void* cache, const int32_t* block_tab
  * near to a half may be the other neighbour, so implementations that sum in another
  * order, the forms for other lengths and alignments here among them, may differ by one
  * in some ten codes of a million; each gives the same bits every time.  Any values
- * whose sums are finite in the type; eps at least 2^-100 for rows whose squares vanish in fp32 (bf16 values below
- * 2^-63).
+ * whose sums are finite in the type; eps at least 2^-100 for rows whose squares vanish in
+ * fp32 (bf16 values below 2^-63).
  *
  * Of both, outputs (residual among them) share no memory with the other arguments or
  * each other.
@@ -481,9 +481,8 @@ int cek_kv4_attention(const void* q, const void* cache, const int32_t* block_tab
  *
  * y shares no memory with the operands.  workspace: the bytes that the
  * _workspace_size of the same sizes gives (0: none needed), 16-byte aligned, no
- * initialisation.  With less the call splits K into as many parts as there is room for and
- * still writes what it was given; only with none (NULL) or too little for two parts it does
- * not split.  Nothing past workspace_bytes is written.  Calls that may overlap in time need
+ * initialisation.  With less the call splits K into fewer parts, which it still writes
+ * there; only with none (NULL) or too little for two parts it does not split.  Nothing past workspace_bytes is written.  Calls that may overlap in time need
  * their own.
  */
 int cek_per_token_quant_int8(const void* x, int64_t rows, int64_t H, int io_dtype, int8_t* q, float* scale, void* stream);
