@@ -482,8 +482,8 @@ int cek_kv4_attention(const void* q, const void* cache, const int32_t* block_tab
  * y shares no memory with the operands.  workspace: the bytes that the
  * _workspace_size of the same sizes gives (0: none needed), 16-byte aligned, no
  * initialisation.  With less the call splits K into fewer parts, which it still writes
- * there; only with none (NULL) or too little for two parts it does not split.  Nothing past workspace_bytes is written.  Calls that may overlap in time need
- * their own.
+ * there; only with none (NULL) or too little for two parts it does not split.  Nothing past
+ * workspace_bytes is written.  Calls that may overlap in time need their own.
  */
 int cek_per_token_quant_int8(const void* x, int64_t rows, int64_t H, int io_dtype, int8_t* q, float* scale, void* stream);
 int cek_fused_add_rms_norm_quant_int8(const void* hidden, void* residual, const void* weight, int64_t rows, int64_t H,
